@@ -32,6 +32,11 @@ TILE_VARIANTS = {"cta128x256": 1, "cta128x128": 2, "swap16": 3, "swap64": 4, "pa
                  "swap16k4": 6, "swap64k2": 7, "rowblock64": 8, "rowblock128": 9, "rowblock256": 10,
                  "swap16fp8": 11, "swap64fp8": 12, "hslice16": 13}
 WEIGHT_FORMATS = {"native": 0, "fp8": 1}
+IDENTITY = 4  # activation of the dense projection only (no hidden layer)
+LINEAR_TILES = {}  # tile families of the dense projection (None = automatic)
+MAX_EXPERTS = 512
+MAX_TOP_K = 32
+MOE_MAX_TOKENS = 256
 # Element type of the partial tiles the fused reduce-scatter sends between GPUs.
 PARTIAL_TYPES = {"fp32": 0, "input": 1, "fp24": 2}
 L2_POLICIES = {"none": 1, "stream_b": 2, "normal": 3, "keep_a": 4}
@@ -49,7 +54,11 @@ EXPORTED = ("ffn_b200_abi_version", "ffn_b200_strerror", "ffn_b200_device_info",
             "ffn_b200_set_owner_map", "ffn_b200_get_owner_map", "ffn_b200_quantize_fp8_rows", "ffn_b200_get_plan", "ffn_b200_swiglu_rows",
             "ffn_b200_destroy", "ffn_b200_launch", "ffn_b200_run_noalloc", "ffn_b200_peer_alloc",
             "ffn_b200_peer_open", "ffn_b200_peer_close", "ffn_b200_peer_free", "ffn_b200_reduce_scatter_bytes",
-            "ffn_b200_set_reduce_scatter")
+            "ffn_b200_set_reduce_scatter",
+            "ffn_b200_linear_make_plan", "ffn_b200_linear_prepare", "ffn_b200_linear_run", "ffn_b200_linear_destroy",
+            "ffn_b200_router_scratch", "ffn_b200_router_run",
+            "ffn_b200_moe_make_plan", "ffn_b200_moe_prepare", "ffn_b200_moe_run", "ffn_b200_moe_reset",
+            "ffn_b200_moe_set_wait_limit", "ffn_b200_moe_set_fault_injection", "ffn_b200_moe_destroy")
 
 
 class Problem(ctypes.Structure):
@@ -94,6 +103,40 @@ class Buffers(ctypes.Structure):
                 ("status", ctypes.c_void_p),
                 ("w1_scale", ctypes.c_void_p), ("w2_scale", ctypes.c_void_p),
                 ("bias1", ctypes.c_void_p), ("bias2", ctypes.c_void_p)]
+
+
+class LinearProblem(ctypes.Structure):
+    _fields_ = [("m", ctypes.c_int64), ("k", ctypes.c_int64), ("n", ctypes.c_int64)] + [
+        (name, ctypes.c_int32) for name in ("dtype", "activation", "block_num", "sm_count", "tile", "reserved")]
+
+
+class LinearPlan(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("tile", "tile_m", "tile_n", "stages", "block_num", "split")] + [
+        (name, ctypes.c_int64) for name in ("smem_bytes", "workspace_floats", "counter_words")]
+
+
+class RouterProblem(ctypes.Structure):
+    _fields_ = [("m", ctypes.c_int64), ("k", ctypes.c_int64)] + [
+        (name, ctypes.c_int32) for name in ("experts", "top_k", "dtype", "weight_f32", "sigmoid", "renormalize")] + [
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class MoeProblem(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int64) for name in ("m", "k", "h", "n")] + [
+        (name, ctypes.c_int32) for name in ("experts", "top_k", "dtype", "activation", "block_num", "sm_count")]
+
+
+class MoePlan(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("block_num", "stages", "chunk", "reserved")] + [
+        (name, ctypes.c_int64) for name in ("smem_bytes", "hidden_rows", "hidden_pitch", "workspace_floats",
+                                            "counter_words", "status_words")]
+
+
+class MoeBuffers(ctypes.Structure):
+    _fields_ = [("w1", ctypes.c_void_p), ("ldw1", ctypes.c_int64), ("stride1", ctypes.c_int64),
+                ("w2", ctypes.c_void_p), ("ldw2", ctypes.c_int64), ("stride2", ctypes.c_int64),
+                ("hidden", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("counters", ctypes.c_void_p),
+                ("status", ctypes.c_void_p)]
 
 
 _lock = threading.Lock()
@@ -148,6 +191,21 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
             "ffn_b200_peer_free": ([vp], i32),
             "ffn_b200_reduce_scatter_bytes": ([vp, i32, i32, ctypes.POINTER(u64), ctypes.POINTER(u64)], i32),
             "ffn_b200_set_reduce_scatter": ([vp, i32, i32, i32, ctypes.POINTER(vp), ctypes.POINTER(vp), vp, i64], i32),
+            "ffn_b200_linear_make_plan": ([ctypes.POINTER(LinearProblem), ctypes.POINTER(LinearPlan)], i32),
+            "ffn_b200_linear_prepare": ([ctypes.POINTER(LinearProblem), vp, i64, vp, vp, vp, i32, ctypes.POINTER(vp)],
+                                        i32),
+            "ffn_b200_linear_run": ([vp, vp, i64, vp, i64, vp, i64, vp], i32),
+            "ffn_b200_linear_destroy": ([vp], i32),
+            "ffn_b200_router_scratch": ([ctypes.POINTER(RouterProblem), ctypes.POINTER(i64), ctypes.POINTER(i64)], i32),
+            "ffn_b200_router_run": ([vp, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp], i32),
+            "ffn_b200_moe_make_plan": ([ctypes.POINTER(MoeProblem), ctypes.POINTER(MoePlan)], i32),
+            "ffn_b200_moe_prepare": ([ctypes.POINTER(MoeProblem), ctypes.POINTER(MoeBuffers), i32, ctypes.POINTER(vp)],
+                                     i32),
+            "ffn_b200_moe_run": ([vp, vp, i64, vp, vp, vp, i64, vp, i64, vp], i32),
+            "ffn_b200_moe_reset": ([vp, vp], i32),
+            "ffn_b200_moe_set_wait_limit": ([vp, u64], i32),
+            "ffn_b200_moe_set_fault_injection": ([vp, i32], i32),
+            "ffn_b200_moe_destroy": ([vp], i32),
         }
         for name, (args, res) in sigs.items():
             fn = getattr(lib, name)

@@ -8,9 +8,11 @@ from __future__ import annotations
 
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -18,8 +20,10 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libffn_b200.so"
-SOURCES = [CSRC / "ffn_capi.cu", CSRC / "ffn_noalloc.cu", CSRC / "ffn_placement.cu", CSRC / "ffn_quant.cu"]
-HEADERS = [CSRC / "ffn_kernel.cuh", CSRC / "ffn_rowblock.cuh", CSRC / "ffn_hslice.cuh", ROOT / "include" / "ffn_b200.h"]
+SOURCES = [CSRC / "ffn_capi.cu", CSRC / "ffn_noalloc.cu", CSRC / "ffn_placement.cu", CSRC / "ffn_quant.cu",
+           CSRC / "ffn_layers.cu"]
+HEADERS = [CSRC / "ffn_kernel.cuh", CSRC / "ffn_rowblock.cuh", CSRC / "ffn_hslice.cuh", CSRC / "layers_simple.cuh",
+           ROOT / "include" / "ffn_b200.h"]
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
 
 
@@ -45,22 +49,51 @@ def up_to_date() -> bool:
     return LIB.exists() and stamp_path().exists() and stamp_path().read_text().strip() == source_digest()
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if its sources changed; returns the library path."""
-    if not force and up_to_date():
-        return LIB
-    LIBDIR.mkdir(exist_ok=True)
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [nvcc(), ARCH, "-O3", "-lineinfo", "-std=c++17", "--shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "-Xptxas", "-v" if verbose else "-O3",
-           "-I", str(ROOT / "include"), "-o", str(tmp)] + [str(s) for s in SOURCES]
+def _included(path: Path, seen: set) -> set:
+    """``path`` and the in-tree files it includes, transitively."""
+    if path not in seen:
+        seen.add(path)
+        for name in re.findall(r'^#include "([^"]+)"', path.read_text(), re.M):
+            _included((path.parent / name).resolve(), seen)
+    return seen
+
+
+def _compile(source: Path, force: bool, verbose: bool) -> Path:
+    """The object file of one source, compiled if it or a file it includes changed."""
+    obj = LIBDIR / (source.stem + ".o")
+    stamp = LIBDIR / (source.stem + ".o.sha256")
+    h = hashlib.sha256()
+    for path in sorted(_included(source.resolve(), set())):
+        h.update(path.read_bytes())
+    digest = h.hexdigest()
+    if not force and obj.exists() and stamp.exists() and stamp.read_text().strip() == digest:
+        return obj
     # -fvisibility=hidden keeps the template kernels private; the extern "C" API is exported
     # through the FFN_B200_EXPORT default-visibility attribute in the header.
+    cmd = [nvcc(), ARCH, "-O3", "-lineinfo", "-std=c++17", "-c", "-Xcompiler", "-fPIC",
+           "-Xcompiler", "-fvisibility=hidden", "-Xptxas", "-v" if verbose else "-O3",
+           "-I", str(ROOT / "include"), "-o", str(obj), str(source)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
     if verbose:
         sys.stderr.write(res.stdout + res.stderr)
+    stamp.write_text(digest + "\n")
+    return obj
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the library if its sources changed; returns the library path."""
+    if not force and up_to_date():
+        return LIB
+    LIBDIR.mkdir(exist_ok=True)
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        objects = list(pool.map(lambda src: _compile(src, force, verbose), SOURCES))
+    tmp = LIB.with_suffix(".so.tmp")
+    cmd = [nvcc(), ARCH, "--shared", "-o", str(tmp)] + [str(o) for o in objects]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
     tmp.replace(LIB)
     stamp_path().write_text(source_digest() + "\n")
     return LIB

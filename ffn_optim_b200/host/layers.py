@@ -1,0 +1,195 @@
+"""Argument checks and storage shared by the dense projection, the router and the
+mixture-of-experts layer (the same rules as :mod:`.inputs`: fp16/bf16, rank 2-8 inputs with the
+features last, dense strided CUDA tensors, no autograd, no fallback)."""
+from __future__ import annotations
+
+from math import prod
+
+from .inputs import _packed, pitch_of
+
+MAX_DIM = 65535
+MAX_ROWS = 2**31 - 16
+
+
+def check_input(x, name="x"):
+    """Rank, dtype, device and autograd rules of an activation tensor; returns (rows, features)."""
+    import torch
+
+    check_tensor(x, name)
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{name}: dtype must be float16 or bfloat16")
+    if not 2 <= x.dim() <= 8:
+        raise ValueError(f"{name}: unsupported rank {x.dim()}")
+    if any(d <= 0 for d in x.shape):
+        raise ValueError(f"{name}: dimensions must be positive")
+    m = prod(x.shape[:-1])
+    if m > MAX_ROWS:
+        raise ValueError(f"{name}: more than {MAX_ROWS} rows")
+    return m, x.shape[-1]
+
+
+def check_tensor(t, name):
+    import torch
+
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.layout != torch.strided:
+        raise ValueError(f"{name}: only dense strided tensors are supported")
+    if t.requires_grad:
+        raise ValueError(f"{name}: inference-only operator; detach inputs explicitly")
+
+
+def check_like(t, x, shape, name, dtype=None):
+    """An operand of the given shape on x's device, of ``dtype`` (x's dtype by default)."""
+    check_tensor(t, name)
+    want = dtype or x.dtype
+    if t.dtype != want or t.device != x.device or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be a {list(shape)} tensor of {want} on {x.device}")
+
+
+def require_cuda(x, what):
+    """CUDA tensors only, checked after the shapes so that a wrong call fails alike everywhere."""
+    if x.device.type != "cuda":
+        raise ValueError(f"{what} requires CUDA tensors; no CPU fallback is used")
+
+
+def addressable(t, rows, cols):
+    """True when ``t`` is a [rows, cols] view whose rows the kernels can read in place: unit
+    column stride, 16-byte base and row pitch (the pitch of a single row is never used)."""
+    if t.dim() != 2 or t.stride(1) != 1 and cols > 1 or t.data_ptr() & 15:
+        return False
+    ld = t.stride(0)
+    return rows == 1 or ld % 8 == 0 and ld >= cols
+
+
+def row_pitch(t, rows, cols):
+    return t.stride(0) if rows > 1 else pitch_of(cols)
+
+
+def packed_weight(w):
+    """A weight [..., rows, cols] the kernels can read in place: ``w`` itself when its rows are
+    addressable and its leading strides are multiples of 8 elements, else a copy with padded rows."""
+    import torch
+
+    cols = w.shape[-1]
+    lead = [w.stride(d) for d in range(w.dim() - 1) if w.shape[d] > 1]
+    if ((w.stride(-1) == 1 or cols == 1) and w.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= cols for s in lead)):
+        return w
+    buf = torch.zeros((*w.shape[:-1], pitch_of(cols)), dtype=w.dtype, device=w.device)
+    buf[..., :cols].copy_(w)
+    return buf[..., :cols]
+
+
+class RowStorage:
+    """Where a prepared operator reads a [rows, cols] operand from: the caller's tensor when its
+    rows are addressable, else a copy in storage owned by the operator."""
+
+    def __init__(self, rows, cols, like, shape):
+        import torch
+
+        self.rows, self.cols, self.shape = rows, cols, tuple(shape)
+        self.dtype, self.device = like.dtype, like.device
+        self._torch = torch
+        self._buf = None
+
+    def bind(self, t, name, out):
+        """(address, row pitch, the tensor that must stay alive); ``out`` is the output buffer a
+        kernel run writes, which an operand may not overlap: such a view is copied first."""
+        if t.shape != self.shape or t.dtype != self.dtype or t.device != self.device:
+            raise ValueError(f"{name} must have the prepared shape, dtype and device")
+        if t.requires_grad:
+            raise ValueError(f"{name}: inference-only operator; detach inputs explicitly")
+        rows, cols = self.rows, self.cols
+        flat = t if t.dim() == 2 else t.reshape(rows, cols)
+        ptr = flat.data_ptr()
+        if addressable(flat, rows, cols) and not out[0] <= ptr < out[1]:
+            return ptr, row_pitch(flat, rows, cols), flat
+        if self._buf is None:
+            self._buf = _packed(flat, rows, cols)
+        else:
+            self._buf[:, :cols].copy_(flat)
+        return self._buf.data_ptr(), self._buf.stride(0), self._buf
+
+
+def output_buffer(rows, cols, like):
+    """[rows, pitch] output storage and its address range."""
+    import torch
+
+    out = torch.empty((rows, pitch_of(cols)), dtype=like.dtype, device=like.device)
+    return out, (out.data_ptr(), out.data_ptr() + out.numel() * out.element_size())
+
+
+def load_library():
+    from .. import _lib
+    from ..api import KernelCompilationError
+
+    try:
+        return _lib.load()
+    except (OSError, RuntimeError) as exc:
+        raise KernelCompilationError(f"{type(exc).__name__}: {exc}") from exc
+
+
+def check_target(x):
+    """SM count of x's device, which must be a B200."""
+    import torch
+
+    props = torch.cuda.get_device_properties(x.device)
+    if (props.major, props.minor) != (10, 0):
+        raise RuntimeError("This implementation targets B200 (sm_100) only")
+    return props.multi_processor_count
+
+
+def check_block_num(block_num):
+    if block_num is not None and (type(block_num) is not int or not 1 <= block_num <= MAX_DIM):
+        raise ValueError("block_num must be a positive integer; hardware limit checked before launch")
+
+
+def raise_for(rc, what):
+    """The Python exception of a C status (as prepare_ffn maps them)."""
+    from .. import _lib
+    from ..api import KernelCompilationError
+
+    if rc == _lib.OK:
+        return
+    msg = f"{what}: {_lib.strerror(rc)}"
+    if rc in (_lib.ERR_INVALID, _lib.ERR_ALIGNMENT, _lib.ERR_TOO_LARGE):
+        raise ValueError(msg)
+    if rc == _lib.ERR_DEVICE:
+        raise RuntimeError(msg)
+    raise KernelCompilationError(msg)
+
+
+class PreparedLayer:
+    """What the prepared operators share: the preparation stream, the reused output and graph
+    capture.  Subclasses launch in ``_launch(stream_pointer, ...)``."""
+
+    def _open(self, device):
+        import torch
+
+        self._torch = torch
+        self.device = device
+        with torch.cuda.device(device):
+            self.stream = torch.cuda.current_stream()
+        self._stream_ptr = self.stream.cuda_stream
+
+    def _check_stream(self):
+        if self._torch.cuda.current_stream(self.device).cuda_stream != self._stream_ptr:
+            raise RuntimeError(f"{type(self).__name__} must run on its preparation stream; "
+                               "concurrent reuse is unsupported")
+
+    def capture_graph(self, runs=1):
+        """Captures ``runs`` launches on the prepared inputs into a ``torch.cuda.CUDAGraph``.
+
+        ``graph.replay()`` on the preparation stream then re-runs them: each reads the tensors
+        given at preparation (fill them in place) and writes the output view.  Replays and eager
+        runs may alternate; like runs, they must not overlap each other."""
+        torch = self._torch
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.device(self.device):
+            side = torch.cuda.Stream()
+            side.wait_stream(self.stream)
+            with torch.cuda.graph(graph, stream=side):
+                for _ in range(runs):
+                    self._capture(side.cuda_stream)
+            self.stream.wait_stream(side)
+        return graph

@@ -72,7 +72,8 @@ typedef enum {
  * followed by the matching 64 up rows (zero rows pad the last block); with swap_ab == 1, gate
  * row i at row 2i and up row i at row 2i + 1.  W1 is then not a Linear weight of shape [h, K]:
  * plan first, pack, then prepare (ffn_optim_b200.prepare_ffn does this). */
-typedef enum { FFN_B200_GELU_RATIONAL = 0, FFN_B200_GELU_ERF = 1, FFN_B200_SILU = 2, FFN_B200_SWIGLU = 3 } ffn_b200_gelu;
+typedef enum { FFN_B200_GELU_RATIONAL = 0, FFN_B200_GELU_ERF = 1, FFN_B200_SILU = 2, FFN_B200_SWIGLU = 3,
+               FFN_B200_IDENTITY = 4 /* ffn_b200_linear_* only */ } ffn_b200_gelu;
 
 /* Weight storage: the input dtype, or fp8 e4m3 codes with one fp32 scale per row
  * (W[r, c] = code[r, c] * scale[r]; see ffn_b200_quantize_fp8_rows).  fp8 weights are
@@ -321,6 +322,128 @@ FFN_B200_EXPORT int ffn_b200_run_noalloc(const ffn_b200_problem* problem, const 
 /* One-shot: prepare, clear the scratch words, run once, release the handle. */
 FFN_B200_EXPORT int ffn_b200_launch(const ffn_b200_problem* problem, const ffn_b200_buffers* buffers,
                     void* stream);
+
+/* ---- Dense projection --------------------------------------------------------------------
+ *     Y = act(X . W^T + bias) + residual
+ * X [M, K], W [N, K], bias [N], residual and Y [M, N], all of one 16-bit dtype; sums, bias,
+ * activation and residual in fp32, one rounding at the end.  No reference counterpart. */
+typedef struct {
+  int64_t m, k, n;
+  int32_t dtype;       /* ffn_b200_dtype */
+  int32_t activation;  /* ffn_b200_gelu except FFN_B200_SWIGLU */
+  int32_t block_num;   /* CTA count at most; 0 = one per SM */
+  int32_t sm_count;    /* SMs of the target device; 0 = query the current device */
+  int32_t tile;        /* ffn_b200_linear_tile; 0 = automatic */
+  int32_t reserved;    /* 0 */
+} ffn_b200_linear_problem;
+
+typedef struct {
+  int32_t tile;        /* the tile family chosen */
+  int32_t tile_m, tile_n, stages;
+  int32_t block_num;   /* CTAs launched */
+  int32_t split;       /* CTAs that share one tile's K range, at most */
+  int64_t smem_bytes;
+  int64_t workspace_floats;
+  int64_t counter_words;
+} ffn_b200_linear_plan;
+
+typedef struct ffn_b200_linear ffn_b200_linear;
+
+FFN_B200_EXPORT int ffn_b200_linear_make_plan(const ffn_b200_linear_problem* problem, ffn_b200_linear_plan* plan);
+/* Binds the weight (and bias, or NULL) and the scratch of the planned sizes (counters zeroed).
+ * Row pitches in elements, multiples of 8; bases 16-byte aligned. */
+FFN_B200_EXPORT int ffn_b200_linear_prepare(const ffn_b200_linear_problem* problem, const void* w, int64_t ldw,
+                                            const void* bias, float* workspace, uint32_t* counters, int device,
+                                            ffn_b200_linear** handle);
+/* One asynchronous launch on `stream`; `residual` may be NULL.  Y must not overlap X or the
+ * residual.  Runs of one handle must be serialised on one stream (they share its scratch). */
+FFN_B200_EXPORT int ffn_b200_linear_run(ffn_b200_linear* handle, const void* x, int64_t ldx, const void* residual,
+                                        int64_t ldr, void* y, int64_t ldy, void* stream);
+FFN_B200_EXPORT int ffn_b200_linear_destroy(ffn_b200_linear* handle);
+
+/* ---- Expert router ------------------------------------------------------------------------
+ *     p = softmax(X . W^T) or sigmoid(X . W^T);  ids = the top_k experts by p + choice_bias;
+ *     weights = p[ids] (divided by their sum when `renormalize`) * scale
+ * Logits and scores are 64-bit, so that the choice does not depend on a summation order; equal
+ * keys go to the lower index, a NaN key ranks below every other.  A token whose mask byte is 0
+ * gets ids -1 and weights 0. */
+typedef struct {
+  int64_t m, k;
+  int32_t experts;     /* at most FFN_B200_MAX_EXPERTS */
+  int32_t top_k;       /* at most FFN_B200_MAX_TOP_K, and experts */
+  int32_t dtype;       /* ffn_b200_dtype of X */
+  int32_t weight_f32;  /* 1: W is fp32, 0: W is of X's dtype */
+  int32_t sigmoid;     /* 0 softmax, 1 sigmoid */
+  int32_t renormalize;
+  float scale;
+  int32_t reserved;    /* 0 */
+} ffn_b200_router_problem;
+
+#define FFN_B200_MAX_EXPERTS 512
+#define FFN_B200_MAX_TOP_K 32
+
+/* Scratch of one run: fp64 logits and u32 counters (zeroed before the first run). */
+FFN_B200_EXPORT int ffn_b200_router_scratch(const ffn_b200_router_problem* problem, int64_t* logit_doubles,
+                                            int64_t* counter_words);
+/* One asynchronous launch on `stream` of the current device.  choice_bias (fp32 [experts]) and
+ * mask (u8 [M]) may be NULL; ids int32 [M, top_k], weights fp32 [M, top_k]. */
+FFN_B200_EXPORT int ffn_b200_router_run(const ffn_b200_router_problem* problem, const void* x, int64_t ldx,
+                                        const void* w, int64_t ldw, const float* choice_bias, const uint8_t* mask,
+                                        int32_t* ids, float* weights, double* logits, uint32_t* counters,
+                                        void* stream);
+
+/* ---- Mixture-of-experts layer for a few tokens ----------------------------------------------
+ *     Y_t = residual_t + sum_j weights[t, j] * (act(X_t . W1_e^T) . W2_e^T),  e = ids[t, j]
+ * X [M, K], W1 [E, H, K] (SwiGLU: [E, 2H, K], gate rows then up rows), W2 [E, N, H]; M at most
+ * FFN_B200_MOE_MAX_TOKENS.  hidden is rounded once to the dtype, all sums are fp32 in a fixed
+ * order.  An id outside [0, experts) contributes nothing. */
+typedef struct {
+  int64_t m, k, h, n;
+  int32_t experts, top_k;
+  int32_t dtype;       /* ffn_b200_dtype */
+  int32_t activation;  /* ffn_b200_gelu except FFN_B200_IDENTITY */
+  int32_t block_num;   /* CTA count; 0 = one per SM */
+  int32_t sm_count;    /* SMs of the target device; 0 = query the current device */
+} ffn_b200_moe_problem;
+
+#define FFN_B200_MOE_MAX_TOKENS 256
+
+typedef struct {
+  int32_t block_num, stages;
+  int32_t chunk;       /* tokens of one expert computed together, at most */
+  int32_t reserved;
+  int64_t smem_bytes;
+  int64_t hidden_rows, hidden_pitch;  /* hidden scratch, elements of the dtype */
+  int64_t workspace_floats;
+  int64_t counter_words;
+  int64_t status_words;
+} ffn_b200_moe_plan;
+
+typedef struct {
+  const void* w1; int64_t ldw1, stride1;  /* row and expert pitches in elements */
+  const void* w2; int64_t ldw2, stride2;
+  void* hidden;
+  float* workspace;
+  uint32_t* counters;                     /* zeroed before the first run */
+  int32_t* status;                        /* zeroed before the first run */
+} ffn_b200_moe_buffers;
+
+typedef struct ffn_b200_moe ffn_b200_moe;
+
+FFN_B200_EXPORT int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* problem, ffn_b200_moe_plan* plan);
+FFN_B200_EXPORT int ffn_b200_moe_prepare(const ffn_b200_moe_problem* problem, const ffn_b200_moe_buffers* buffers,
+                                         int device, ffn_b200_moe** handle);
+/* One asynchronous launch on `stream`; residual may be NULL.  Y must not overlap X or the
+ * residual.  Runs of one handle must be serialised on one stream (they share its scratch). */
+FFN_B200_EXPORT int ffn_b200_moe_run(ffn_b200_moe* handle, const void* x, int64_t ldx, const int32_t* ids,
+                                     const float* weights, const void* residual, int64_t ldr, void* y, int64_t ldy,
+                                     void* stream);
+/* Clears counters and status; call after a run reported a kernel error. */
+FFN_B200_EXPORT int ffn_b200_moe_reset(ffn_b200_moe* handle, void* stream);
+/* Bounded waits and the test hook that makes one run out, as for ffn_b200_handle. */
+FFN_B200_EXPORT int ffn_b200_moe_set_wait_limit(ffn_b200_moe* handle, uint64_t nanoseconds);
+FFN_B200_EXPORT int ffn_b200_moe_set_fault_injection(ffn_b200_moe* handle, int mode);
+FFN_B200_EXPORT int ffn_b200_moe_destroy(ffn_b200_moe* handle);
 
 #ifdef __cplusplus
 }

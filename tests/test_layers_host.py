@@ -1,0 +1,134 @@
+"""CPU tests of the dense projection, the router and the mixture-of-experts layer: what their
+entry points refuse, and the C planners and struct layouts (no GPU)."""
+import ctypes
+import subprocess
+import tempfile
+from pathlib import Path
+
+import pytest
+import torch
+
+from ffn_optim_b200 import NotApplicable, _lib, linear, moe_ffn, prepare_linear, prepare_moe_ffn, route_experts
+from ffn_optim_b200.host import layers as L
+
+HEADER = Path(__file__).resolve().parents[1] / "include" / "ffn_b200.h"
+
+
+def t(*shape, dtype=torch.bfloat16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def test_linear_refusals():
+    x, w = t(4, 8), t(6, 8)
+    with pytest.raises(ValueError, match="requires CUDA"):
+        linear(x, w, bias=t(6), residual=t(4, 6))
+    with pytest.raises(TypeError):
+        linear(x.float().numpy(), w)
+    with pytest.raises(TypeError):
+        linear(x, None)
+    for bad in (dict(x=t(8)), dict(x=t(4, 8, dtype=torch.float32)), dict(x=t(0, 8)), dict(x=t(*[1] * 8, 8)),
+                dict(x=t(4, 7)), dict(weight=t(6, 8, dtype=torch.float16)), dict(weight=t(6)), dict(weight=t(0, 8)),
+                dict(bias=t(7)), dict(bias=t(6, dtype=torch.float32)), dict(bias=t(1, 6)), dict(residual=t(4, 7)),
+                dict(residual=t(6)), dict(residual=t(1, 6)), dict(activation="relu"), dict(activation="swiglu"),
+                dict(gelu="tanh", activation="gelu"), dict(block_num=0), dict(block_num=1.5), dict(tile="bogus"),
+                dict(x=x.clone().requires_grad_()), dict(weight=w.clone().requires_grad_()),
+                dict(bias=t(6).requires_grad_()), dict(x=t(2, 65536), weight=t(2, 65536)),
+                dict(x=x.to_sparse())):
+        with pytest.raises(ValueError) as err:
+            prepare_linear(**{"x": x, "weight": w, **bad})
+        assert "requires CUDA" not in str(err.value), bad
+
+
+def test_router_refusals():
+    x, w = t(4, 8), t(6, 8)
+    good = dict(top_k=2)
+    with pytest.raises(ValueError, match="requires CUDA"):
+        route_experts(x, w.float(), choice_bias=t(6, dtype=torch.float32), mask=t(4, dtype=torch.bool), **good)
+    for bad in (dict(top_k=0), dict(top_k=7), dict(top_k=2.0), dict(top_k=True), dict(scoring="relu"),
+                dict(choice_bias=t(6)), dict(choice_bias=t(5, dtype=torch.float32)), dict(mask=t(4)),
+                dict(mask=t(3, dtype=torch.bool)), dict(mask=t(4, 1, dtype=torch.bool)), dict(weight=t(6, 7)),
+                dict(weight=t(6, 8, dtype=torch.float16)), dict(weight=t(6, 8, dtype=torch.float64)),
+                dict(weight=t(513, 8)), dict(weight=t(40, 8), top_k=33)):
+        with pytest.raises(ValueError) as err:
+            route_experts(**{"x": x, "weight": w, **good, **bad})
+        assert "requires CUDA" not in str(err.value), bad
+
+
+def test_moe_refusals():
+    x, wr, w1, w2 = t(4, 8), t(3, 8), t(3, 10, 8), t(3, 6, 5)
+    good = dict(x=x, router_weight=wr, weight1=w1, weight2=w2, top_k=2)
+    with pytest.raises(ValueError, match="requires CUDA"):
+        moe_ffn(**good, residual=t(4, 6))
+    with pytest.raises(NotApplicable, match="few-token"):
+        moe_ffn(**{**good, "x": t(257, 8)})
+    for bad in (dict(weight1=t(3, 5, 8)), dict(weight1=t(3, 10, 7)), dict(weight1=t(2, 10, 8)), dict(weight2=t(3, 6, 4)),
+                dict(weight2=t(6, 5)), dict(weight2=t(3, 0, 5)), dict(activation="gelu"), dict(activation="none"),
+                dict(router_weight=t(4, 8)), dict(router_weight=t(3, 9)), dict(residual=t(4, 8)), dict(top_k=4),
+                dict(weight2=t(3, 6, 5, dtype=torch.float16)), dict(block_num=-1),
+                dict(weight1=w1.clone().requires_grad_())):
+        with pytest.raises(ValueError) as err:
+            prepare_moe_ffn(**{**good, **bad})
+        assert "requires CUDA" not in str(err.value), bad
+
+
+def test_structs_match_the_header():
+    names = {"ffn_b200_linear_problem": _lib.LinearProblem, "ffn_b200_linear_plan": _lib.LinearPlan,
+             "ffn_b200_router_problem": _lib.RouterProblem, "ffn_b200_moe_problem": _lib.MoeProblem,
+             "ffn_b200_moe_plan": _lib.MoePlan, "ffn_b200_moe_buffers": _lib.MoeBuffers}
+    body = "".join(f'printf("%zu\\n", sizeof({n}));' for n in names)
+    body += "".join(f'printf("%zu\\n", offsetof({n}, {f}));' for n, c in names.items() for f, _ in c._fields_)
+    src = f'#include <stdio.h>\n#include <stddef.h>\n#include "{HEADER}"\nint main(void) {{ {body} return 0; }}'
+    with tempfile.TemporaryDirectory() as d:
+        c, exe = Path(d) / "s.c", Path(d) / "s"
+        c.write_text(src)
+        subprocess.run(["gcc", "-o", str(exe), str(c)], check=True)
+        got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    want = [ctypes.sizeof(c) for c in names.values()]
+    want += [getattr(c, f).offset for c in names.values() for f, _ in c._fields_]
+    assert got == want
+
+
+def test_c_entries_reject_bad_problems(lib):
+    lp = _lib.LinearPlan()
+    for args in ((0, 8, 8, 1, 4, 0, 148, 0, 0), (8, 70000, 8, 1, 4, 0, 148, 0, 0), (8, 8, 8, 2, 4, 0, 148, 0, 0),
+                 (8, 8, 8, 1, 3, 0, 148, 0, 0), (8, 8, 8, 1, 5, 0, 148, 0, 0), (8, 8, 8, 1, 4, -1, 148, 0, 0),
+                 (8, 8, 8, 1, 4, 0, 148, 99, 0)):
+        assert lib.ffn_b200_linear_make_plan(ctypes.byref(_lib.LinearProblem(*args)), ctypes.byref(lp)) == _lib.ERR_INVALID
+    a, b = ctypes.c_int64(), ctypes.c_int64()
+    for args in ((0, 8, 4, 2, 1, 0, 0, 1, 1.0, 0), (8, 8, 513, 2, 1, 0, 0, 1, 1.0, 0), (8, 8, 4, 5, 1, 0, 0, 1, 1.0, 0),
+                 (8, 8, 4, 2, 1, 2, 0, 1, 1.0, 0), (8, 8, 4, 2, 7, 0, 0, 1, 1.0, 0)):
+        assert lib.ffn_b200_router_scratch(ctypes.byref(_lib.RouterProblem(*args)), ctypes.byref(a),
+                                           ctypes.byref(b)) == _lib.ERR_INVALID
+    mp = _lib.MoePlan()
+    for args in ((0, 8, 8, 8, 4, 2, 1, 3, 0, 148), (8, 8, 70000, 8, 4, 2, 1, 3, 0, 148), (8, 8, 8, 8, 4, 5, 1, 3, 0, 148),
+                 (8, 8, 8, 8, 4, 2, 1, 4, 0, 148), (8, 8, 8, 8, 0, 0, 1, 3, 0, 148)):
+        assert lib.ffn_b200_moe_make_plan(ctypes.byref(_lib.MoeProblem(*args)), ctypes.byref(mp)) == _lib.ERR_INVALID
+    many = _lib.MoeProblem(257, 8, 8, 8, 4, 2, 1, 3, 0, 148)
+    assert lib.ffn_b200_moe_make_plan(ctypes.byref(many), ctypes.byref(mp)) == _lib.ERR_TOO_LARGE
+    for fn in (lib.ffn_b200_linear_run, lib.ffn_b200_moe_run):
+        assert fn(None, None, 8, None, *([None] if fn is lib.ffn_b200_moe_run else []),
+                  *([None] if fn is lib.ffn_b200_moe_run else []), 8, None, 8, None) == _lib.ERR_INVALID
+    assert lib.ffn_b200_moe_reset(None, None) == _lib.ERR_INVALID
+
+
+def test_operands_read_in_place_or_copied():
+    """Which views the kernels read in place: unit column stride, 16-byte base, pitch a multiple of 8."""
+    base = torch.zeros(9 * 40, dtype=torch.bfloat16)
+    assert base.data_ptr() % 16 == 0
+    m = base.view(9, 40)
+    assert L.addressable(m, 9, 40) and L.addressable(m[:, 8:30], 9, 22) and L.addressable(m[:1, :7], 1, 7)
+    assert not L.addressable(m[:, 4:30], 9, 26)       # base off the 16-byte grid
+    assert not L.addressable(m.t(), 40, 9)            # columns not contiguous
+    assert not L.addressable(base[:39 * 9].view(9, 39), 9, 39)  # odd pitch
+    assert not L.addressable(m[:1].expand(9, 40), 9, 40)        # rows on top of one another
+    w = torch.zeros(4, 6, 24, dtype=torch.bfloat16)
+    assert L.packed_weight(w) is w and L.packed_weight(w[:, ::2]).data_ptr() == w.data_ptr()
+    odd = torch.randn(4, 6, 21).to(torch.bfloat16)
+    packed = L.packed_weight(odd)
+    assert torch.equal(packed, odd) and packed.stride() == (6 * 24, 24, 1)
+    store = L.RowStorage(9, 40, m, m.shape)
+    assert store.bind(m, "x", (0, 0))[0] == m.data_ptr()
+    own = (m.data_ptr(), m.data_ptr() + m.numel() * 2)
+    assert store.bind(m[:, :], "x", own)[0] != m.data_ptr()     # inside the output: copied
+    with pytest.raises(ValueError, match="prepared shape"):
+        store.bind(m[:8], "x", (0, 0))
