@@ -2,14 +2,17 @@
 // (declarations in include/ffn_b200.h).
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <mutex>
 #include <new>
 
 #include "../../include/ffn_b200.h"
 #include "layers_simple.cuh"
+#include "stream_kernel.cuh"
 
 namespace {
 
@@ -60,6 +63,91 @@ int check_device(int device) {
   return maj == 10 && min == 0 ? FFN_B200_OK : FFN_B200_ERR_DEVICE;
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+
+int get_encode() {
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult st;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &st) == cudaSuccess &&
+        st == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  });
+  return g_encode ? FFN_B200_OK : FFN_B200_ERR_CUDA;
+}
+
+// 128B-swizzled tensor map of 16-bit elements; `strides` in elements, one per dimension but the first.
+int encode(CUtensorMap* tm, const void* base, int dtype, int rank, const int64_t* dims, const int64_t* strides,
+           const uint32_t* box) {
+  cuuint64_t gdim[4], gstr[3];
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) gdim[i] = static_cast<cuuint64_t>(dims[i]);
+  for (int i = 0; i + 1 < rank; ++i) gstr[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+  const CUresult r = g_encode(tm, dtype == FFN_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdim, gstr, box, ones,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FFN_B200_OK : FFN_B200_ERR_CUDA;
+}
+// Weights [experts][halves][rows][cols] in boxes of 128 rows, or of 16 rows of both halves.
+int encode_weights(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int64_t rows, int64_t halves,
+                   int64_t experts, int64_t ld, int64_t stride) {
+  const int64_t dims[4] = {cols, rows, halves, experts};
+  const int64_t strides[3] = {ld, rows * ld, stride};
+  const uint32_t box[4] = {64, halves == 2 ? 16u : 128u, halves == 2 ? 2u : 1u, 1};
+  return encode(tm, base, dtype, 4, dims, strides, box);
+}
+// Rows [rows][cols] for gathered loads (a box of one row).
+int encode_rows(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int64_t rows, int64_t ld) {
+  const int64_t dims[2] = {cols, rows};
+  const uint32_t box[2] = {64, 1};
+  return encode(tm, base, dtype, 2, dims, &ld, box);
+}
+
+constexpr int kMaxSmem = 232448;
+
+int stream_chunk(int64_t tokens) { return tokens <= 16 ? 16 : (tokens <= 32 ? 32 : (tokens <= 64 ? 64 : 128)); }
+// Ring slots beside `list_bytes` of lists, and the dynamic shared memory they add up to.
+int stream_stages(int chunk, int list_bytes, int64_t* smem) {
+  const int stage = ffnb200::kABytes + chunk * 128, fixed = 1024 + ffnb200::kStreamBarBytes + list_bytes;
+  const int stages = std::min(ffnb200::kStreamMaxStages, (kMaxSmem - fixed) / stage);
+  *smem = static_cast<int64_t>(stages) * stage + fixed;
+  return stages;
+}
+
+using StreamFn = void (*)(const ffnb200::StreamParams);
+
+int launch_stream(StreamFn fn, const ffnb200::StreamParams& params, int grid, int64_t smem, bool cooperative,
+                  void* stream) {
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(ffnb200::kStreamThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  if (cooperative) {  // CTAs wait on one another: all resident at once
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+  } else {  // no waits between CTAs: set-up overlaps the previous kernel's end
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, fn, params) == cudaSuccess) return FFN_B200_OK;
+  cudaGetLastError();
+  return FFN_B200_ERR_CUDA;
+}
+
+int set_smem(const void* fn, int64_t smem) {
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess)
+    return FFN_B200_OK;
+  cudaGetLastError();
+  return FFN_B200_ERR_CUDA;
+}
+
 int check_linear(const ffn_b200_linear_problem& p) {
   if (p.m <= 0 || p.k <= 0 || p.n <= 0 || p.k > kMaxDim || p.n > kMaxDim || p.m > (int64_t(1) << 31) - 16)
     return FFN_B200_ERR_INVALID;
@@ -101,6 +189,8 @@ struct ffn_b200_linear {
   const void* w;
   int64_t ldw;
   const void* bias;
+  ffnb200::StreamParams params;
+  StreamFn fn;
 };
 
 struct ffn_b200_moe {
@@ -108,8 +198,8 @@ struct ffn_b200_moe {
   ffn_b200_moe_plan plan;
   ffn_b200_moe_buffers buf;
   int device;
-  uint64_t wait_limit_ns;
-  int inject;
+  ffnb200::StreamParams params;
+  StreamFn fn;
 };
 
 extern "C" {
@@ -123,8 +213,19 @@ int ffn_b200_linear_make_plan(const ffn_b200_linear_problem* pr, ffn_b200_linear
   rc = device_sms(pr->sm_count, &sms);
   if (rc) return rc;
   std::memset(out, 0, sizeof(*out));
-  out->block_num = sms;
-  out->split = 1;
+  const int grid = pr->block_num ? pr->block_num : sms;
+  out->block_num = grid;
+  out->tile = pr->tile ? pr->tile : (pr->m <= 1024 ? 1 : 2);
+  if (out->tile == 1) {
+    const int chunk = stream_chunk(pr->m);
+    out->tile_m = chunk;
+    out->tile_n = 128;
+    out->stages = stream_stages(chunk, 0, &out->smem_bytes);
+    out->workspace_floats = 2ll * grid * chunk * 128;
+    out->counter_words = grid;
+    const int64_t steps = cdiv(pr->n, 128) * cdiv(pr->m, chunk) * cdiv(pr->k, 64);
+    if (steps >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
+  }
   return FFN_B200_OK;
 }
 
@@ -137,6 +238,12 @@ int ffn_b200_linear_prepare(const ffn_b200_linear_problem* pr, const void* w, in
   if (!rc) rc = ffn_b200_linear_make_plan(pr, &plan);
   if (rc) return rc;
   if (bad_rows(w, ldw, pr->k)) return FFN_B200_ERR_ALIGNMENT;
+  if (bias && !aligned16(bias)) return FFN_B200_ERR_ALIGNMENT;
+  if (!workspace || !counters) return FFN_B200_ERR_INVALID;
+  rc = get_encode();
+  if (rc) return rc;
+  DeviceScope scope(device);
+  if (!scope.ok) return FFN_B200_ERR_DEVICE;
   auto* h = new (std::nothrow) ffn_b200_linear();
   if (!h) return FFN_B200_ERR_INVALID;
   h->prob = *pr;
@@ -145,6 +252,29 @@ int ffn_b200_linear_prepare(const ffn_b200_linear_problem* pr, const void* w, in
   h->w = w;
   h->ldw = ldw;
   h->bias = bias;
+  if (plan.tile == 1) {
+    ffnb200::StreamParams& P = h->params;
+    std::memset(&P, 0, sizeof(P));
+    rc = encode_weights(&P.tm_w1, w, pr->dtype, pr->k, pr->n, 1, 1, ldw, pr->n * ldw);
+    P.tokens = static_cast<int>(pr->m);
+    P.chunk = plan.tile_m;
+    P.items = static_cast<int>(cdiv(pr->m, P.chunk));
+    P.tiles1 = static_cast<int>(cdiv(pr->n, 128));
+    P.steps1 = static_cast<int>(cdiv(pr->k, 64));
+    P.feat1 = static_cast<int>(pr->n);
+    P.stages = plan.stages;
+    P.act = pr->activation;
+    P.bias = static_cast<const uint16_t*>(bias);
+    P.partial1 = workspace;
+    P.counters = counters;
+    P.wait_limit_ns = 4000000000ull;
+    h->fn = pr->dtype == FFN_B200_BF16 ? ffnb200::stream_kernel<true, false> : ffnb200::stream_kernel<false, false>;
+    if (!rc) rc = set_smem(reinterpret_cast<const void*>(h->fn), kMaxSmem);
+  }
+  if (rc) {
+    delete h;
+    return rc;
+  }
   *out = h;
   return FFN_B200_OK;
 }
@@ -156,6 +286,16 @@ int ffn_b200_linear_run(ffn_b200_linear* h, const void* x, int64_t ldx, const vo
   if (bad_rows(x, ldx, p.k) || bad_rows(y, ldy, p.n) || (res && bad_rows(res, ldr, p.n))) return FFN_B200_ERR_ALIGNMENT;
   DeviceScope scope(h->device);
   if (!scope.ok) return FFN_B200_ERR_DEVICE;
+  if (h->plan.tile == 1) {
+    ffnb200::StreamParams P = h->params;
+    const int rc = encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx);
+    if (rc) return rc;
+    P.residual = static_cast<const uint16_t*>(res);
+    P.ldr = ldr;
+    P.y = static_cast<uint16_t*>(y);
+    P.ldy = ldy;
+    return launch_stream(h->fn, P, h->plan.block_num, h->plan.smem_bytes, false, stream);
+  }
   const int64_t blocks = cdiv(p.m * p.n, 256);
   if (blocks >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
   auto* kern = p.dtype == FFN_B200_BF16 ? ffnb200::simple_linear<true> : ffnb200::simple_linear<false>;
@@ -204,11 +344,20 @@ int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* pr, ffn_b200_moe_plan* ou
   rc = device_sms(pr->sm_count, &sms);
   if (rc) return rc;
   std::memset(out, 0, sizeof(*out));
-  out->block_num = pr->block_num ? pr->block_num : sms;
+  const int grid = pr->block_num ? pr->block_num : sms;
+  const int tokens = static_cast<int>(pr->m);
+  const ffnb200::StreamLists lists(tokens, pr->experts, pr->top_k);
+  out->block_num = grid;
+  out->chunk = stream_chunk(pr->m);
+  out->stages = stream_stages(out->chunk, lists.bytes, &out->smem_bytes);
   out->hidden_rows = pr->m * pr->top_k;
   out->hidden_pitch = pitch_of(pr->h);
-  out->workspace_floats = 4;
-  out->counter_words = 4;
+  const int64_t slots = 2ll * grid * out->chunk * 128;
+  const int64_t items = ffnb200::StreamLists::stream_items(tokens, pr->experts, pr->top_k);
+  const int64_t up = cdiv(pr->h, pr->activation == FFN_B200_SWIGLU ? 64 : 128), down = cdiv(pr->n, 128);
+  if (items * std::max(up * cdiv(pr->k, 64), down * cdiv(pr->h, 64)) >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
+  out->workspace_floats = 2 * slots + out->hidden_rows * down * 128;
+  out->counter_words = grid + ffnb200::kStreamSync + items;
   out->status_words = 4;
   return FFN_B200_OK;
 }
@@ -221,17 +370,57 @@ int ffn_b200_moe_prepare(const ffn_b200_moe_problem* pr, const ffn_b200_moe_buff
   int rc = check_device(device);
   if (!rc) rc = ffn_b200_moe_make_plan(pr, &plan);
   if (rc) return rc;
+  int sms = 0, maj = 0, min = 0;
+  rc = ffn_b200_device_info(device, &sms, &maj, &min);
+  if (rc) return rc;
+  if (plan.block_num > sms) return FFN_B200_ERR_DEVICE;  // the CTAs wait on one another
   if (!b->w1 || !b->w2 || !b->hidden || !b->workspace || !b->counters || !b->status) return FFN_B200_ERR_INVALID;
-  if (bad_rows(b->w1, b->ldw1, pr->k) || bad_rows(b->w2, b->ldw2, pr->h) || b->stride1 % 8 || b->stride2 % 8)
+  if (bad_rows(b->w1, b->ldw1, pr->k) || bad_rows(b->w2, b->ldw2, pr->h) || b->stride1 % 8 || b->stride2 % 8 ||
+      b->stride1 <= 0 || b->stride2 <= 0 || !aligned16(b->hidden) || !aligned16(b->workspace))
     return FFN_B200_ERR_ALIGNMENT;
+  rc = get_encode();
+  if (rc) return rc;
+  DeviceScope scope(device);
+  if (!scope.ok) return FFN_B200_ERR_DEVICE;
   auto* h = new (std::nothrow) ffn_b200_moe();
   if (!h) return FFN_B200_ERR_INVALID;
   h->prob = *pr;
   h->plan = plan;
   h->buf = *b;
   h->device = device;
-  h->wait_limit_ns = 4000000000ull;
-  h->inject = 0;
+  ffnb200::StreamParams& P = h->params;
+  std::memset(&P, 0, sizeof(P));
+  const bool glu = pr->activation == FFN_B200_SWIGLU;
+  rc = encode_weights(&P.tm_w1, b->w1, pr->dtype, pr->k, pr->h, glu ? 2 : 1, pr->experts, b->ldw1, b->stride1);
+  if (!rc) rc = encode_weights(&P.tm_w2, b->w2, pr->dtype, pr->h, pr->n, 1, pr->experts, b->ldw2, b->stride2);
+  if (!rc) rc = encode_rows(&P.tm_h, b->hidden, pr->dtype, pr->h, plan.hidden_rows, plan.hidden_pitch);
+  P.tokens = static_cast<int>(pr->m);
+  P.tiles1 = static_cast<int>(cdiv(pr->h, glu ? 64 : 128));
+  P.steps1 = static_cast<int>(cdiv(pr->k, 64));
+  P.feat1 = static_cast<int>(pr->h);
+  P.tiles2 = static_cast<int>(cdiv(pr->n, 128));
+  P.steps2 = static_cast<int>(cdiv(pr->h, 64));
+  P.feat2 = static_cast<int>(pr->n);
+  P.chunk = plan.chunk;
+  P.stages = plan.stages;
+  P.act = pr->activation;
+  P.hidden = static_cast<uint16_t*>(b->hidden);
+  P.ldh = plan.hidden_pitch;
+  const int64_t slots = 2ll * plan.block_num * plan.chunk * 128;
+  P.partial1 = b->workspace;
+  P.partial2 = b->workspace + slots;
+  P.whole2 = b->workspace + 2 * slots;
+  P.counters = b->counters;
+  P.status = b->status;
+  P.experts = pr->experts;
+  P.top = pr->top_k;
+  P.wait_limit_ns = 4000000000ull;
+  h->fn = pr->dtype == FFN_B200_BF16 ? ffnb200::stream_kernel<true, true> : ffnb200::stream_kernel<false, true>;
+  if (!rc) rc = set_smem(reinterpret_cast<const void*>(h->fn), kMaxSmem);
+  if (rc) {
+    delete h;
+    return rc;
+  }
   *out = h;
   return FFN_B200_OK;
 }
@@ -240,20 +429,19 @@ int ffn_b200_moe_run(ffn_b200_moe* h, const void* x, int64_t ldx, const int32_t*
                      const void* res, int64_t ldr, void* y, int64_t ldy, void* stream) {
   if (!h || !x || !ids || !weights || !y) return FFN_B200_ERR_INVALID;
   const ffn_b200_moe_problem& p = h->prob;
-  const ffn_b200_moe_buffers& b = h->buf;
   if (bad_rows(x, ldx, p.k) || bad_rows(y, ldy, p.n) || (res && bad_rows(res, ldr, p.n))) return FFN_B200_ERR_ALIGNMENT;
   DeviceScope scope(h->device);
   if (!scope.ok) return FFN_B200_ERR_DEVICE;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool bf = p.dtype == FFN_B200_BF16;
-  const int k = static_cast<int>(p.k), hh = static_cast<int>(p.h), n = static_cast<int>(p.n);
-  const dim3 up(static_cast<unsigned>(cdiv(hh, 128)), static_cast<unsigned>(p.m * p.top_k));
-  const dim3 dn(static_cast<unsigned>(cdiv(n, 128)), static_cast<unsigned>(p.m));
-  (bf ? ffnb200::simple_expert_up<true> : ffnb200::simple_expert_up<false>)<<<up, 128, 0, st>>>(
-      x, ldx, ids, p.experts, b.w1, b.ldw1, b.stride1, b.hidden, h->plan.hidden_pitch, p.top_k, k, hh, p.activation);
-  (bf ? ffnb200::simple_expert_down<true> : ffnb200::simple_expert_down<false>)<<<dn, 128, 0, st>>>(
-      b.hidden, h->plan.hidden_pitch, ids, weights, p.experts, b.w2, b.ldw2, b.stride2, res, ldr, y, ldy, p.top_k, hh, n);
-  return launched();
+  ffnb200::StreamParams P = h->params;
+  const int rc = encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx);
+  if (rc) return rc;
+  P.ids = ids;
+  P.weights = weights;
+  P.residual = static_cast<const uint16_t*>(res);
+  P.ldr = ldr;
+  P.y = static_cast<uint16_t*>(y);
+  P.ldy = ldy;
+  return launch_stream(h->fn, P, h->plan.block_num, h->plan.smem_bytes, true, stream);
 }
 
 int ffn_b200_moe_reset(ffn_b200_moe* h, void* stream) {
@@ -269,13 +457,13 @@ int ffn_b200_moe_reset(ffn_b200_moe* h, void* stream) {
 
 int ffn_b200_moe_set_wait_limit(ffn_b200_moe* h, uint64_t ns) {
   if (!h || ns == 0) return FFN_B200_ERR_INVALID;
-  h->wait_limit_ns = ns;
+  h->params.wait_limit_ns = ns;
   return FFN_B200_OK;
 }
 
 int ffn_b200_moe_set_fault_injection(ffn_b200_moe* h, int mode) {
   if (!h || mode < 0 || mode > 1) return FFN_B200_ERR_INVALID;
-  h->inject = mode;
+  h->params.inject = mode;
   return FFN_B200_OK;
 }
 

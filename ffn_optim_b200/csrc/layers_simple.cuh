@@ -79,42 +79,4 @@ __global__ void simple_route(const void* x, int64_t ldx, const void* w, int64_t 
     weights[t * top + j] = static_cast<float>(row[ids[t * top + j]] / (renorm ? total : 1.0) * static_cast<double>(scale));
 }
 
-template <bool BF16>
-__global__ void simple_expert_up(const void* x, int64_t ldx, const int32_t* ids, int experts, const void* w1,
-                                 int64_t ldw, int64_t es, void* hidden, int64_t ldh, int top, int k, int h, int act) {
-  const int64_t pair = blockIdx.y;
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  const int e = ids[pair];
-  if (c >= h || e < 0 || e >= experts) return;
-  const int64_t xo = pair / top * ldx;
-  const int64_t wo = e * es + c * ldw;
-  float z = 0.f, u = 0.f;
-  for (int j = 0; j < k; ++j) {
-    const float xv = elem<BF16>(x, xo + j);
-    z = fmaf(xv, elem<BF16>(w1, wo + j), z);
-    if (act == 3) u = fmaf(xv, elem<BF16>(w1, wo + h * ldw + j), u);
-  }
-  static_cast<uint16_t*>(hidden)[pair * ldh + c] = cvt1<BF16>(act == 3 ? silu(z) * u : apply_act(z, act));
-}
-
-template <bool BF16>
-__global__ void simple_expert_down(const void* hidden, int64_t ldh, const int32_t* ids, const float* weights,
-                                   int experts, const void* w2, int64_t ldw, int64_t es, const void* res, int64_t ldr,
-                                   void* y, int64_t ldy, int top, int h, int n) {
-  const int64_t t = blockIdx.y;
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= n) return;
-  float acc = 0.f;
-  for (int j = 0; j < top; ++j) {
-    const int e = ids[t * top + j];
-    if (e < 0 || e >= experts) continue;
-    float z = 0.f;
-    for (int i = 0; i < h; ++i)
-      z = fmaf(elem<BF16>(hidden, (t * top + j) * ldh + i), elem<BF16>(w2, e * es + c * ldw + i), z);
-    acc = fmaf(weights[t * top + j], z, acc);
-  }
-  if (res) acc += elem<BF16>(res, t * ldr + c);
-  static_cast<uint16_t*>(y)[t * ldy + c] = cvt1<BF16>(acc);
-}
-
 }  // namespace ffnb200
