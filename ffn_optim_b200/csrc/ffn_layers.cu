@@ -12,6 +12,7 @@
 
 #include "../../include/ffn_b200.h"
 #include "layers_simple.cuh"
+#include "router_kernel.cuh"
 #include "stream_kernel.cuh"
 
 namespace {
@@ -137,6 +138,33 @@ int launch_stream(StreamFn fn, const ffnb200::StreamParams& params, int grid, in
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, fn, params) == cudaSuccess) return FFN_B200_OK;
+  cudaGetLastError();
+  return FFN_B200_ERR_CUDA;
+}
+
+using RouteFn = void (*)(const ffnb200::RouteParams);
+
+int launch_route(RouteFn fn, const ffnb200::RouteParams& P, int mt, int nt, void* stream) {
+  const int64_t rows = cdiv(P.M, 16 * mt);
+  if (rows > 65535) return FFN_B200_ERR_TOO_LARGE;
+  const int smem = ffnb200::kRouteWarps * 128 * mt * nt * 12;
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return FFN_B200_ERR_CUDA;
+  }
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(cdiv(P.E, 8 * nt)), static_cast<unsigned>(rows), 1);
+  cfg.blockDim = dim3(ffnb200::kRouteThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, fn, P) == cudaSuccess) return FFN_B200_OK;
   cudaGetLastError();
   return FFN_B200_ERR_CUDA;
 }
@@ -314,8 +342,9 @@ int ffn_b200_router_scratch(const ffn_b200_router_problem* pr, int64_t* logit_do
   if (!pr || !logit_doubles || !counter_words) return FFN_B200_ERR_INVALID;
   const int rc = check_router(*pr);
   if (rc) return rc;
-  *logit_doubles = pr->m * pr->experts;
-  *counter_words = cdiv(pr->m, 8);
+  const int64_t cells = pr->m * pr->experts;
+  *logit_doubles = cells + (cells + 1) / 2;  // fp64 logits, then fp32 sums of |x w|
+  *counter_words = cdiv(pr->m, 16);
   return FFN_B200_OK;
 }
 
@@ -326,13 +355,25 @@ int ffn_b200_router_run(const ffn_b200_router_problem* pr, const void* x, int64_
   const int rc = check_router(*pr);
   if (rc) return rc;
   if (bad_rows(x, ldx, pr->k) || bad_rows(w, ldw, pr->k)) return FFN_B200_ERR_ALIGNMENT;
-  auto* kern = pr->dtype == FFN_B200_BF16
-                   ? (pr->weight_f32 ? ffnb200::simple_route<true, true> : ffnb200::simple_route<true, false>)
-                   : (pr->weight_f32 ? ffnb200::simple_route<false, true> : ffnb200::simple_route<false, false>);
-  kern<<<static_cast<unsigned>(pr->m), 128, 0, static_cast<cudaStream_t>(stream)>>>(
-      x, ldx, w, ldw, cbias, mask, ids, weights, logits, static_cast<int>(pr->k), pr->experts, pr->top_k, pr->sigmoid,
-      pr->renormalize, pr->scale);
-  return launched();
+  ffnb200::RouteParams P;
+  P.x = x; P.ldx = ldx; P.w = w; P.ldw = ldw;
+  P.choice_bias = cbias; P.mask = mask; P.ids = ids; P.weights = weights;
+  P.logits = logits;
+  P.sums = reinterpret_cast<float*>(logits + pr->m * pr->experts);
+  P.counters = counters;
+  P.M = static_cast<int>(pr->m); P.K = static_cast<int>(pr->k); P.E = pr->experts; P.top = pr->top_k;
+  P.sigmoid = pr->sigmoid; P.renormalize = pr->renormalize; P.scale = pr->scale;
+  const bool bf = pr->dtype == FFN_B200_BF16, w32 = pr->weight_f32 != 0;
+  // Small tiles spread few tokens over more CTAs; from 128 tokens on the larger tile halves and
+  // quarters the operand reads.
+  if (pr->m < 128) {
+    return launch_route(bf ? (w32 ? ffnb200::route_kernel<true, true, 1, 1> : ffnb200::route_kernel<true, false, 1, 1>)
+                           : (w32 ? ffnb200::route_kernel<false, true, 1, 1> : ffnb200::route_kernel<false, false, 1, 1>),
+                        P, 1, 1, stream);
+  }
+  return launch_route(bf ? (w32 ? ffnb200::route_kernel<true, true, 2, 4> : ffnb200::route_kernel<true, false, 2, 4>)
+                         : (w32 ? ffnb200::route_kernel<false, true, 2, 4> : ffnb200::route_kernel<false, false, 2, 4>),
+                      P, 2, 4, stream);
 }
 
 // ---- mixture-of-experts layer --------------------------------------------------------------

@@ -102,8 +102,8 @@ def prepare_router(x, weight, *, top_k, scoring="softmax", choice_bias=None, ren
     ``sigmoid`` of the logits; the ``top_k`` experts of the largest score (+ ``choice_bias``, fp32
     [E], which takes no part in the weights) are chosen, equal keys by the lower index, a NaN key
     after every other.  ``weights`` are their scores, divided by their sum if ``renormalize``,
-    times ``scale``.  Logits and scores are 64-bit.  Tokens whose ``mask`` (bool, x's leading
-    shape) is False get ids -1 and weights 0."""
+    times ``scale``.  The ids are those of 64-bit logits, the weights have fp32 accuracy.  Tokens
+    whose ``mask`` (bool, x's leading shape) is False get ids -1 and weights 0."""
     return PreparedRouter(x, weight, top_k, scoring, choice_bias, renormalize, scale, mask)
 
 

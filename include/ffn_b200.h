@@ -364,9 +364,9 @@ FFN_B200_EXPORT int ffn_b200_linear_destroy(ffn_b200_linear* handle);
 /* ---- Expert router ------------------------------------------------------------------------
  *     p = softmax(X . W^T) or sigmoid(X . W^T);  ids = the top_k experts by p + choice_bias;
  *     weights = p[ids] (divided by their sum when `renormalize`) * scale
- * Logits and scores are 64-bit, so that the choice does not depend on a summation order; equal
- * keys go to the lower index, a NaN key ranks below every other.  A token whose mask byte is 0
- * gets ids -1 and weights 0. */
+ * The ids are those of 64-bit logits (sums whose error could decide a choice are taken again in
+ * fp64); the weights have fp32 accuracy.  Equal keys go to the lower index, a NaN key ranks below
+ * every other.  A token whose mask byte is 0 gets ids -1 and weights 0. */
 typedef struct {
   int64_t m, k;
   int32_t experts;     /* at most FFN_B200_MAX_EXPERTS */
@@ -382,7 +382,7 @@ typedef struct {
 #define FFN_B200_MAX_EXPERTS 512
 #define FFN_B200_MAX_TOP_K 32
 
-/* Scratch of one run: fp64 logits and u32 counters (zeroed before the first run). */
+/* Scratch of one run: fp64 logits (with their error bounds) and u32 counters (zeroed before the first run). */
 FFN_B200_EXPORT int ffn_b200_router_scratch(const ffn_b200_router_problem* problem, int64_t* logit_doubles,
                                             int64_t* counter_words);
 /* One asynchronous launch on `stream` of the current device.  choice_bias (fp32 [experts]) and

@@ -28,9 +28,16 @@ def check_route(got, x, w, **kw):
     assert got_ids.dtype == torch.int32 and got_w.dtype == torch.float32
     assert got_ids.shape == (*x.shape[:-1], kw["top_k"]) == got_w.shape
     assert torch.equal(got_ids.reshape(ids.shape), ids)
-    # one rounding to fp32 (2^-24), the 64-bit arithmetic far below it
+    # A logit is summed in fp32 chains of 64 products (four MMAs, each off by at most 2^-22 of its
+    # sum |x w|) that are added in 64 bits: off by at most 2^-20 S, S = sum |x w|.  A weight moves
+    # by at most twice that relatively (its own logit's error and its normaliser's), plus one
+    # rounding to fp32.  Chains' errors are independent, so in the 2-norm the weights keep
+    # fp32 accuracy: K/64 chains of error 2^-23 of a 1/sqrt(K/64) part of the logit each.
     off = (got_w.double().reshape(wt.shape) - wt).abs()
-    assert (off <= 2.0 ** -24 * 1.01 * wt.abs() + 2.0 ** -149).all()
+    size = x.double().abs().reshape(-1, x.shape[-1]) @ w.double().abs().t()
+    worst = 2.0 ** -24 + (0 if w.dtype == torch.float32 else 2 * 2.0 ** -20 * size.amax(1, keepdim=True))
+    assert (off <= 1.01 * worst * wt.abs() + 2.0 ** -149).all()
+    assert off.norm() <= 1e-6 * wt.norm()
 
 
 @pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 64, 257, 1000])
@@ -86,8 +93,10 @@ def test_router_nan_inf_and_masked_rows():
     assert torch.equal(ids[2], torch.arange(4, dtype=torch.int32, device="cuda")) and wt[2].isnan().all()
     assert (ids[7] == -1).all() and (wt[7] == 0).all()
     assert not (ids == 5).any() or (ids[2] == 5).sum() == (ids == 5).sum()
-    live = [i for i in range(12) if i not in (2,)]
-    assert ((wt[live].double() - ref_w[live]).abs() <= 2.0 ** -23 * ref_w[live].abs()).all()
+    live = [i for i in range(12) if i not in (2, 7)]
+    size = x.double().abs() @ w.nan_to_num().double().abs().t()
+    bound = (2.0 ** -24 + 2 * 2.0 ** -20 * size[live].amax(1, keepdim=True)) * ref_w[live].abs()
+    assert ((wt[live].double() - ref_w[live]).abs() <= 1.01 * bound).all()
 
 
 @pytest.mark.parametrize("m", [1, 300])
