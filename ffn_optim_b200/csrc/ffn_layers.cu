@@ -147,7 +147,7 @@ using RouteFn = void (*)(const ffnb200::RouteParams);
 int launch_route(RouteFn fn, const ffnb200::RouteParams& P, int mt, int nt, void* stream) {
   const int64_t rows = cdiv(P.M, 16 * mt);
   if (rows > 65535) return FFN_B200_ERR_TOO_LARGE;
-  const int smem = ffnb200::kRouteWarps * 128 * mt * nt * 12;
+  const int smem = ffnb200::kRouteWarps * std::max(128 * mt * nt * 12, P.E * 16);  // parts of K; then logits and scores
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();

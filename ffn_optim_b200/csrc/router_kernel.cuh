@@ -26,7 +26,6 @@ namespace ffnb200 {
 constexpr int kRouteWarps = 8;
 constexpr int kRouteThreads = 32 * kRouteWarps;
 constexpr int kRouteStep = 64;                 // K per chain
-constexpr int kRouteMaxPerLane = 16;           // 512 experts / 32 lanes
 constexpr double kRouteLoss = 1.0 / (1 << 20); // error of a logit over the sum of its |x w|
 
 struct RouteParams {
@@ -93,112 +92,114 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// One token's choice by a warp.  Lane l holds experts l, l + 32, ...
+// A double as an unsigned integer of the same order (no NaN).
+__device__ __forceinline__ unsigned long long ordered(double v) {
+  const long long b = __double_as_longlong(v + 0.0);  // (+ 0.0: one zero)
+  return static_cast<unsigned long long>(b ^ (b < 0 ? -1ll : static_cast<long long>(1ull << 63)));
+}
+// The key of expert e: its score, with the choice bias; NaN ranks last.
+__device__ __forceinline__ double route_key(const RouteParams& p, double score, int e) {
+  const double key = p.choice_bias ? score + static_cast<double>(__ldg(p.choice_bias + e)) : score;
+  return key == key ? key : -INFINITY;
+}
+
+// One token's choice by a warp; z and q: this warp's logits and scores in shared memory [E].
+// (Loops are kept rolled: the code runs once per token, and fetching it costs more than running it.)
 template <bool BF16, bool W32>
-__device__ __forceinline__ void route_token(const RouteParams& p, int t, int lane) {
+__device__ __forceinline__ void route_token(const RouteParams& p, int t, int lane, double* z, double* q) {
   int* ids = p.ids + static_cast<size_t>(t) * p.top;
   float* weights = p.weights + static_cast<size_t>(t) * p.top;
   if (p.mask && !p.mask[t]) {
     for (int j = lane; j < p.top; j += 32) ids[j] = -1, weights[j] = 0.f;
     return;
   }
-  const int per = (p.E + 31) / 32;
-  double* logit = p.logits + static_cast<size_t>(t) * p.E;
-  double z[kRouteMaxPerLane];
-#pragma unroll
-  for (int i = 0; i < kRouteMaxPerLane; ++i)
-    if (i < per) z[i] = lane + 32 * i < p.E ? __ldcg(logit + lane + 32 * i) : -INFINITY;
   float s = 0.f;
   bool odd = false;  // a logit left fp32's range
-  if (!W32) {
-    for (int i = 0; i < per; ++i) {
-      const int e = lane + 32 * i;
-      if (e < p.E) s = fmaxf(s, __ldcg(p.sums + static_cast<size_t>(t) * p.E + e));
+#pragma unroll 2
+  for (int e = lane; e < p.E; e += 32) {
+    const double v = __ldcg(p.logits + static_cast<size_t>(t) * p.E + e);
+    if (!W32) {
+      s = fmaxf(s, __ldcg(p.sums + static_cast<size_t>(t) * p.E + e));
+      odd |= !isfinite(v);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
-#pragma unroll
-    for (int i = 0; i < kRouteMaxPerLane; ++i)
-      if (i < per && lane + 32 * i < p.E && !isfinite(z[i])) odd = true;
+    z[e] = v;
   }
-  const double loss = kRouteLoss * static_cast<double>(s);
-  unsigned again = 0;  // bit i: expert lane + 32 i has to be summed again
-  int chosen = -1;     // lane j < top: the j-th choice
-  double score = 0.0;  // and its score
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    // Scores.  The largest logit goes first as in any stable softmax; a NaN makes all of them NaN.
-    double q[kRouteMaxPerLane];
-    if (p.sigmoid) {
 #pragma unroll
-      for (int i = 0; i < kRouteMaxPerLane; ++i)
-        if (i < per) q[i] = 1.0 / (1.0 + exp(-z[i]));
-    } else {
+  for (int o = 16; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+  const double loss = kRouteLoss * static_cast<double>(s);
+  int chosen = -1;     // lane j < top: the j-th choice,
+  double score = 0.0;  // its score
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
+    // Scores.  A NaN logit makes every softmax score NaN.
+    double scale = 1.0;
+    if (!p.sigmoid) {
       double top = -INFINITY, sum = 0.0;
       bool nan = false;
-#pragma unroll
-      for (int i = 0; i < kRouteMaxPerLane; ++i)
-        if (i < per) top = fmax(top, z[i]), nan |= z[i] != z[i];
+#pragma unroll 1
+      for (int e = lane; e < p.E; e += 32) top = fmax(top, z[e]), nan |= z[e] != z[e];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (__any_sync(0xffffffffu, nan)) top = NAN;
-#pragma unroll
-      for (int i = 0; i < kRouteMaxPerLane; ++i)
-        if (i < per) {
-          q[i] = lane + 32 * i < p.E ? exp(z[i] - top) : 0.0;
-          sum += q[i];
-        }
-      sum = warp_sum(sum);
-#pragma unroll
-      for (int i = 0; i < kRouteMaxPerLane; ++i)
-        if (i < per) q[i] /= sum;
-    }
-    double key[kRouteMaxPerLane];
-#pragma unroll
-    for (int i = 0; i < kRouteMaxPerLane; ++i)
-      if (i < per) {
-        const int e = lane + 32 * i;
-        key[i] = e < p.E ? q[i] + (p.choice_bias ? static_cast<double>(__ldg(p.choice_bias + e)) : 0.0) : 0.0;
-        if (key[i] != key[i]) key[i] = -INFINITY;
-      }
-    // The k (+ 1 on the first pass) largest keys, equal ones by index.
-    unsigned used = 0;
 #pragma unroll 1
-    for (int j = 0; j <= p.top; ++j) {
-      if (j == p.top && (W32 || pass || j == p.E)) break;
-      double best = 0.0, bq = 0.0;
-      int at = INT32_MAX;
-#pragma unroll
-      for (int i = 0; i < kRouteMaxPerLane; ++i)
-        if (i < per && lane + 32 * i < p.E && !(used >> i & 1u) && (at == INT32_MAX || key[i] > best)) {
-          best = key[i];
-          bq = q[i];
-          at = lane + 32 * i;
-        }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double ob = __shfl_xor_sync(0xffffffffu, best, o), oq = __shfl_xor_sync(0xffffffffu, bq, o);
-        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-        if (oa != INT32_MAX && (at == INT32_MAX || ob > best || (ob == best && oa < at))) best = ob, bq = oq, at = oa;
-      }
-      if ((at & 31) == lane) used |= 1u << (at >> 5);
-      if (j < p.top && lane == j) chosen = at, score = bq;
-      if (!W32 && !pass) {
-#pragma unroll
-        for (int i = 0; i < kRouteMaxPerLane; ++i)
-          if (i < per) {
-            const int e = lane + 32 * i;
-            const double m = fmax(q[i], bq);
-            // Two logits' errors, each times the slope of the score: at most p, for the sigmoid p (1 - p).
-            const double slope = p.sigmoid ? m * (1.0 - fmin(q[i], bq)) + 1e-15 : 2.0 * m;
-            if (e < p.E && e != at && fabs(key[i] - best) < 2.0 * loss * slope) again |= 1u << i;
-          }
-      }
+      for (int e = lane; e < p.E; e += 32) sum += q[e] = exp(z[e] - top);
+      scale = 1.0 / warp_sum(sum);
     }
-    if (W32 || pass || !__any_sync(0xffffffffu, again != 0 || odd)) break;
-    // Sums again in fp64.  A token that is not finite itself keeps what the first sums gave.
+    // This lane's best expert not yet chosen.
+    unsigned used = 0;  // bit i: expert lane + 32 i
+    int at = -1;
+    double best = 0.0;
+    unsigned long long order = 0;
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += 32) {
+      const double v = p.sigmoid ? 1.0 / (1.0 + exp(-z[e])) : q[e] * scale;
+      q[e] = v;
+      const double key = route_key(p, v, e);
+      if (at < 0 || key > best) best = key, at = e;
+    }
+    order = at < 0 ? 0 : ordered(best);
+    // The k largest keys and the next one, equal ones by index.
+    double key = 0.0, rest = 0.0;  // lane j: the j-th key; the key after the last choice
+    const int want = W32 || pass || p.top == p.E ? p.top : p.top + 1;
+#pragma unroll 1
+    for (int j = 0; j < want; ++j) {
+      const unsigned hi = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(order >> 32));
+      bool mine = static_cast<unsigned>(order >> 32) == hi;
+      const unsigned lo = __reduce_max_sync(0xffffffffu, mine ? static_cast<unsigned>(order) : 0u);
+      mine = mine && static_cast<unsigned>(order) == lo;
+      const unsigned e = __reduce_min_sync(0xffffffffu, mine && at >= 0 ? static_cast<unsigned>(at) : 0xffffffffu);
+      const double kj = __shfl_sync(0xffffffffu, best, static_cast<int>(e & 31u));
+      if (j == p.top) {
+        rest = kj;
+        break;
+      }
+      if (lane == j) chosen = static_cast<int>(e), key = kj, score = q[e];
+      if (lane == static_cast<int>(e & 31u)) {
+        used |= 1u << (e >> 5);
+        at = -1;
+#pragma unroll 1
+        for (int f = lane; f < p.E; f += 32)
+          if (!(used >> (f >> 5) & 1u)) {
+            const double v = route_key(p, q[f], f);
+            if (at < 0 || v > best) best = v, at = f;
+          }
+        order = at < 0 ? 0 : ordered(best);
+      }
+      __syncwarp();
+    }
+    if (W32 || pass) break;
+    // Could the errors of two logits have swapped neighbours?  A score moves by at most its slope
+    // times a logit's error: p (1 - p) for the sigmoid, 2 p with softmax's normaliser.
+    const double after = __shfl_down_sync(0xffffffffu, key, 1);
+    const double next = lane == p.top - 1 ? rest : after;
+    const double slope = p.sigmoid ? 0.25 : 2.0 * score;
+    const bool last = lane == p.top - 1 && p.top == p.E;
+    const bool near = lane < p.top && !last && key - next <= 2.0 * loss * slope && loss > 0.0;
+    if (!__any_sync(0xffffffffu, near || odd)) break;
+    // Sums again in fp64, unless the token itself is not finite.
     const long long xo = static_cast<long long>(t) * p.ldx;
     bool finite = true;
+#pragma unroll 1
     for (int k = 8 * lane; k < p.K; k += 256) {
       const uint4 v = row_chunk(p.x, xo, k, p.K);
       const uint32_t r[4] = {v.x, v.y, v.z, v.w};
@@ -206,18 +207,30 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
       for (int i = 0; i < 4; ++i) finite = finite && isfinite(unpack_lo<BF16>(r[i])) && isfinite(unpack_hi<BF16>(r[i]));
     }
     if (!__all_sync(0xffffffffu, finite)) break;
-#pragma unroll
-    for (int i = 0; i < kRouteMaxPerLane; ++i)
-      if (i < per && lane + 32 * i < p.E && !isfinite(z[i])) again |= 1u << i;
-#pragma unroll
-    for (int i = 0; i < kRouteMaxPerLane; ++i) {
-      if (i >= per) continue;
-      unsigned todo = __ballot_sync(0xffffffffu, again >> i & 1u);
+    // Which: logits out of range, and experts whose key is as close to a chosen one's or to the
+    // next one's.  (Of two scores within reach of one another the chosen one's slope is the larger.)
+#pragma unroll 1
+    for (int base = 0; base < p.E; base += 32) {
+      const int e = base + lane;
+      const double ke = e < p.E ? route_key(p, q[e], e) : 0.0;
+      bool again = e < p.E && !isfinite(z[e]);
+#pragma unroll 1
+      for (int j = 0; j < p.top; ++j) {
+        const double kj = __shfl_sync(0xffffffffu, key, j), sj = __shfl_sync(0xffffffffu, slope, j);
+        const int cj = __shfl_sync(0xffffffffu, chosen, j);
+        again |= e < p.E && e != cj && fabs(ke - kj) <= 2.0 * loss * sj;
+        // (the chosen one itself, when its neighbour is that close)
+        const bool nj = __shfl_sync(0xffffffffu, near, j) || (j > 0 && __shfl_sync(0xffffffffu, near, j > 0 ? j - 1 : 0));
+        again |= e == cj && nj;
+      }
+      unsigned todo = __ballot_sync(0xffffffffu, again);
+#pragma unroll 1
       while (todo) {
         const int src = __ffs(todo) - 1;
         todo &= todo - 1;
-        const long long wo = static_cast<long long>(src + 32 * i) * p.ldw;
+        const long long wo = static_cast<long long>(base + src) * p.ldw;
         double a = 0.0, b = 0.0;
+#pragma unroll 1
         for (int k = 8 * lane; k < p.K; k += 512) {
           const uint4 xa = row_chunk(p.x, xo, k, p.K), wa = row_chunk(p.w, wo, k, p.K);
           const uint4 xb = row_chunk(p.x, xo, k + 256, p.K), wb = row_chunk(p.w, wo, k + 256, p.K);
@@ -225,9 +238,10 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
           b = dot8<BF16>(xb, wb, b);
         }
         a = warp_sum(a + b);
-        if (lane == src) z[i] = a;
+        if (lane == src) z[base + src] = a;
       }
     }
+    __syncwarp();
   }
   const double total = warp_sum(lane < p.top ? score : 0.0);
   if (lane < p.top) {
@@ -256,7 +270,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
     for (int i = 0; i < 2 * MT; ++i) xo[i] = static_cast<long long>(min(t0 + 8 * i + g, p.M - 1)) * p.ldx;
 #pragma unroll
     for (int j = 0; j < NT; ++j) wo[j] = static_cast<long long>(min(e0 + 8 * j + g, p.E - 1)) * p.ldw;
-#pragma unroll 2
+#pragma unroll(MT == 1 ? 4 : 1)
     for (int k0 = warp * kRouteStep; k0 < p.K; k0 += kRouteWarps * kRouteStep) {
       uint4 xv[2][2 * MT], wv[2][NT];
 #pragma unroll
@@ -342,7 +356,12 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   __syncthreads();
   if (!last) return;
   __threadfence();
-  for (int t = t0 + warp; t < min(t0 + 16 * MT, p.M); t += kRouteWarps) route_token<BF16, W32>(p, t, lane);
+  double* z_of = reinterpret_cast<double*>(smem) + 2 * warp * p.E;  // (the parts have been added up)
+#pragma unroll 1
+  for (int t = t0 + warp; t < min(t0 + 16 * MT, p.M); t += kRouteWarps) {
+    route_token<BF16, W32>(p, t, lane, z_of, z_of + p.E);
+    __syncwarp();
+  }
 }
 
 }  // namespace ffnb200
