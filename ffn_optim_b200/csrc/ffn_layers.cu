@@ -91,31 +91,39 @@ int encode(CUtensorMap* tm, const void* base, int dtype, int rank, const int64_t
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FFN_B200_OK : FFN_B200_ERR_CUDA;
 }
-// Weights [experts][halves][rows][cols] in boxes of 128 rows, or of 16 rows of both halves.
+// Weights [experts][halves][rows][cols] in boxes of `box_rows` rows of every half.
 int encode_weights(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int64_t rows, int64_t halves,
-                   int64_t experts, int64_t ld, int64_t stride) {
+                   int64_t experts, int64_t ld, int64_t stride, int box_rows) {
   const int64_t dims[4] = {cols, rows, halves, experts};
   const int64_t strides[3] = {ld, rows * ld, stride};
-  const uint32_t box[4] = {64, halves == 2 ? 16u : 128u, halves == 2 ? 2u : 1u, 1};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), static_cast<uint32_t>(halves), 1};
   return encode(tm, base, dtype, 4, dims, strides, box);
 }
-// Rows [rows][cols] for gathered loads (a box of one row).
-int encode_rows(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int64_t rows, int64_t ld) {
+// Rows [rows][cols] in boxes of `box_rows` (1: gathered loads).
+int encode_rows(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int64_t rows, int64_t ld, int box_rows) {
   const int64_t dims[2] = {cols, rows};
-  const uint32_t box[2] = {64, 1};
+  const uint32_t box[2] = {64, static_cast<uint32_t>(box_rows)};
   return encode(tm, base, dtype, 2, dims, &ld, box);
 }
 
 constexpr int kMaxSmem = 232448;
 
 int stream_chunk(int64_t tokens) { return tokens <= 16 ? 16 : (tokens <= 32 ? 32 : (tokens <= 64 ? 64 : 128)); }
-// Ring slots beside `list_bytes` of lists, and the dynamic shared memory they add up to.
-int stream_stages(int chunk, int list_bytes, int64_t* smem) {
-  const int stage = ffnb200::kABytes + chunk * 128, fixed = 1024 + ffnb200::kStreamBarBytes + list_bytes;
-  const int stages = std::min(ffnb200::kStreamMaxStages, (kMaxSmem - fixed) / stage);
-  *smem = static_cast<int64_t>(stages) * stage + fixed;
-  return stages;
-}
+// The ring beside `list_bytes` of lists: K steps per slot (of `slab` weight bytes and `chunk` token
+// rows each; about 32 KB, at most 4 steps), slots, and the dynamic shared memory they add up to.
+// (The MMA reads 128 rows from a slab's start.)
+struct StreamRing {
+  int blocks, stages;
+  int64_t smem;
+  StreamRing(int slab, int chunk, int list_bytes) {
+    const int step = slab + chunk * 128;
+    blocks = std::max(1, std::min(4, 36864 / step));
+    const int fixed = 1024 + ffnb200::kStreamBarBytes + list_bytes +
+                      std::max(0, ffnb200::kABytes - slab - blocks * chunk * 128);
+    stages = std::min(ffnb200::kStreamMaxStages, (kMaxSmem - fixed) / (blocks * step));
+    smem = static_cast<int64_t>(stages) * blocks * step + fixed;
+  }
+};
 
 using StreamFn = void (*)(const ffnb200::StreamParams);
 
@@ -243,16 +251,18 @@ int ffn_b200_linear_make_plan(const ffn_b200_linear_problem* pr, ffn_b200_linear
   std::memset(out, 0, sizeof(*out));
   const int grid = pr->block_num ? pr->block_num : sms;
   out->block_num = grid;
-  out->tile = pr->tile ? pr->tile : (pr->m <= 1024 ? 1 : 2);
+  if (pr->tile == 1 && pr->m > 128) return FFN_B200_ERR_INVALID;
+  out->tile = pr->tile ? pr->tile : (pr->m <= 128 ? 1 : 2);
+  out->workspace_floats = 4;
+  out->counter_words = 4;
   if (out->tile == 1) {
-    const int chunk = stream_chunk(pr->m);
-    out->tile_m = chunk;
-    out->tile_n = 128;
-    out->stages = stream_stages(chunk, 0, &out->smem_bytes);
-    out->workspace_floats = 2ll * grid * chunk * 128;
-    out->counter_words = grid;
-    const int64_t steps = cdiv(pr->n, 128) * cdiv(pr->m, chunk) * cdiv(pr->k, 64);
-    if (steps >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
+    // Equal numbers of weight rows per CTA, in tiles of at most 128.
+    const int64_t per_cta = cdiv(pr->n, static_cast<int64_t>(grid) * 128);
+    out->tile_m = static_cast<int32_t>(cdiv(pr->n, grid * per_cta));
+    out->tile_n = stream_chunk(pr->m);
+    const StreamRing ring(static_cast<int>(cdiv(out->tile_m, 8)) * 1024, out->tile_n, 0);
+    out->stages = ring.stages;
+    out->smem_bytes = ring.smem;
   }
   return FFN_B200_OK;
 }
@@ -283,18 +293,21 @@ int ffn_b200_linear_prepare(const ffn_b200_linear_problem* pr, const void* w, in
   if (plan.tile == 1) {
     ffnb200::StreamParams& P = h->params;
     std::memset(&P, 0, sizeof(P));
-    rc = encode_weights(&P.tm_w1, w, pr->dtype, pr->k, pr->n, 1, 1, ldw, pr->n * ldw);
+    const int rows = plan.tile_m;
+    rc = encode_weights(&P.tm_w1, w, pr->dtype, pr->k, pr->n, 1, 1, ldw, pr->n * ldw, rows);
     P.tokens = static_cast<int>(pr->m);
-    P.chunk = plan.tile_m;
-    P.items = static_cast<int>(cdiv(pr->m, P.chunk));
-    P.tiles1 = static_cast<int>(cdiv(pr->n, 128));
+    P.groups1 = static_cast<int>(cdiv(pr->n, rows));
+    P.group_rows = P.group_feats = rows;
+    P.unit_groups = 1;
     P.steps1 = static_cast<int>(cdiv(pr->k, 64));
     P.feat1 = static_cast<int>(pr->n);
-    P.stages = plan.stages;
+    P.slab = static_cast<int>(cdiv(rows, 8)) * 1024;
+    P.chunk = plan.tile_n;
+    const StreamRing ring(P.slab, P.chunk, 0);
+    P.blocks = ring.blocks;
+    P.stages = ring.stages;
     P.act = pr->activation;
     P.bias = static_cast<const uint16_t*>(bias);
-    P.partial1 = workspace;
-    P.counters = counters;
     P.wait_limit_ns = 4000000000ull;
     h->fn = pr->dtype == FFN_B200_BF16 ? ffnb200::stream_kernel<true, false> : ffnb200::stream_kernel<false, false>;
     if (!rc) rc = set_smem(reinterpret_cast<const void*>(h->fn), kMaxSmem);
@@ -316,7 +329,7 @@ int ffn_b200_linear_run(ffn_b200_linear* h, const void* x, int64_t ldx, const vo
   if (!scope.ok) return FFN_B200_ERR_DEVICE;
   if (h->plan.tile == 1) {
     ffnb200::StreamParams P = h->params;
-    const int rc = encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx);
+    const int rc = encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx, P.chunk);
     if (rc) return rc;
     P.residual = static_cast<const uint16_t*>(res);
     P.ldr = ldr;
@@ -390,15 +403,17 @@ int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* pr, ffn_b200_moe_plan* ou
   const ffnb200::StreamLists lists(tokens, pr->experts, pr->top_k);
   out->block_num = grid;
   out->chunk = stream_chunk(pr->m);
-  out->stages = stream_stages(out->chunk, lists.bytes, &out->smem_bytes);
+  const StreamRing ring(ffnb200::kABytes, out->chunk, lists.bytes);
+  out->stages = ring.stages;
+  out->smem_bytes = ring.smem;
   out->hidden_rows = pr->m * pr->top_k;
   out->hidden_pitch = pitch_of(pr->h);
   const int64_t slots = 2ll * grid * out->chunk * 128;
   const int64_t items = ffnb200::StreamLists::stream_items(tokens, pr->experts, pr->top_k);
-  const int64_t up = cdiv(pr->h, pr->activation == FFN_B200_SWIGLU ? 64 : 128), down = cdiv(pr->n, 128);
-  if (items * std::max(up * cdiv(pr->k, 64), down * cdiv(pr->h, 64)) >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
-  out->workspace_floats = 2 * slots + out->hidden_rows * down * 128;
-  out->counter_words = grid + ffnb200::kStreamSync + items;
+  const int64_t down = cdiv(pr->n, 128);
+  if (items * down * cdiv(pr->h, 64) >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
+  out->workspace_floats = slots + out->hidden_rows * down * 128;
+  out->counter_words = ffnb200::kStreamSync + items;
   out->status_words = 4;
   return FFN_B200_OK;
 }
@@ -432,25 +447,33 @@ int ffn_b200_moe_prepare(const ffn_b200_moe_problem* pr, const ffn_b200_moe_buff
   ffnb200::StreamParams& P = h->params;
   std::memset(&P, 0, sizeof(P));
   const bool glu = pr->activation == FFN_B200_SWIGLU;
-  rc = encode_weights(&P.tm_w1, b->w1, pr->dtype, pr->k, pr->h, glu ? 2 : 1, pr->experts, b->ldw1, b->stride1);
-  if (!rc) rc = encode_weights(&P.tm_w2, b->w2, pr->dtype, pr->h, pr->n, 1, pr->experts, b->ldw2, b->stride2);
-  if (!rc) rc = encode_rows(&P.tm_h, b->hidden, pr->dtype, pr->h, plan.hidden_rows, plan.hidden_pitch);
+  // Groups of 16 weight rows: 16 hidden features, or gate and up rows of 8.
+  P.group_rows = 16;
+  P.group_feats = glu ? 8 : 16;
+  P.unit_groups = 8;
+  P.slab = ffnb200::kABytes;
+  rc = encode_weights(&P.tm_w1, b->w1, pr->dtype, pr->k, pr->h, glu ? 2 : 1, pr->experts, b->ldw1, b->stride1,
+                      P.group_feats);
+  if (!rc)
+    rc = encode_weights(&P.tm_w2, b->w2, pr->dtype, pr->h, pr->n, 1, pr->experts, b->ldw2, b->stride2, 128);
+  if (!rc) rc = encode_rows(&P.tm_h, b->hidden, pr->dtype, pr->h, plan.hidden_rows, plan.hidden_pitch, 8);
   P.tokens = static_cast<int>(pr->m);
-  P.tiles1 = static_cast<int>(cdiv(pr->h, glu ? 64 : 128));
+  P.groups1 = static_cast<int>(cdiv(pr->h, P.group_feats));
   P.steps1 = static_cast<int>(cdiv(pr->k, 64));
   P.feat1 = static_cast<int>(pr->h);
   P.tiles2 = static_cast<int>(cdiv(pr->n, 128));
   P.steps2 = static_cast<int>(cdiv(pr->h, 64));
   P.feat2 = static_cast<int>(pr->n);
   P.chunk = plan.chunk;
-  P.stages = plan.stages;
+  const StreamRing ring(P.slab, P.chunk, ffnb200::StreamLists(P.tokens, pr->experts, pr->top_k).bytes);
+  P.blocks = ring.blocks;
+  P.stages = ring.stages;
   P.act = pr->activation;
   P.hidden = static_cast<uint16_t*>(b->hidden);
   P.ldh = plan.hidden_pitch;
   const int64_t slots = 2ll * plan.block_num * plan.chunk * 128;
-  P.partial1 = b->workspace;
-  P.partial2 = b->workspace + slots;
-  P.whole2 = b->workspace + 2 * slots;
+  P.pieces = b->workspace;
+  P.whole = b->workspace + slots;
   P.counters = b->counters;
   P.status = b->status;
   P.experts = pr->experts;
@@ -474,7 +497,7 @@ int ffn_b200_moe_run(ffn_b200_moe* h, const void* x, int64_t ldx, const int32_t*
   DeviceScope scope(h->device);
   if (!scope.ok) return FFN_B200_ERR_DEVICE;
   ffnb200::StreamParams P = h->params;
-  const int rc = encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx);
+  const int rc = encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx, 1);
   if (rc) return rc;
   P.ids = ids;
   P.weights = weights;

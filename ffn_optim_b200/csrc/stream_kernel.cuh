@@ -6,26 +6,27 @@
 //                Y_t = R_t + sum_j w_tj hidden_p . W2_e^T
 //
 // With few tokens every weight is used a few times only, so the floor is the weights' bytes over
-// HBM bandwidth.  The weight rows are the MMA's 128-row A operand and the tokens its N columns
-// (a multiple of 16, at most 128), so one K step of 64 moves 16 KB of weights for one
-// 128 x N x 64 product.  All CTAs (one per SM) read equal stretches of the weights:
+// HBM bandwidth.  The weight rows are the MMA's A operand (up to 128 rows) and the tokens its N
+// columns (a multiple of 16, at most 128); a K step is 64 columns of both, and a ring slot holds
+// `blocks` of them (a wait on a barrier costs its thread about 150 clocks, which small slots would
+// spend per step).
 //
-//   A phase is `items` x `tiles` x L steps (item: an expert's tokens, or a chunk of the
-//   projection's; tile: 128 weight rows; step: 64 of K) in one line; CTA c takes the stretch
-//   [T c / C, T (c+1) / C).  A stretch that covers a tile's whole K goes straight to the epilogue;
-//   a tile cut by a stretch's end is summed from fp32 partials in ascending CTA order, which
-//   keeps results the same from run to run.
-//
-//   Projection and experts' first product: every CTA that shares a tile writes its partial and
-//   counts up; the one that counts last adds them all and finishes the tile, so nobody waits.
-//   Experts' second product: partials are added in the final combination over the token's
-//   experts, which starts when all CTAs have counted (the one grid-wide wait; cooperative launch).
-//   A second-product step waits for its item's hidden rows; the weight half of the ring (A) runs
-//   ahead of that wait, so HBM stays busy across the change of phase.
+// First product (the only one of the projection): the weight rows are dealt out evenly over the
+// CTAs (one per SM) in groups -- the projection's rows / CTAs, or 16 rows of an expert -- and a
+// CTA takes each of its tiles over the whole of K, so no sum is ever split between CTAs.
+// Second product (experts): a line of items x tiles of 128 rows x K steps of 64 is cut into equal
+// stretches.  An uncut tile goes to memory whole; of a cut one every CTA leaves its fp32 piece, and
+// the final combination over the token's experts adds the pieces in ascending CTA order, which
+// keeps results the same from run to run.  It starts when all CTAs have counted (the one
+// grid-wide wait; cooperative launch).  A second-product step waits for its item's hidden
+// rows; the weight half of the ring (A) runs ahead of that wait, so HBM stays busy across the
+// change of product.
 //
 // Roles: warp 0 weight loads (TMA), warp 1 MMA issue (tcgen05, accumulators in two TMEM halves),
-// warp 2 token rows (TMA gather of four rows per instruction), warps 4-7 epilogue.  Every wait is
-// bounded as in ffn_kernel.cuh.
+// warp 2 token rows (TMA; the experts' first product gathers four per instruction), warps 4-7
+// epilogue.  Each of the first three is one thread that its warp elects: TMA and MMA instructions
+// then issue every 12 to 35 clocks, where they took 45 behind a test of the lane number.  Every
+// wait is bounded as in ffn_kernel.cuh.
 #pragma once
 
 #include "ffn_kernel.cuh"
@@ -33,17 +34,23 @@
 namespace ffnb200 {
 
 constexpr int kStreamThreads = 256;
-constexpr int kStreamMaxStages = 12;
-constexpr int kStreamMinSteps = 4;   // fewest K steps worth a CTA of their own
-constexpr int kStreamBarBytes = 512;
+constexpr int kStreamMaxStages = 40;
+constexpr int kStreamMinSteps = 4;   // fewest K steps of the second product worth a CTA of their own
+constexpr int kStreamBarBytes = 1024;
 
 struct StreamParams {
-  CUtensorMap tm_w1, tm_w2;  // weights [E][halves][rows][K]: box 64 x 128 rows, or 64 x 16 x 2 halves (SwiGLU)
-  CUtensorMap tm_x, tm_h;    // token rows, box 64 x 1 (gathered)
-  int tokens, items;         // items: the projection's token chunks (experts: found on the device)
-  int tiles1, steps1, feat1; // first product: tiles per item, K steps per tile, output features
+  CUtensorMap tm_w1, tm_w2;  // weights [E][halves][rows][K]: a box is one group's rows (SwiGLU: 8 of
+                             // both halves), or 128 rows of the second product
+  CUtensorMap tm_x, tm_h;    // token rows: the projection's in one box, the experts' in boxes of one
+                             // row (gathered); hidden rows in boxes of 8
+  int tokens;
+  int groups1, group_rows, group_feats, unit_groups;  // first product: row groups per item, weight rows and
+                             // output features of a group, groups of one tile at most
+  int steps1, feat1;         // K steps; output features
   int tiles2, steps2, feat2; // second product (experts)
-  int chunk, stages;         // tokens per item at most (16, 32, 64 or 128); ring slots
+  int slab;                  // bytes of a step's weights in a ring slot (a multiple of 1024)
+  int chunk;                 // tokens per item at most (16, 32, 64 or 128)
+  int blocks, stages;        // K steps per ring slot; ring slots
   int act;                   // ffn_b200_gelu
   const uint16_t* bias;      // projection, optional [N]
   const uint16_t* residual;  // optional
@@ -52,10 +59,9 @@ struct StreamParams {
   long long ldy;
   uint16_t* hidden;          // experts: [pair][ldh], pairs ordered by expert, then token
   long long ldh;
-  float* partial1;           // [2 C][chunk][128] partial tiles of the first product
-  float* partial2;           // same for the second
-  float* whole2;             // [pair][tiles2 * 128] uncut tiles of the second product
-  unsigned* counters;        // [C] arrivals at cut tiles, then kStreamSync words, then items' finished tiles
+  float* pieces;             // [2 C][chunk][128] pieces of cut tiles of the second product
+  float* whole;              // [pair][tiles2 * 128] its uncut tiles
+  unsigned* counters;        // kStreamSync words, then the items' finished groups
   int* status;
   const int* ids;            // experts: [tokens][top]
   const float* weights;
@@ -86,17 +92,19 @@ struct StreamLists {
   }
 };
 
-// One row stretch [s0, s1) of a phase with T steps over `ctas` CTAs, and the CTA of a step.
+// `total` things in a line dealt out over at most `grid` CTAs in even stretches of at least `least`.
 struct StreamSplit {
-  long long T;
+  long long total;
   int ctas;
-  __device__ StreamSplit(long long total, int grid) : T(total) {
-    const long long most = total / kStreamMinSteps;
+  __device__ StreamSplit(long long n, int grid, int least) : total(n) {
+    const long long most = n / least;
     ctas = most < 1 ? 1 : (most < grid ? static_cast<int>(most) : grid);
   }
-  __device__ int begin(int c) const { return c >= ctas ? static_cast<int>(T) : static_cast<int>(T * c / ctas); }
-  __device__ int cta_of(int step) const {
-    return static_cast<int>(((static_cast<long long>(step) + 1) * ctas - 1) / T);
+  __device__ int begin(int c) const {
+    return c >= ctas ? static_cast<int>(total) : static_cast<int>(total * c / ctas);
+  }
+  __device__ int cta_of(int i) const {
+    return static_cast<int>(((static_cast<long long>(i) + 1) * ctas - 1) / total);
   }
 };
 
@@ -115,6 +123,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
+}
+// One lane of a converged warp, as the compiler knows a single one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r != 0;
 }
 // All 128 epilogue threads meet; true when every one brought true.
 __device__ __forceinline__ int epilogue_all(int ok) {
@@ -182,7 +196,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
   const int ST = p.stages;
-  const uint32_t stage_bytes = kABytes + static_cast<uint32_t>(p.chunk) * 128u;
+  const uint32_t slab = static_cast<uint32_t>(p.slab);
+  const uint32_t token_bytes = static_cast<uint32_t>(p.chunk) * 128u;
+  const int KS = p.blocks;
+  const uint32_t stage_bytes = KS * (slab + token_bytes);
   const uint32_t sBar = base + ST * stage_bytes;
   uint8_t* ctrl = gbase + ST * stage_bytes;
   auto full_bar = [&](int s) { return sBar + 8u * s; };
@@ -221,7 +238,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
-    *n_items = p.items;
+    *n_items = 1;
     fence_barrier_init();
     fence_async_shared();
   }
@@ -301,14 +318,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   }
 
   const int items = *n_items;
-  unsigned* arrivals = p.counters;
-  unsigned* sync_words = p.counters + C;
+  unsigned* sync_words = p.counters;
   unsigned* item_done = sync_words + kStreamSync;
-  const int phases = MOE ? 2 : 1;
-  // Unit u of a phase: the projection takes its token chunks innermost, so that CTAs next to one
-  // another share a weight tile; the experts' units are item-major.
-  auto unit_item = [&](int u, int tiles) { return MOE ? u / tiles : u % items; };
-  auto unit_tile = [&](int u, int tiles) { return MOE ? u % tiles : u / items; };
+  const bool glu = MOE && p.act == 3;
   auto item_of = [&](int it, int& expert, int& start, int& count) {
     if constexpr (MOE) {
       const uint2 v = item_list[it];
@@ -316,53 +328,67 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       count = static_cast<int>(v.x >> 16);
       start = static_cast<int>(v.y);
     } else {
-      expert = 0;
-      start = it * p.chunk;
-      count = min(p.chunk, p.tokens - start);
+      expert = 0, start = 0, count = p.tokens;
+    }
+  };
+  // This CTA's tiles, in the same order for every role: tile(ph, item, g0, groups, k0, k1) returns
+  // false to stop.  First product: groups [g0, g0 + groups) of the item over all of K.  Second:
+  // tile g0, K steps [k0, k1).
+  auto for_tiles = [&](auto&& tile) {
+    if (items == 0) return;
+    const StreamSplit rows(static_cast<long long>(items) * p.groups1, C, 1);
+    for (int g = rows.begin(c), end = rows.begin(c + 1); g < end;) {
+      const int it = g / p.groups1, g0 = g - it * p.groups1;
+      const int n = min(min(p.unit_groups, p.groups1 - g0), end - g);
+      if (!tile(0, it, g0, n, 0, p.steps1)) return;
+      g += n;
+    }
+    if constexpr (MOE) {
+      const StreamSplit line(static_cast<long long>(items) * p.tiles2 * p.steps2, C, kStreamMinSteps);
+      for (int s = line.begin(c), end = line.begin(c + 1); s < end;) {
+        const int u = s / p.steps2, k0 = s - u * p.steps2, k1 = min(p.steps2, k0 + end - s);
+        const int it = u / p.tiles2;
+        if (!tile(1, it, u - it * p.tiles2, 1, k0, k1)) return;
+        s += k1 - k0;
+      }
     }
   };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ weight loads
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       long long issued = 0;
-      bool ok = true;
+      const uint32_t box_bytes = static_cast<uint32_t>(p.group_rows) * 128u;
+      for_tiles([&](int ph, int it, int g0, int n, int k0, int k1) {
+        int expert, start, count;
+        item_of(it, expert, start, count);
+        const uint32_t bytes = ph ? static_cast<uint32_t>(kABytes) : box_bytes * n;
 #pragma unroll 1
-      for (int ph = 0; ph < phases && ok; ++ph) {
-        const int tiles = ph ? p.tiles2 : p.tiles1, L = ph ? p.steps2 : p.steps1;
-        const StreamSplit split(static_cast<long long>(items) * tiles * L, C);
-        const int end = items ? split.begin(c + 1) : 0;
-        int s = items ? split.begin(c) : 0;
-        const CUtensorMap* tm = ph ? &p.tm_w2 : &p.tm_w1;
-        const bool glu = ph == 0 && p.act == 3;
+        for (int kb = k0; kb < k1; kb += KS) {
+          const int nb = min(KS, k1 - kb);
+          if (!stream_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, 100 + stage)) return false;
+          const uint32_t dst = base + stage * stage_bytes;
+          mbar_expect_tx(full_bar(stage), bytes * nb);
 #pragma unroll 1
-        while (s < end && ok) {
-          const int u = s / L, k0 = s - u * L, k1 = min(L, k0 + end - s);
-          int expert, start, count;
-          item_of(unit_item(u, tiles), expert, start, count);
-          const int tile = unit_tile(u, tiles);
-#pragma unroll 1
-          for (int kb = k0; kb < k1; ++kb) {
-            if (!stream_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, 100 + stage)) { ok = false; break; }
-            const uint32_t dst = base + stage * stage_bytes;
-            mbar_expect_tx(full_bar(stage), kABytes);
-            if (glu) {  // rows 32 w + (0..15) gate, (16..31) up: a warp's TMEM lanes hold both
-#pragma unroll
-              for (int w = 0; w < 4; ++w)
-                tma_load_4d(dst + w * 4096, tm, kb * kBK, tile * 64 + 16 * w, 0, expert, full_bar(stage));
+          for (int i = 0; i < nb; ++i) {
+            if (MOE && ph) {
+              tma_load_4d(dst + i * slab, &p.tm_w2, (kb + i) * kBK, g0 * kBM, 0, expert, full_bar(stage));
             } else {
-              tma_load_4d(dst, tm, kb * kBK, tile * kBM, 0, expert, full_bar(stage));
+#pragma unroll 1
+              for (int j = 0; j < n; ++j)
+                tma_load_4d(dst + i * slab + j * box_bytes, &p.tm_w1, (kb + i) * kBK, (g0 + j) * p.group_feats, 0, expert,
+                            full_bar(stage));
             }
-            ++issued;
-            if (++stage == ST) { stage = 0; phase ^= 1u; }
           }
-          s += k1 - k0;
+          ++issued;
+          if (++stage == ST) { stage = 0; phase ^= 1u; }
         }
-      }
+        return true;
+      });
       // Every load lands before the CTA may leave.  After an abort the token rows of a slot may
-      // never have been asked for and its barrier never completes: wait for the limit then.
+      // never have been asked for and its barrier never completes: a millisecond then.
       const uint64_t t0 = gtimer();
       bool late = false;
       for (long long i = issued > ST ? issued - ST : 0; i < issued && !late; ++i)
@@ -371,44 +397,41 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       int n_acc = 0;
-      bool ok = true;
+      for_tiles([&](int, int it, int, int, int k0, int k1) {
+        int expert, start, count;
+        item_of(it, expert, start, count);
+        const uint32_t idesc = make_idesc<BF16, 0, kBM>() | static_cast<uint32_t>((count + 15) / 16 * 2) << 17;
+        const int b = n_acc & 1;
+        if (!stream_wait(acc_empty(b), ((n_acc >> 1) & 1) ^ 1u, abort_flag, p, 200 + b)) return false;
+        tc_fence_after();
+        const uint32_t d = tmem_base + static_cast<uint32_t>(b * p.chunk);
 #pragma unroll 1
-      for (int ph = 0; ph < phases && ok; ++ph) {
-        const int tiles = ph ? p.tiles2 : p.tiles1, L = ph ? p.steps2 : p.steps1;
-        const StreamSplit split(static_cast<long long>(items) * tiles * L, C);
-        const int end = items ? split.begin(c + 1) : 0;
-        int s = items ? split.begin(c) : 0;
-#pragma unroll 1
-        while (s < end && ok) {
-          const int u = s / L, k0 = s - u * L, k1 = min(L, k0 + end - s);
-          int expert, start, count;
-          item_of(unit_item(u, tiles), expert, start, count);
-          const uint32_t idesc = make_idesc<BF16, 0, kBM>() | static_cast<uint32_t>((count + 15) / 16 * 2) << 17;
-          const int b = n_acc & 1;
-          if (!stream_wait(acc_empty(b), ((n_acc >> 1) & 1) ^ 1u, abort_flag, p, 200 + b)) { ok = false; break; }
+        for (int kb = k0; kb < k1; kb += KS) {
+          const int nb = min(KS, k1 - kb);
+          if (!stream_wait(full_bar(stage), phase, abort_flag, p, 300 + stage)) return false;
           tc_fence_after();
-          const uint32_t d = tmem_base + static_cast<uint32_t>(b * p.chunk);
+          // (A tile of fewer than 128 rows reads on into what lies behind: its TMEM lanes are not used.)
+          uint64_t da = sw128_desc(base + stage * stage_bytes);
+          uint64_t db = sw128_desc(base + stage * stage_bytes + KS * slab);
 #pragma unroll 1
-          for (int kb = k0; kb < k1; ++kb) {
-            if (!stream_wait(full_bar(stage), phase, abort_flag, p, 300 + stage)) { ok = false; break; }
-            tc_fence_after();
-            const uint64_t da = sw128_desc(base + stage * stage_bytes);
-            const uint64_t db = sw128_desc(base + stage * stage_bytes + kABytes);
+          for (int i = 0; i < nb; ++i) {
 #pragma unroll
-            for (int k = 0; k < kBK / 16; ++k) umma_f16(d, da + 2 * k, db + 2 * k, idesc, kb > k0 || k > 0 ? 1u : 0u);
-            umma_commit(empty_bar(stage));
-            if (++stage == ST) { stage = 0; phase ^= 1u; }
+            for (int k = 0; k < kBK / 16; ++k)
+              umma_f16(d, da + 2 * k, db + 2 * k, idesc, kb > k0 || i > 0 || k > 0 ? 1u : 0u);
+            da += slab >> 4;
+            db += token_bytes >> 4;
           }
-          if (!ok) break;
-          umma_commit(acc_full(b));
-          ++n_acc;
-          s += k1 - k0;
+          umma_commit(empty_bar(stage));
+          if (++stage == ST) { stage = 0; phase ^= 1u; }
         }
-      }
+        umma_commit(acc_full(b));
+        ++n_acc;
+        return true;
+      });
       umma_commit(drain_bar);
       const uint64_t t0 = gtimer();
       while (!mbar_try_wait(drain_bar, 0))
@@ -416,54 +439,55 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ token rows
-    int stage = 0;
-    uint32_t phase = 0;
-    int ok = 1;
-#pragma unroll 1
-    for (int ph = 0; ph < phases && ok; ++ph) {
-      const int tiles = ph ? p.tiles2 : p.tiles1, L = ph ? p.steps2 : p.steps1;
-      const StreamSplit split(static_cast<long long>(items) * tiles * L, C);
-      const int end = items ? split.begin(c + 1) : 0;
-      int s = items ? split.begin(c) : 0;
-      const CUtensorMap* tm = ph ? &p.tm_h : &p.tm_x;
-#pragma unroll 1
-      while (s < end && ok) {
-        const int u = s / L, k0 = s - u * L, k1 = min(L, k0 + end - s);
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for_tiles([&](int ph, int it, int, int, int k0, int k1) {
         int expert, start, count;
-        const int it = unit_item(u, tiles);
         item_of(it, expert, start, count);
-        const int groups = (count + 3) / 4;
-        int r[4];  // this lane's four rows; a group that runs past the item repeats its last row
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = start + min(4 * lane + j, count - 1);
-          r[j] = MOE && ph == 0 ? token_of[at] : at;
-        }
         if (MOE && ph == 1) {
-          if (lane == 0)
-            ok = stream_wait_word(item_done + it, static_cast<unsigned>(p.tiles1 + (p.inject ? 1 : 0)), abort_flag, p, 2, it);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
+          ok = stream_wait_word(item_done + it, static_cast<unsigned>(p.groups1 + (p.inject ? 1 : 0)), abort_flag, p, 2, it);
+          if (!ok) return false;
           fence_async_global();  // hidden rows written by other CTAs' threads, read by this one's TMA
         }
+        const uint32_t bytes = !MOE ? token_bytes : (ph ? (count + 7) / 8 * 1024u : (count + 3) / 4 * 512u);
 #pragma unroll 1
-        for (int kb = k0; kb < k1; ++kb) {
-          if (lane == 0) ok = stream_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, 120 + stage) ? 1 : 0;
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(full_bar(stage), static_cast<uint32_t>(groups) * 512u);
-          __syncwarp();
-          if (lane < groups)
-            tma_gather4(base + stage * stage_bytes + kABytes + lane * 512u, tm, kb * kBK, r[0], r[1], r[2], r[3],
-                        full_bar(stage));
+        for (int kb = k0; kb < k1; kb += KS) {
+          const int nb = min(KS, k1 - kb);
+          ok = stream_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, 150 + stage);
+          if (!ok) return false;
+          const uint32_t bar = full_bar(stage);
+          const uint32_t dst = base + stage * stage_bytes + KS * slab;
+          mbar_expect_tx(bar, bytes * nb);
+          if (!MOE) {
+#pragma unroll 1
+            for (int i = 0; i < nb; ++i) tma_load_2d(dst + i * token_bytes, &p.tm_x, (kb + i) * kBK, 0, bar);
+          } else if (ph) {  // (rows behind the item's last belong to columns nobody reads)
+#pragma unroll 1
+            for (int r = 0; r < count; r += 8)
+#pragma unroll 1
+              for (int i = 0; i < nb; ++i)
+                tma_load_2d(dst + i * token_bytes + r * 128, &p.tm_h, (kb + i) * kBK, start + r, bar);
+          } else {
+#pragma unroll 1
+            for (int r = 0; r < count; r += 4) {  // (a group that runs past the item repeats its last row)
+              const int last = count - 1;
+              const int r0 = token_of[start + r], r1 = token_of[start + min(r + 1, last)];
+              const int r2 = token_of[start + min(r + 2, last)], r3 = token_of[start + min(r + 3, last)];
+#pragma unroll 1
+              for (int i = 0; i < nb; ++i)
+                tma_gather4(dst + i * token_bytes + r * 128, &p.tm_x, (kb + i) * kBK, r0, r1, r2, r3, bar);
+            }
+          }
           if (++stage == ST) { stage = 0; phase ^= 1u; }
         }
-        s += k1 - k0;
-      }
-    }
-    if (!ok) {  // (token rows asked for before the abort land before the CTA leaves)
-      const uint64_t t0 = gtimer();
-      while (gtimer() - t0 < 1000000ull) {
+        return true;
+      });
+      if (!ok) {  // (token rows asked for before the abort land before the CTA leaves)
+        const uint64_t t0 = gtimer();
+        while (gtimer() - t0 < 1000000ull) {
+        }
       }
     }
   } else if (warp >= 4) {
@@ -472,135 +496,89 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     const uint32_t lane_off = static_cast<uint32_t>(sub * 32) << 16;
     const int row = sub * 32 + lane;  // weight row of the tile
     int n_acc = 0;
-    int ok = 1;
+    for_tiles([&](int ph, int it, int g0, int n, int k0, int k1) {
+      int expert, start, count;
+      item_of(it, expert, start, count);
+      const int b = n_acc & 1;
+      int ok = 1;
+      if (lane == 0) ok = stream_wait(acc_full(b), (n_acc >> 1) & 1, abort_flag, p, 400 + b) ? 1 : 0;
+      if (!epilogue_all(lane != 0 || ok)) return false;
+      tc_fence_after();
+      const uint32_t acc = tmem_base + lane_off + static_cast<uint32_t>(b * p.chunk);
+      if (MOE && ph == 1) {
+        // fp32 sums [token][128 rows]: a piece, or a whole tile.
+        size_t pitch = kBM;
+        float* dst;
+        if (k0 > 0 || k1 < p.steps2) {
+          dst = p.pieces + (2 * static_cast<size_t>(c) + (k0 == 0 ? 1 : 0)) * static_cast<size_t>(p.chunk) * kBM;
+        } else {
+          pitch = static_cast<size_t>(p.tiles2) * kBM;
+          dst = p.whole + static_cast<size_t>(start) * pitch + static_cast<size_t>(g0) * kBM;
+        }
 #pragma unroll 1
-    for (int ph = 0; ph < phases && ok; ++ph) {
-      const int tiles = ph ? p.tiles2 : p.tiles1, L = ph ? p.steps2 : p.steps1;
-      const StreamSplit split(static_cast<long long>(items) * tiles * L, C);
-      const int end = items ? split.begin(c + 1) : 0;
-      int s = items ? split.begin(c) : 0;
+        for (int c0 = 0; c0 < count; c0 += 16) {
+          float v[16];
+          tmem_ld16(acc + c0, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < count) __stcg(dst + static_cast<size_t>(c0 + j) * pitch + row, v[j]);
+        }
+      } else {
+        // SwiGLU: of a group's 16 rows the first 8 are gates, the others the matching up rows.
+        const int feature = glu ? (g0 + (row >> 4)) * p.group_feats + (row & 7) : g0 * p.group_feats + row;
+        const bool live = row < n * p.group_rows && feature < p.feat1;
+        const float bias = !MOE && p.bias && live ? unpack_lo<BF16>(static_cast<uint32_t>(__ldg(p.bias + feature))) : 0.f;
 #pragma unroll 1
-      while (s < end && ok) {
-        const int u = s / L, k0 = s - u * L, k1 = min(L, k0 + end - s);
-        int expert, start, count;
-        const int it = unit_item(u, tiles), tile = unit_tile(u, tiles);
-        item_of(it, expert, start, count);
-        const int b = n_acc & 1;
-        if (lane == 0) ok = stream_wait(acc_full(b), (n_acc >> 1) & 1, abort_flag, p, 400 + b) ? 1 : 0;
-        ok = epilogue_all(lane != 0 || ok);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t acc = tmem_base + lane_off + static_cast<uint32_t>(b * p.chunk);
-        const bool cut = k0 > 0 || k1 < L;
-        if (cut || (MOE && ph == 1)) {
-          // Partial sums, or an uncut tile of the experts' second product: [token][128 rows] fp32.
-          float* dst;
-          size_t pitch = kBM;
-          if (cut) {
-            dst = (ph ? p.partial2 : p.partial1) +
-                  (2 * static_cast<size_t>(c) + (k0 == 0 ? 1 : 0)) * static_cast<size_t>(p.chunk) * kBM;
-          } else {
-            pitch = static_cast<size_t>(p.tiles2) * kBM;
-            dst = p.whole2 + static_cast<size_t>(start) * pitch + static_cast<size_t>(tile) * kBM;
-          }
-#pragma unroll 1
-          for (int c0 = 0; c0 < count; c0 += 16) {
-            float v[16];
+        for (int c0 = 0; c0 < count; c0 += 16) {
+          float v[16];
+          if constexpr (MOE) {
             tmem_ld16(acc + c0, v);
+            if (glu) {
+              // Lane l holds a gate row, lane l + 8 the matching up row: of each column pair the
+              // lower lane finishes the first, the upper lane the second.
+              const bool low = (lane & 8) == 0;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c0 + j < count) __stcg(dst + static_cast<size_t>(c0 + j) * pitch + row, v[j]);
-          }
-        }
-        int finish = !cut && !(MOE && ph == 1);
-        int c_first = c, c_last = c;
-        if (cut && !(MOE && ph == 1)) {
-          // The CTA that arrives last at this tile finishes it.
-          c_first = split.cta_of(u * L);
-          c_last = split.cta_of(u * L + L - 1);
-          __threadfence();
-          epilogue_all(1);
-          if (threadIdx.x == 128) {
-            const unsigned old = atom_add_acq_rel(arrivals + c_first, 1u);
-            const int last = old == static_cast<unsigned>(c_last - c_first);
-            if (last) arrivals[c_first] = 0;  // for the next launch
-            *last_flag = last;
-          }
-          epilogue_all(1);
-          finish = *last_flag;
-          __threadfence();
-        }
-        if (finish) {
-          const bool glu = MOE && p.act == 3;
-          const int feature = glu ? tile * 64 + sub * 16 + (lane & 15) : tile * kBM + row;
-          const bool live = feature < p.feat1;
-          const float bias = !MOE && p.bias && live ? unpack_lo<BF16>(static_cast<uint32_t>(__ldg(p.bias + feature))) : 0.f;
-#pragma unroll 1
-          for (int c0 = 0; c0 < count; c0 += 16) {
-            float v[16];
-            if (!cut) {
-              tmem_ld16(acc + c0, v);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = 0.f;
-#pragma unroll 1
-              for (int q = c_first; q <= c_last; ++q) {
-                // (the first CTA's stretch begins the tile: its second slot)
-                const float* src = p.partial1 +
-                                   (2 * static_cast<size_t>(q) + (q == c_first ? 1 : 0)) * static_cast<size_t>(p.chunk) * kBM +
-                                   row;
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  if (c0 + j < count) v[j] += __ldcg(src + static_cast<size_t>(c0 + j) * kBM);
-              }
-            }
-            if constexpr (MOE) {
-              if (glu) {
-                // Lane l < 16 holds gate row l, lane l + 16 the matching up row: of each column
-                // pair the lower lane finishes the first, the upper lane the second.
-#pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                  const float got = __shfl_xor_sync(0xffffffffu, lane < 16 ? v[j + 1] : v[j], 16);
-                  const float gate = lane < 16 ? v[j] : got, up = lane < 16 ? got : v[j + 1];
-                  const int col = c0 + j + (lane < 16 ? 0 : 1);
-                  if (live && col < count)
-                    p.hidden[static_cast<long long>(start + col) * p.ldh + feature] = cvt1<BF16>(silu(gate) * up);
-                }
-              } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  if (live && c0 + j < count)
-                    p.hidden[static_cast<long long>(start + c0 + j) * p.ldh + feature] = cvt1<BF16>(act_value(v[j], p.act));
+              for (int j = 0; j < 16; j += 2) {
+                const float got = __shfl_xor_sync(0xffffffffu, low ? v[j + 1] : v[j], 8);
+                const float gate = low ? v[j] : got, up = low ? got : v[j + 1];
+                const int col = c0 + j + (low ? 0 : 1);
+                if (live && col < count)
+                  p.hidden[static_cast<long long>(start + col) * p.ldh + feature] = cvt1<BF16>(silu(gate) * up);
               }
             } else {
-              float r[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                r[j] = p.residual && live && c0 + j < count
-                           ? unpack_lo<BF16>(static_cast<uint32_t>(
-                                 __ldg(p.residual + static_cast<long long>(start + c0 + j) * p.ldr + feature)))
-                           : 0.f;
 #pragma unroll
               for (int j = 0; j < 16; ++j)
                 if (live && c0 + j < count)
-                  p.y[static_cast<long long>(start + c0 + j) * p.ldy + feature] =
-                      cvt1<BF16>(act_value(v[j] + bias, p.act) + r[j]);
+                  p.hidden[static_cast<long long>(start + c0 + j) * p.ldh + feature] = cvt1<BF16>(act_value(v[j], p.act));
             }
-          }
-          if constexpr (MOE) {
-            fence_async_global();  // hidden: written here, read through other CTAs' TMA
-            __threadfence();
-            epilogue_all(1);
-            if (threadIdx.x == 128) red_release_add(item_done + it, 1u);
+          } else {
+            float r[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              r[j] = p.residual && live && c0 + j < count
+                         ? unpack_lo<BF16>(static_cast<uint32_t>(
+                               __ldg(p.residual + static_cast<long long>(c0 + j) * p.ldr + feature)))
+                         : 0.f;
+            tmem_ld16(acc + c0, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (live && c0 + j < count)
+                p.y[static_cast<long long>(c0 + j) * p.ldy + feature] = cvt1<BF16>(act_value(v[j] + bias, p.act) + r[j]);
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty(b));
-        ++n_acc;
-        s += k1 - k0;
+        if constexpr (MOE) {
+          fence_async_global();  // hidden: written here, read through other CTAs' TMA
+          __threadfence();
+          epilogue_all(1);
+          if (threadIdx.x == 128) red_release_add(item_done + it, static_cast<unsigned>(n));
+        }
       }
-    }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(b));
+      ++n_acc;
+      return true;
+    });
   }
 
   tc_fence_before();
@@ -620,15 +598,25 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     __syncthreads();
     if (!*abort_flag) {
       __threadfence();
-      const StreamSplit split(static_cast<long long>(items) * p.tiles2 * p.steps2, C);
-      const int L = p.steps2;
-      const size_t whole_pitch = static_cast<size_t>(p.tiles2) * kBM;
-      for (long long unit = static_cast<long long>(warp) * C + c; unit < static_cast<long long>(p.tokens) * p.tiles2;
-           unit += static_cast<long long>(C) * (kStreamThreads / 32)) {
-        const int t = static_cast<int>(unit / p.tiles2), tile = static_cast<int>(unit % p.tiles2);
-        // Lane j knows choice j: its weight, the first piece's address and the pieces' count.
+      const StreamSplit line(static_cast<long long>(items) * p.tiles2 * p.steps2, C, kStreamMinSteps);
+      const size_t pitch = static_cast<size_t>(p.tiles2) * kBM;
+      const size_t slot = static_cast<size_t>(p.chunk) * kBM;
+      const int n_units = p.tokens * p.tiles2;
+#pragma unroll 1
+      for (int unit = warp * C + c; unit < n_units; unit += C * (kStreamThreads / 32)) {
+        const int t = unit / p.tiles2, tile = unit - t * p.tiles2;
+        // The residual first: it does not depend on anything read here.
+        float r4[4] = {0.f, 0.f, 0.f, 0.f};
+        const int f0 = tile * kBM + 4 * lane;
+        if (p.residual) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (f0 + q < p.feat2)
+              r4[q] = unpack_lo<BF16>(static_cast<uint32_t>(__ldg(p.residual + static_cast<long long>(t) * p.ldr + f0 + q)));
+        }
+        // Lane j knows choice j: its weight, its pieces and where the first one lies.
         const float* src = nullptr;
-        int pieces = 0, c_first = 0;
+        int pieces = 0;
         float wt = 0.f;
         if (lane < p.top) {
           const int e = __ldg(p.ids + t * p.top + lane);
@@ -637,43 +625,54 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
             int rank = 0;
             for (int w = 0; w < (t >> 5); ++w) rank += __popc(sets[e * lists.words + w]);
             rank += __popc(sets[e * lists.words + (t >> 5)] & ((1u << (t & 31)) - 1u));
-            const int it = first[e] + rank / p.chunk;
-            const int u = it * p.tiles2 + tile;
-            c_first = split.cta_of(u * L);
-            pieces = split.cta_of(u * L + L - 1) - c_first + 1;
-            if (pieces == 1)
-              src = p.whole2 + static_cast<size_t>(offset[e] + rank) * whole_pitch + static_cast<size_t>(tile) * kBM;
-            else
-              src = p.partial2 + static_cast<size_t>(rank % p.chunk) * kBM;
+            const int chunk_of = rank / p.chunk;
+            const int s = ((first[e] + chunk_of) * p.tiles2 + tile) * p.steps2;
+            const int c_first = line.cta_of(s);
+            pieces = line.cta_of(s + p.steps2 - 1) - c_first + 1;
+            src = pieces == 1 ? p.whole + static_cast<size_t>(offset[e] + rank) * pitch + static_cast<size_t>(tile) * kBM
+                              : p.pieces + (2 * static_cast<size_t>(c_first) + 1) * slot +
+                                    static_cast<size_t>(rank - chunk_of * p.chunk) * kBM;
           }
         }
+        // Four experts' first two pieces in flight at a time.  (Piece q > 0 of a cut tile lies in
+        // the first slot of CTA c_first + q: 2 q - 1 slots behind piece 0.)
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        const size_t slot = static_cast<size_t>(p.chunk) * kBM;
-        for (int j = 0; j < p.top; ++j) {
-          const int n = __shfl_sync(0xffffffffu, pieces, j);
-          const int cf = __shfl_sync(0xffffffffu, c_first, j);
-          const float wj = __shfl_sync(0xffffffffu, wt, j);
-          const float* sj = reinterpret_cast<const float*>(
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j));
-          if (n == 0) continue;
-          float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int q = 0; q < n; ++q) {
-            const float* at = n == 1 ? sj : sj + (2 * static_cast<size_t>(cf + q) + (q == 0 ? 1 : 0)) * slot;
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(at) + lane);
-            z.x += v.x, z.y += v.y, z.z += v.z, z.w += v.w;
+#pragma unroll 1
+        for (int j0 = 0; j0 < p.top; j0 += 4) {
+          float4 z[4], z1[4];
+          int n[4];
+          const float4* at[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = j0 + i;  // (lanes from `top` on bring no pieces)
+            n[i] = j < 32 ? __shfl_sync(0xffffffffu, pieces, j & 31) : 0;
+            at[i] = reinterpret_cast<const float4*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j & 31)) + lane;
           }
-          sum.x = fmaf(wj, z.x, sum.x), sum.y = fmaf(wj, z.y, sum.y);
-          sum.z = fmaf(wj, z.z, sum.z), sum.w = fmaf(wj, z.w, sum.w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            z[i] = n[i] > 0 ? __ldcg(at[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            z1[i] = n[i] > 1 ? __ldcg(at[i] + slot / 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            z[i].x += z1[i].x, z[i].y += z1[i].y, z[i].z += z1[i].z, z[i].w += z1[i].w;
+#pragma unroll 4
+            for (int q = 2; q < n[i]; ++q) {
+              const float4 v = __ldcg(at[i] + static_cast<size_t>(2 * q - 1) * (slot / 4));
+              z[i].x += v.x, z[i].y += v.y, z[i].z += v.z, z[i].w += v.w;
+            }
+            const float wj = __shfl_sync(0xffffffffu, wt, (j0 + i) & 31);
+            if (n[i] > 0) {
+              sum.x = fmaf(wj, z[i].x, sum.x), sum.y = fmaf(wj, z[i].y, sum.y);
+              sum.z = fmaf(wj, z[i].z, sum.z), sum.w = fmaf(wj, z[i].w, sum.w);
+            }
+          }
         }
         const float s4[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int f = tile * kBM + 4 * lane + q;
-          if (f < p.feat2) {
-            const float r = p.residual ? unpack_lo<BF16>(static_cast<uint32_t>(p.residual[static_cast<long long>(t) * p.ldr + f])) : 0.f;
-            p.y[static_cast<long long>(t) * p.ldy + f] = cvt1<BF16>(s4[q] + r);
-          }
-        }
+        for (int q = 0; q < 4; ++q)
+          if (f0 + q < p.feat2) p.y[static_cast<long long>(t) * p.ldy + f0 + q] = cvt1<BF16>(s4[q] + r4[q]);
       }
     }
     // The last CTA to leave clears the counters for the next launch.
