@@ -128,15 +128,15 @@ class MoeProblem(ctypes.Structure):
 
 class MoePlan(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in ("block_num", "stages", "chunk", "reserved")] + [
-        (name, ctypes.c_int64) for name in ("smem_bytes", "hidden_rows", "hidden_pitch", "workspace_floats",
+        (name, ctypes.c_int64) for name in ("smem_bytes", "hidden_rows", "hidden_pitch", "sorted_pitch", "workspace_floats",
                                             "counter_words", "status_words")]
 
 
 class MoeBuffers(ctypes.Structure):
     _fields_ = [("w1", ctypes.c_void_p), ("ldw1", ctypes.c_int64), ("stride1", ctypes.c_int64),
                 ("w2", ctypes.c_void_p), ("ldw2", ctypes.c_int64), ("stride2", ctypes.c_int64),
-                ("hidden", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("counters", ctypes.c_void_p),
-                ("status", ctypes.c_void_p)]
+                ("hidden", ctypes.c_void_p), ("sorted", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("counters", ctypes.c_void_p), ("status", ctypes.c_void_p)]
 
 
 _lock = threading.Lock()

@@ -107,6 +107,10 @@ int encode_rows(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int6
 }
 
 constexpr int kMaxSmem = 232448;
+// Tokens up to which the experts' first product gathers its token rows itself (a gather of four rows
+// takes the TMA about 200 clocks, so a step's weights hide three); above, they are copied into
+// the pairs' order first.
+constexpr int64_t kMoeGather = 16;
 
 int stream_chunk(int64_t tokens) { return tokens <= 16 ? 16 : (tokens <= 32 ? 32 : (tokens <= 64 ? 64 : 128)); }
 // The ring beside `list_bytes` of lists: K steps per slot (of `slab` weight bytes and `chunk` token
@@ -408,6 +412,7 @@ int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* pr, ffn_b200_moe_plan* ou
   out->smem_bytes = ring.smem;
   out->hidden_rows = pr->m * pr->top_k;
   out->hidden_pitch = pitch_of(pr->h);
+  out->sorted_pitch = pr->m > kMoeGather ? pitch_of(pr->k) : 0;
   const int64_t slots = 2ll * grid * out->chunk * 128;
   const int64_t items = ffnb200::StreamLists::stream_items(tokens, pr->experts, pr->top_k);
   const int64_t down = cdiv(pr->n, 128);
@@ -431,8 +436,9 @@ int ffn_b200_moe_prepare(const ffn_b200_moe_problem* pr, const ffn_b200_moe_buff
   if (rc) return rc;
   if (plan.block_num > sms) return FFN_B200_ERR_DEVICE;  // the CTAs wait on one another
   if (!b->w1 || !b->w2 || !b->hidden || !b->workspace || !b->counters || !b->status) return FFN_B200_ERR_INVALID;
+  if (plan.sorted_pitch && !b->sorted) return FFN_B200_ERR_INVALID;
   if (bad_rows(b->w1, b->ldw1, pr->k) || bad_rows(b->w2, b->ldw2, pr->h) || b->stride1 % 8 || b->stride2 % 8 ||
-      b->stride1 <= 0 || b->stride2 <= 0 || !aligned16(b->hidden) || !aligned16(b->workspace))
+      b->stride1 <= 0 || b->stride2 <= 0 || !aligned16(b->hidden) || !aligned16(b->sorted) || !aligned16(b->workspace))
     return FFN_B200_ERR_ALIGNMENT;
   rc = get_encode();
   if (rc) return rc;
@@ -456,7 +462,14 @@ int ffn_b200_moe_prepare(const ffn_b200_moe_problem* pr, const ffn_b200_moe_buff
                       P.group_feats);
   if (!rc)
     rc = encode_weights(&P.tm_w2, b->w2, pr->dtype, pr->h, pr->n, 1, pr->experts, b->ldw2, b->stride2, 128);
-  if (!rc) rc = encode_rows(&P.tm_h, b->hidden, pr->dtype, pr->h, plan.hidden_rows, plan.hidden_pitch, 8);
+  if (!rc) rc = encode_rows(&P.tm_h8, b->hidden, pr->dtype, pr->h, plan.hidden_rows, plan.hidden_pitch, 8);
+  if (!rc) rc = encode_rows(&P.tm_h64, b->hidden, pr->dtype, pr->h, plan.hidden_rows, plan.hidden_pitch, 64);
+  if (plan.sorted_pitch) {
+    if (!rc) rc = encode_rows(&P.tm_x8, b->sorted, pr->dtype, pr->k, plan.hidden_rows, plan.sorted_pitch, 8);
+    if (!rc) rc = encode_rows(&P.tm_x64, b->sorted, pr->dtype, pr->k, plan.hidden_rows, plan.sorted_pitch, 64);
+    P.sorted = static_cast<uint16_t*>(b->sorted);
+    P.lds = plan.sorted_pitch;
+  }
   P.tokens = static_cast<int>(pr->m);
   P.groups1 = static_cast<int>(cdiv(pr->h, P.group_feats));
   P.steps1 = static_cast<int>(cdiv(pr->k, 64));
@@ -497,7 +510,9 @@ int ffn_b200_moe_run(ffn_b200_moe* h, const void* x, int64_t ldx, const int32_t*
   DeviceScope scope(h->device);
   if (!scope.ok) return FFN_B200_ERR_DEVICE;
   ffnb200::StreamParams P = h->params;
-  const int rc = encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx, 1);
+  const int rc = P.sorted ? FFN_B200_OK : encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx, 1);
+  P.x = static_cast<const uint16_t*>(x);
+  P.ldx = ldx;
   if (rc) return rc;
   P.ids = ids;
   P.weights = weights;

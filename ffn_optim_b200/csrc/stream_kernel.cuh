@@ -33,7 +33,7 @@
 
 namespace ffnb200 {
 
-constexpr int kStreamThreads = 256;
+constexpr int kStreamThreads = 512;  // 8 warps with roles, 8 more for the lists and the combination
 constexpr int kStreamMaxStages = 40;
 constexpr int kStreamMinSteps = 4;   // fewest K steps of the second product worth a CTA of their own
 constexpr int kStreamBarBytes = 1024;
@@ -41,8 +41,9 @@ constexpr int kStreamBarBytes = 1024;
 struct StreamParams {
   CUtensorMap tm_w1, tm_w2;  // weights [E][halves][rows][K]: a box is one group's rows (SwiGLU: 8 of
                              // both halves), or 128 rows of the second product
-  CUtensorMap tm_x, tm_h;    // token rows: the projection's in one box, the experts' in boxes of one
-                             // row (gathered); hidden rows in boxes of 8
+  CUtensorMap tm_x;          // token rows: the projection's in one box, the experts' in boxes of one row
+  CUtensorMap tm_x8, tm_x64; // experts, `sorted` not null: its rows in boxes of 8 and 64
+  CUtensorMap tm_h8, tm_h64; // hidden rows
   int tokens;
   int groups1, group_rows, group_feats, unit_groups;  // first product: row groups per item, weight rows and
                              // output features of a group, groups of one tile at most
@@ -57,6 +58,10 @@ struct StreamParams {
   long long ldr;
   uint16_t* y;
   long long ldy;
+  const uint16_t* x;         // experts with `sorted`: the token rows, copied to [pair][ldx] in its order
+  long long ldx;
+  uint16_t* sorted;
+  long long lds;
   uint16_t* hidden;          // experts: [pair][ldh], pairs ordered by expert, then token
   long long ldh;
   float* pieces;             // [2 C][chunk][128] pieces of cut tiles of the second product
@@ -69,7 +74,7 @@ struct StreamParams {
   unsigned long long wait_limit_ns;
   int inject;
 };
-constexpr int kStreamSync = 2;  // CTAs done with the second product; CTAs leaving
+constexpr int kStreamSync = 3;  // CTAs done with the second product; CTAs leaving; CTAs done with `sorted`
 
 // Shared memory behind the ring and barriers for the experts' lists.
 struct StreamLists {
@@ -211,7 +216,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* last_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
   int* n_items = reinterpret_cast<int*>(tmem_slot + 3);
-  int* warp_sums = reinterpret_cast<int*>(tmem_slot + 4);  // [8] x 2
+  int* n_pairs = n_items + 1;
+  int* warp_sums = n_items + 2;  // [16] x 2
   const StreamLists lists(p.tokens, MOE ? p.experts : 0, MOE ? p.top : 0);
   uint8_t* lbase = ctrl + kStreamBarBytes;
   unsigned* sets = reinterpret_cast<unsigned*>(lbase + lists.sets);
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     prefetch_tmap(&p.tm_x);
     if (MOE) {
       prefetch_tmap(&p.tm_w2);
-      prefetch_tmap(&p.tm_h);
+      prefetch_tmap(&p.tm_h8);
     }
   }
   if (warp == 1) {
@@ -275,38 +281,31 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         atomicOr(&sets[e * lists.words + (t >> 5)], 1u << (t & 31));
     }
     __syncthreads();
-    // Exclusive sums over the experts of pairs and items; thread i takes experts 2i and 2i + 1.
-    int cnt[2], itm[2];
-    for (int q = 0; q < 2; ++q) {
-      const int e = 2 * threadIdx.x + q;
-      cnt[q] = 0;
-      if (e < p.experts)
-        for (int w = 0; w < lists.words; ++w) cnt[q] += __popc(sets[e * lists.words + w]);
-      itm[q] = (cnt[q] + p.chunk - 1) / p.chunk;
-    }
-    int a = cnt[0] + cnt[1], b = itm[0] + itm[1];
-    const int mine_a = a, mine_b = b;
+    // Exclusive sums over the experts of pairs and items; thread i takes expert i.
+    static_assert(kStreamThreads >= 512, "one thread per expert");
+    const int e = threadIdx.x;
+    int cnt = 0;
+    if (e < p.experts)
+      for (int w = 0; w < lists.words; ++w) cnt += __popc(sets[e * lists.words + w]);
+    const int itm = (cnt + p.chunk - 1) / p.chunk;
+    int a = cnt, b = itm;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int ua = __shfl_up_sync(0xffffffffu, a, o), ub = __shfl_up_sync(0xffffffffu, b, o);
       if (lane >= o) a += ua, b += ub;
     }
-    if (lane == 31) warp_sums[warp] = a, warp_sums[8 + warp] = b;
+    if (lane == 31) warp_sums[warp] = a, warp_sums[16 + warp] = b;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) a += warp_sums[w], b += warp_sums[8 + w];
-    int pa = a - mine_a, pb = b - mine_b;
-    for (int q = 0; q < 2; ++q) {
-      const int e = 2 * threadIdx.x + q;
-      if (e < p.experts) {
-        offset[e] = static_cast<uint16_t>(pa);
-        first[e] = static_cast<uint16_t>(pb);
-        for (int i = 0; i < itm[q]; ++i)
-          item_list[pb + i] = make_uint2(static_cast<unsigned>(e) |
-                                             static_cast<unsigned>(min(p.chunk, cnt[q] - i * p.chunk)) << 16,
-                                         static_cast<unsigned>(pa + i * p.chunk));
-      }
-      pa += cnt[q], pb += itm[q];
+#pragma unroll 1
+    for (int w = 0; w < warp; ++w) a += warp_sums[w], b += warp_sums[16 + w];
+    if (e < p.experts) {
+      offset[e] = static_cast<uint16_t>(a - cnt);
+      first[e] = static_cast<uint16_t>(b - itm);
+      for (int i = 0; i < itm; ++i)
+        item_list[b - itm + i] = make_uint2(static_cast<unsigned>(e) | static_cast<unsigned>(min(p.chunk, cnt - i * p.chunk)) << 16,
+                                            static_cast<unsigned>(a - cnt + i * p.chunk));
     }
-    if (threadIdx.x == kStreamThreads - 1) *n_items = pb;
+    if (threadIdx.x == kStreamThreads - 1) *n_items = b, *n_pairs = a;
     __syncthreads();
     for (int i = threadIdx.x; i < p.experts * lists.words; i += kStreamThreads) {
       const int e = i / lists.words, w = i - e * lists.words;
@@ -331,13 +330,29 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       expert = 0, start = 0, count = p.tokens;
     }
   };
+  // Experts, first product: C / items CTAs per item where that takes no more than a quarter longer than
+  // an even deal (one token, 6 of 64 experts: ends 6 us earlier, as no CTA is left with two tiles).
+  const int per_item = max(1, MOE && items ? C / items : 1);
+  const bool whole_items =
+      items <= C && 4ll * items * p.groups1 >= 3ll * C * ((p.groups1 + per_item - 1) / per_item);
   // This CTA's tiles, in the same order for every role: tile(ph, item, g0, groups, k0, k1) returns
   // false to stop.  First product: groups [g0, g0 + groups) of the item over all of K.  Second:
   // tile g0, K steps [k0, k1).
   auto for_tiles = [&](auto&& tile) {
     if (items == 0) return;
     const StreamSplit rows(static_cast<long long>(items) * p.groups1, C, 1);
-    for (int g = rows.begin(c), end = rows.begin(c + 1); g < end;) {
+    int g = rows.begin(c), end = rows.begin(c + 1);
+    if (MOE && whole_items) {
+      // Few items: each gets CTAs of its own, so that none has two short tiles instead of one.
+      const int it = c / per_item;
+      const StreamSplit one(p.groups1, per_item, 1);
+      g = end = 0;
+      if (it < items) {
+        g = it * p.groups1 + one.begin(c - it * per_item);
+        end = it * p.groups1 + one.begin(c - it * per_item + 1);
+      }
+    }
+    while (g < end) {
       const int it = g / p.groups1, g0 = g - it * p.groups1;
       const int n = min(min(p.unit_groups, p.groups1 - g0), end - g);
       if (!tile(0, it, g0, n, 0, p.steps1)) return;
@@ -446,12 +461,21 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       for_tiles([&](int ph, int it, int, int, int k0, int k1) {
         int expert, start, count;
         item_of(it, expert, start, count);
-        if (MOE && ph == 1) {
-          ok = stream_wait_word(item_done + it, static_cast<unsigned>(p.groups1 + (p.inject ? 1 : 0)), abort_flag, p, 2, it);
+        if (MOE && (ph || p.sorted)) {
+          ok = ph ? stream_wait_word(item_done + it, static_cast<unsigned>(p.groups1 + (p.inject ? 1 : 0)), abort_flag, p, 2, it)
+                  : stream_wait_word(p.counters + 2, static_cast<unsigned>(C), abort_flag, p, 2, -1);
           if (!ok) return false;
-          fence_async_global();  // hidden rows written by other CTAs' threads, read by this one's TMA
+          fence_async_global();  // rows written by other CTAs' threads, read by this one's TMA
         }
-        const uint32_t bytes = !MOE ? token_bytes : (ph ? (count + 7) / 8 * 1024u : (count + 3) / 4 * 512u);
+        const bool gathered = MOE && ph == 0 && !p.sorted;
+        // Boxes of 64 rows, of 8 for a remainder of up to 24.  (Rows behind the item's last belong to
+        // columns nobody reads.)
+        const int wide = p.chunk < 64 ? 0 : (count % 64 > 24 ? (count + 63) / 64 : count / 64);
+        const int narrow = max(0, count - wide * 64 + 7) / 8;
+        const uint32_t bytes =
+            !MOE ? token_bytes : (gathered ? (count + 3) / 4 * 512u : static_cast<uint32_t>(wide) * 8192u + narrow * 1024u);
+        const CUtensorMap* tm8 = ph ? &p.tm_h8 : &p.tm_x8;
+        const CUtensorMap* tm64 = ph ? &p.tm_h64 : &p.tm_x64;
 #pragma unroll 1
         for (int kb = k0; kb < k1; kb += KS) {
           const int nb = min(KS, k1 - kb);
@@ -463,12 +487,16 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
           if (!MOE) {
 #pragma unroll 1
             for (int i = 0; i < nb; ++i) tma_load_2d(dst + i * token_bytes, &p.tm_x, (kb + i) * kBK, 0, bar);
-          } else if (ph) {  // (rows behind the item's last belong to columns nobody reads)
+          } else if (!gathered) {
 #pragma unroll 1
-            for (int r = 0; r < count; r += 8)
+            for (int i = 0; i < nb; ++i) {
 #pragma unroll 1
-              for (int i = 0; i < nb; ++i)
-                tma_load_2d(dst + i * token_bytes + r * 128, &p.tm_h, (kb + i) * kBK, start + r, bar);
+              for (int r = 0; r < wide; ++r)
+                tma_load_2d(dst + i * token_bytes + r * 8192, tm64, (kb + i) * kBK, start + 64 * r, bar);
+#pragma unroll 1
+              for (int r = 0; r < narrow; ++r)
+                tma_load_2d(dst + i * token_bytes + wide * 8192 + r * 1024, tm8, (kb + i) * kBK, start + 64 * wide + 8 * r, bar);
+            }
           } else {
 #pragma unroll 1
             for (int r = 0; r < count; r += 4) {  // (a group that runs past the item repeats its last row)
@@ -490,7 +518,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         }
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp >= 4 && warp < 8) {
     // ------------------------------------------------------------------ epilogue
     const int sub = warp - 4;  // TMEM lane sub-partition
     const uint32_t lane_off = static_cast<uint32_t>(sub * 32) << 16;
@@ -568,8 +596,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         }
         if constexpr (MOE) {
           fence_async_global();  // hidden: written here, read through other CTAs' TMA
-          __threadfence();
-          epilogue_all(1);
+          epilogue_all(1);       // (the release below covers what all 128 threads wrote before it)
           if (threadIdx.x == 128) red_release_add(item_done + it, static_cast<unsigned>(n));
         }
       }
@@ -581,6 +608,23 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     });
   }
 
+  else if (MOE && warp >= 8 && p.sorted) {
+    // ------------------------------------------------------------------ token rows in the pairs' order
+    // Dealt out over the CTAs, a warp taking 512 bytes of a row at a time.  The weights, already on
+    // their way, hide the grid-wide wait for them.
+    const int vecs = static_cast<int>(p.lds / 8), strips = (vecs + 31) / 32;
+#pragma unroll 2
+    for (int i = (warp - 8) * C + c; i < *n_pairs * strips; i += C * (kStreamThreads / 32 - 8)) {
+      const int pair = i / strips, v = (i - pair * strips) * 32 + lane;
+      if (v < vecs)
+        reinterpret_cast<uint4*>(p.sorted + static_cast<long long>(pair) * p.lds)[v] =
+            __ldg(reinterpret_cast<const uint4*>(p.x + static_cast<long long>(token_of[pair]) * p.ldx) + v);
+    }
+    fence_async_global();  // written here, read through every CTA's TMA
+    asm volatile("barrier.cta.sync 2, %0;" ::"n"(kStreamThreads - 256) : "memory");
+    if (threadIdx.x == 256) red_release_add(p.counters + 2, 1u);
+  }
+
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -590,50 +634,58 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     // Combination: when every CTA's second-product sums are in memory, each warp takes
     // (token, 128 output features) and adds the token's experts in order, each expert's pieces in
     // ascending CTA order, with the fp32 weights, then the residual; rounded once.
+    // What the sums do not depend on is looked up before the wait.
+    const StreamSplit line(static_cast<long long>(items) * p.tiles2 * p.steps2, C, kStreamMinSteps);
+    const size_t pitch = static_cast<size_t>(p.tiles2) * kBM;
+    const size_t slot = static_cast<size_t>(p.chunk) * kBM;
+    const int n_units = p.tokens * p.tiles2;
+    // Lane j < top knows choice j: its weight, its pieces and where the first one lies; every lane
+    // its four features of the residual.
+    const float* src = nullptr;
+    int pieces = 0, t = 0, f0 = 0;
+    float wt = 0.f;
+    uint2 res = make_uint2(0u, 0u);
+    auto look_up = [&](int unit) {
+      t = unit / p.tiles2;
+      const int tile = unit - t * p.tiles2;
+      f0 = tile * kBM + 4 * lane;
+      if (p.residual) {  // (rows are 16-byte aligned and padded to 8 elements: four at a time stay inside)
+        const uint16_t* r = p.residual + static_cast<long long>(t) * p.ldr + f0;
+        if (f0 + 4 <= p.feat2) {
+          res = __ldg(reinterpret_cast<const uint2*>(r));
+        } else {
+          res = make_uint2(0u, 0u);
+          for (int q = 0; f0 + q < p.feat2; ++q) (q < 2 ? res.x : res.y) |= static_cast<uint32_t>(__ldg(r + q)) << (16 * (q & 1));
+        }
+      }
+      pieces = 0;
+      if (lane < p.top) {
+        const int e = __ldg(p.ids + t * p.top + lane);
+        if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts)) {
+          wt = __ldg(p.weights + t * p.top + lane);
+          int rank = 0;
+          for (int w = 0; w < (t >> 5); ++w) rank += __popc(sets[e * lists.words + w]);
+          rank += __popc(sets[e * lists.words + (t >> 5)] & ((1u << (t & 31)) - 1u));
+          const int chunk_of = rank / p.chunk;
+          const int s = ((first[e] + chunk_of) * p.tiles2 + tile) * p.steps2;
+          const int c_first = line.cta_of(s);
+          pieces = line.cta_of(s + p.steps2 - 1) - c_first + 1;
+          src = pieces == 1 ? p.whole + static_cast<size_t>(offset[e] + rank) * pitch + static_cast<size_t>(tile) * kBM
+                            : p.pieces + (2 * static_cast<size_t>(c_first) + 1) * slot +
+                                  static_cast<size_t>(rank - chunk_of * p.chunk) * kBM;
+        }
+      }
+    };
+    int unit = warp * C + c;
+    if (unit < n_units) look_up(unit);
     if (threadIdx.x == 0) {
-      __threadfence();
-      red_release_add(sync_words, 1u);
+      red_release_add(sync_words, 1u);  // (covers the whole CTA's sums: the barrier above)
       if (!*abort_flag) stream_wait_word(sync_words, static_cast<unsigned>(C), abort_flag, p, 3, -1);
     }
     __syncthreads();
     if (!*abort_flag) {
-      __threadfence();
-      const StreamSplit line(static_cast<long long>(items) * p.tiles2 * p.steps2, C, kStreamMinSteps);
-      const size_t pitch = static_cast<size_t>(p.tiles2) * kBM;
-      const size_t slot = static_cast<size_t>(p.chunk) * kBM;
-      const int n_units = p.tokens * p.tiles2;
 #pragma unroll 1
-      for (int unit = warp * C + c; unit < n_units; unit += C * (kStreamThreads / 32)) {
-        const int t = unit / p.tiles2, tile = unit - t * p.tiles2;
-        // The residual first: it does not depend on anything read here.
-        float r4[4] = {0.f, 0.f, 0.f, 0.f};
-        const int f0 = tile * kBM + 4 * lane;
-        if (p.residual) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (f0 + q < p.feat2)
-              r4[q] = unpack_lo<BF16>(static_cast<uint32_t>(__ldg(p.residual + static_cast<long long>(t) * p.ldr + f0 + q)));
-        }
-        // Lane j knows choice j: its weight, its pieces and where the first one lies.
-        const float* src = nullptr;
-        int pieces = 0;
-        float wt = 0.f;
-        if (lane < p.top) {
-          const int e = __ldg(p.ids + t * p.top + lane);
-          if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts)) {
-            wt = __ldg(p.weights + t * p.top + lane);
-            int rank = 0;
-            for (int w = 0; w < (t >> 5); ++w) rank += __popc(sets[e * lists.words + w]);
-            rank += __popc(sets[e * lists.words + (t >> 5)] & ((1u << (t & 31)) - 1u));
-            const int chunk_of = rank / p.chunk;
-            const int s = ((first[e] + chunk_of) * p.tiles2 + tile) * p.steps2;
-            const int c_first = line.cta_of(s);
-            pieces = line.cta_of(s + p.steps2 - 1) - c_first + 1;
-            src = pieces == 1 ? p.whole + static_cast<size_t>(offset[e] + rank) * pitch + static_cast<size_t>(tile) * kBM
-                              : p.pieces + (2 * static_cast<size_t>(c_first) + 1) * slot +
-                                    static_cast<size_t>(rank - chunk_of * p.chunk) * kBM;
-          }
-        }
+      while (unit < n_units) {
         // Four experts' first two pieces in flight at a time.  (Piece q > 0 of a cut tile lies in
         // the first slot of CTA c_first + q: 2 q - 1 slots behind piece 0.)
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -644,10 +696,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
           const float4* at[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int j = j0 + i;  // (lanes from `top` on bring no pieces)
-            n[i] = j < 32 ? __shfl_sync(0xffffffffu, pieces, j & 31) : 0;
+            const int j = (j0 + i) & 31;  // (lanes from `top` on bring no pieces)
+            n[i] = __shfl_sync(0xffffffffu, pieces, j);
             at[i] = reinterpret_cast<const float4*>(
-                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j & 31)) + lane;
+                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j)) + lane;
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -669,10 +721,20 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
             }
           }
         }
-        const float s4[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (f0 + q < p.feat2) p.y[static_cast<long long>(t) * p.ldy + f0 + q] = cvt1<BF16>(s4[q] + r4[q]);
+        if (p.residual) {
+          sum.x += unpack_lo<BF16>(res.x), sum.y += unpack_hi<BF16>(res.x);
+          sum.z += unpack_lo<BF16>(res.y), sum.w += unpack_hi<BF16>(res.y);
+        }
+        uint16_t* y = p.y + static_cast<long long>(t) * p.ldy + f0;
+        const uint2 out = make_uint2(pack2<BF16>(sum.x, sum.y), pack2<BF16>(sum.z, sum.w));
+        if (f0 + 4 <= p.feat2) {
+          *reinterpret_cast<uint2*>(y) = out;
+        } else {
+          for (int q = 0; f0 + q < p.feat2; ++q)
+            y[q] = static_cast<uint16_t>((q < 2 ? out.x : out.y) >> (16 * (q & 1)));
+        }
+        unit += C * (kStreamThreads / 32);
+        if (unit < n_units) look_up(unit);
       }
     }
     // The last CTA to leave clears the counters for the next launch.

@@ -155,6 +155,7 @@ class PreparedMoE(L.PreparedLayer):
         with torch.cuda.device(x.device):
             self._w1, self._w2 = L.packed_weight(weight1), L.packed_weight(weight2)
             self._hidden = torch.empty((plan.hidden_rows, plan.hidden_pitch), dtype=x.dtype, device=x.device)
+            self._sorted = torch.empty(plan.hidden_rows * plan.sorted_pitch, dtype=x.dtype, device=x.device)
             self._out, self._range = L.output_buffer(m, n, x)
             self._ws = torch.empty(max(plan.workspace_floats, 4), dtype=torch.float32, device=x.device)
             self._counters = torch.zeros(max(plan.counter_words, 4), dtype=torch.int32, device=x.device)
@@ -165,8 +166,8 @@ class PreparedMoE(L.PreparedLayer):
         self.x, self.residual = x, residual
         bufs = _lib.MoeBuffers(self._w1.data_ptr(), self._pitch(self._w1, 1), self._pitch(self._w1, 0),
                                self._w2.data_ptr(), self._pitch(self._w2, 1), self._pitch(self._w2, 0),
-                               self._hidden.data_ptr(), self._ws.data_ptr(), self._counters.data_ptr(),
-                               self._status.data_ptr())
+                               self._hidden.data_ptr(), self._sorted.data_ptr() or None, self._ws.data_ptr(),
+                               self._counters.data_ptr(), self._status.data_ptr())
         handle = ctypes.c_void_p()
         L.raise_for(lib.ffn_b200_moe_prepare(ctypes.byref(prob), ctypes.byref(bufs), x.device.index or 0,
                                              ctypes.byref(handle)), "prepare_moe_ffn")

@@ -414,6 +414,8 @@ typedef struct {
   int32_t reserved;
   int64_t smem_bytes;
   int64_t hidden_rows, hidden_pitch;  /* hidden scratch, elements of the dtype */
+  int64_t sorted_pitch;               /* token rows in the experts' order: hidden_rows of this
+                                         pitch; 0: none needed */
   int64_t workspace_floats;
   int64_t counter_words;
   int64_t status_words;
@@ -423,6 +425,7 @@ typedef struct {
   const void* w1; int64_t ldw1, stride1;  /* row and expert pitches in elements */
   const void* w2; int64_t ldw2, stride2;
   void* hidden;
+  void* sorted;                           /* NULL if the plan needs none */
   float* workspace;
   uint32_t* counters;                     /* zeroed before the first run */
   int32_t* status;                        /* zeroed before the first run */
