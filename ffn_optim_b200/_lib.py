@@ -33,7 +33,7 @@ TILE_VARIANTS = {"cta128x256": 1, "cta128x128": 2, "swap16": 3, "swap64": 4, "pa
                  "swap16fp8": 11, "swap64fp8": 12, "hslice16": 13}
 WEIGHT_FORMATS = {"native": 0, "fp8": 1}
 IDENTITY = 4  # activation of the dense projection only (no hidden layer)
-LINEAR_TILES = {}  # tile families of the dense projection (None = automatic)
+LINEAR_TILES = {"stream": 1, "pair256": 2, "cta128": 3, "cta64": 4}  # tile families of the dense projection (None = automatic)
 MAX_EXPERTS = 512
 MAX_TOP_K = 32
 MOE_MAX_TOKENS = 256
@@ -55,7 +55,8 @@ EXPORTED = ("ffn_b200_abi_version", "ffn_b200_strerror", "ffn_b200_device_info",
             "ffn_b200_destroy", "ffn_b200_launch", "ffn_b200_run_noalloc", "ffn_b200_peer_alloc",
             "ffn_b200_peer_open", "ffn_b200_peer_close", "ffn_b200_peer_free", "ffn_b200_reduce_scatter_bytes",
             "ffn_b200_set_reduce_scatter",
-            "ffn_b200_linear_make_plan", "ffn_b200_linear_prepare", "ffn_b200_linear_run", "ffn_b200_linear_destroy",
+            "ffn_b200_linear_make_plan", "ffn_b200_linear_prepare", "ffn_b200_linear_run", "ffn_b200_linear_reset",
+            "ffn_b200_linear_destroy",
             "ffn_b200_router_scratch", "ffn_b200_router_run",
             "ffn_b200_moe_make_plan", "ffn_b200_moe_prepare", "ffn_b200_moe_run", "ffn_b200_moe_reset",
             "ffn_b200_moe_set_wait_limit", "ffn_b200_moe_set_fault_injection", "ffn_b200_moe_destroy")
@@ -112,7 +113,7 @@ class LinearProblem(ctypes.Structure):
 
 class LinearPlan(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in ("tile", "tile_m", "tile_n", "stages", "block_num", "split")] + [
-        (name, ctypes.c_int64) for name in ("smem_bytes", "workspace_floats", "counter_words")]
+        (name, ctypes.c_int64) for name in ("smem_bytes", "status_words")]
 
 
 class RouterProblem(ctypes.Structure):
@@ -192,9 +193,9 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
             "ffn_b200_reduce_scatter_bytes": ([vp, i32, i32, ctypes.POINTER(u64), ctypes.POINTER(u64)], i32),
             "ffn_b200_set_reduce_scatter": ([vp, i32, i32, i32, ctypes.POINTER(vp), ctypes.POINTER(vp), vp, i64], i32),
             "ffn_b200_linear_make_plan": ([ctypes.POINTER(LinearProblem), ctypes.POINTER(LinearPlan)], i32),
-            "ffn_b200_linear_prepare": ([ctypes.POINTER(LinearProblem), vp, i64, vp, vp, vp, i32, ctypes.POINTER(vp)],
-                                        i32),
+            "ffn_b200_linear_prepare": ([ctypes.POINTER(LinearProblem), vp, i64, vp, vp, i32, ctypes.POINTER(vp)], i32),
             "ffn_b200_linear_run": ([vp, vp, i64, vp, i64, vp, i64, vp], i32),
+            "ffn_b200_linear_reset": ([vp, vp], i32),
             "ffn_b200_linear_destroy": ([vp], i32),
             "ffn_b200_router_scratch": ([ctypes.POINTER(RouterProblem), ctypes.POINTER(i64), ctypes.POINTER(i64)], i32),
             "ffn_b200_router_run": ([vp, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp], i32),

@@ -11,7 +11,7 @@
 #include <new>
 
 #include "../../include/ffn_b200.h"
-#include "layers_simple.cuh"
+#include "gemm_kernel.cuh"
 #include "router_kernel.cuh"
 #include "stream_kernel.cuh"
 
@@ -39,11 +39,6 @@ struct DeviceScope {
     if (before >= 0) cudaSetDevice(before);
   }
 };
-
-int launched() {
-  if (cudaGetLastError() == cudaSuccess) return FFN_B200_OK;
-  return FFN_B200_ERR_CUDA;
-}
 
 int device_sms(int given, int* sms) {
   *sms = given;
@@ -129,6 +124,23 @@ struct StreamRing {
   }
 };
 
+using GemmFn = void (*)(const ffnb200::GemmParams);
+// A tile family of the dense projection.
+struct GemmTile {
+  int rows, cols, box_rows, smem, stages;  // box_rows: rows of a weight load
+  GemmFn fn[2];                            // fp16, bf16
+};
+template <int BN, bool PAIR>
+GemmTile gemm_tile() {
+  using LY = ffnb200::GemmLayout<BN, PAIR>;
+  return {PAIR ? 256 : 128, BN, LY::kBRows, LY::kSmem, LY::kStages,
+          {ffnb200::gemm_kernel<false, BN, PAIR>, ffnb200::gemm_kernel<true, BN, PAIR>}};
+}
+GemmTile gemm_tile(int tile) {
+  if (tile == FFN_B200_LINEAR_PAIR256) return gemm_tile<256, true>();
+  return tile == FFN_B200_LINEAR_CTA128 ? gemm_tile<128, false>() : gemm_tile<64, false>();
+}
+
 using StreamFn = void (*)(const ffnb200::StreamParams);
 
 int launch_stream(StreamFn fn, const ffnb200::StreamParams& params, int grid, int64_t smem, bool cooperative,
@@ -194,7 +206,7 @@ int check_linear(const ffn_b200_linear_problem& p) {
   if (p.dtype != FFN_B200_F16 && p.dtype != FFN_B200_BF16) return FFN_B200_ERR_INVALID;
   if (p.activation < 0 || p.activation > FFN_B200_IDENTITY || p.activation == FFN_B200_SWIGLU)
     return FFN_B200_ERR_INVALID;
-  if (p.block_num < 0 || p.reserved || p.tile < 0 || p.tile > 2) return FFN_B200_ERR_INVALID;
+  if (p.block_num < 0 || p.reserved || p.tile < 0 || p.tile > FFN_B200_LINEAR_CTA64) return FFN_B200_ERR_INVALID;
   return FFN_B200_OK;
 }
 
@@ -229,8 +241,10 @@ struct ffn_b200_linear {
   const void* w;
   int64_t ldw;
   const void* bias;
-  ffnb200::StreamParams params;
+  int32_t* status;
+  ffnb200::StreamParams params;  // tile FFN_B200_LINEAR_STREAM
   StreamFn fn;
+  ffnb200::GemmParams gemm;      // the other tiles
 };
 
 struct ffn_b200_moe {
@@ -242,9 +256,16 @@ struct ffn_b200_moe {
   StreamFn fn;
 };
 
+// ---- dense projection ----------------------------------------------------------------------
+static int linear_tile(const ffn_b200_linear_problem& p, int grid) {
+  if (p.m <= 128) return FFN_B200_LINEAR_STREAM;
+  const int64_t pairs = cdiv(p.m, 256) * cdiv(p.n, 256), steps = cdiv(p.k, 64);
+  if (grid >= 2 && pairs >= grid / 2 && steps >= 8) return FFN_B200_LINEAR_PAIR256;
+  return cdiv(p.m, 128) * cdiv(p.n, 128) >= grid / 2 ? FFN_B200_LINEAR_CTA128 : FFN_B200_LINEAR_CTA64;
+}
+
 extern "C" {
 
-// ---- dense projection ----------------------------------------------------------------------
 int ffn_b200_linear_make_plan(const ffn_b200_linear_problem* pr, ffn_b200_linear_plan* out) {
   if (!pr || !out) return FFN_B200_ERR_INVALID;
   int rc = check_linear(*pr);
@@ -255,11 +276,11 @@ int ffn_b200_linear_make_plan(const ffn_b200_linear_problem* pr, ffn_b200_linear
   std::memset(out, 0, sizeof(*out));
   const int grid = pr->block_num ? pr->block_num : sms;
   out->block_num = grid;
-  if (pr->tile == 1 && pr->m > 128) return FFN_B200_ERR_INVALID;
-  out->tile = pr->tile ? pr->tile : (pr->m <= 128 ? 1 : 2);
-  out->workspace_floats = 4;
-  out->counter_words = 4;
-  if (out->tile == 1) {
+  out->split = 1;
+  if (pr->tile == FFN_B200_LINEAR_STREAM && pr->m > 128) return FFN_B200_ERR_INVALID;
+  out->status_words = 4;
+  out->tile = pr->tile ? pr->tile : linear_tile(*pr, grid);
+  if (out->tile == FFN_B200_LINEAR_STREAM) {
     // Equal numbers of weight rows per CTA, in tiles of at most 128.
     const int64_t per_cta = cdiv(pr->n, static_cast<int64_t>(grid) * 128);
     out->tile_m = static_cast<int32_t>(cdiv(pr->n, grid * per_cta));
@@ -267,12 +288,28 @@ int ffn_b200_linear_make_plan(const ffn_b200_linear_problem* pr, ffn_b200_linear
     const StreamRing ring(static_cast<int>(cdiv(out->tile_m, 8)) * 1024, out->tile_n, 0);
     out->stages = ring.stages;
     out->smem_bytes = ring.smem;
+    return FFN_B200_OK;
+  }
+  const GemmTile tile = gemm_tile(out->tile);
+  const int64_t tiles = cdiv(pr->m, tile.rows) * cdiv(pr->n, tile.cols), steps = cdiv(pr->k, 64);
+  if (tiles >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
+  out->tile_m = tile.rows;
+  out->tile_n = tile.cols;
+  out->stages = tile.stages;
+  out->smem_bytes = tile.smem;
+  if (out->tile == FFN_B200_LINEAR_PAIR256) {
+    if (grid < 2) return FFN_B200_ERR_INVALID;
+    out->block_num = static_cast<int32_t>(2 * std::min<int64_t>(tiles, grid / 2));
+  } else {
+    // Few tiles: clusters of up to 8 CTAs split K while each keeps at least 4 steps.
+    while (out->split < 8 && tiles * out->split * 2 <= grid && steps >= out->split * 2 * 4) out->split *= 2;
+    out->block_num = static_cast<int32_t>(std::min<int64_t>(tiles, grid / out->split) * out->split);
   }
   return FFN_B200_OK;
 }
 
 int ffn_b200_linear_prepare(const ffn_b200_linear_problem* pr, const void* w, int64_t ldw, const void* bias,
-                            float* workspace, uint32_t* counters, int device, ffn_b200_linear** out) {
+                            int32_t* status, int device, ffn_b200_linear** out) {
   if (!pr || !w || !out) return FFN_B200_ERR_INVALID;
   *out = nullptr;
   ffn_b200_linear_plan plan;
@@ -281,7 +318,11 @@ int ffn_b200_linear_prepare(const ffn_b200_linear_problem* pr, const void* w, in
   if (rc) return rc;
   if (bad_rows(w, ldw, pr->k)) return FFN_B200_ERR_ALIGNMENT;
   if (bias && !aligned16(bias)) return FFN_B200_ERR_ALIGNMENT;
-  if (!workspace || !counters) return FFN_B200_ERR_INVALID;
+  if (!status) return FFN_B200_ERR_INVALID;
+  int sms = 0, maj = 0, min = 0;
+  rc = ffn_b200_device_info(device, &sms, &maj, &min);
+  if (rc) return rc;
+  if (plan.block_num > sms) return FFN_B200_ERR_DEVICE;
   rc = get_encode();
   if (rc) return rc;
   DeviceScope scope(device);
@@ -294,7 +335,8 @@ int ffn_b200_linear_prepare(const ffn_b200_linear_problem* pr, const void* w, in
   h->w = w;
   h->ldw = ldw;
   h->bias = bias;
-  if (plan.tile == 1) {
+  h->status = status;
+  if (plan.tile == FFN_B200_LINEAR_STREAM) {
     ffnb200::StreamParams& P = h->params;
     std::memset(&P, 0, sizeof(P));
     const int rows = plan.tile_m;
@@ -312,9 +354,27 @@ int ffn_b200_linear_prepare(const ffn_b200_linear_problem* pr, const void* w, in
     P.stages = ring.stages;
     P.act = pr->activation;
     P.bias = static_cast<const uint16_t*>(bias);
+    P.status = status;
     P.wait_limit_ns = 4000000000ull;
     h->fn = pr->dtype == FFN_B200_BF16 ? ffnb200::stream_kernel<true, false> : ffnb200::stream_kernel<false, false>;
     if (!rc) rc = set_smem(reinterpret_cast<const void*>(h->fn), kMaxSmem);
+  } else {
+    const GemmTile tile = gemm_tile(plan.tile);
+    ffnb200::GemmParams& G = h->gemm;
+    std::memset(&G, 0, sizeof(G));
+    rc = encode_rows(&G.tm_w, w, pr->dtype, pr->k, pr->n, ldw, tile.box_rows);
+    G.M = static_cast<int>(pr->m);
+    G.N = static_cast<int>(pr->n);
+    G.steps = static_cast<int>(cdiv(pr->k, 64));
+    G.tiles_m = static_cast<int>(cdiv(pr->m, tile.rows));
+    G.tiles_n = static_cast<int>(cdiv(pr->n, tile.cols));
+    G.group = std::min(G.tiles_m, 8);
+    G.split = plan.split;
+    G.act = pr->activation;
+    G.bias = static_cast<const uint16_t*>(bias);
+    G.status = status;
+    G.wait_limit_ns = 4000000000ull;
+    if (!rc) rc = set_smem(reinterpret_cast<const void*>(tile.fn[pr->dtype == FFN_B200_BF16]), tile.smem);
   }
   if (rc) {
     delete h;
@@ -331,7 +391,7 @@ int ffn_b200_linear_run(ffn_b200_linear* h, const void* x, int64_t ldx, const vo
   if (bad_rows(x, ldx, p.k) || bad_rows(y, ldy, p.n) || (res && bad_rows(res, ldr, p.n))) return FFN_B200_ERR_ALIGNMENT;
   DeviceScope scope(h->device);
   if (!scope.ok) return FFN_B200_ERR_DEVICE;
-  if (h->plan.tile == 1) {
+  if (h->plan.tile == FFN_B200_LINEAR_STREAM) {
     ffnb200::StreamParams P = h->params;
     const int rc = encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx, P.chunk);
     if (rc) return rc;
@@ -341,12 +401,44 @@ int ffn_b200_linear_run(ffn_b200_linear* h, const void* x, int64_t ldx, const vo
     P.ldy = ldy;
     return launch_stream(h->fn, P, h->plan.block_num, h->plan.smem_bytes, false, stream);
   }
-  const int64_t blocks = cdiv(p.m * p.n, 256);
-  if (blocks >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
-  auto* kern = p.dtype == FFN_B200_BF16 ? ffnb200::simple_linear<true> : ffnb200::simple_linear<false>;
-  kern<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      x, ldx, h->w, h->ldw, h->bias, res, ldr, y, ldy, p.m, static_cast<int>(p.k), static_cast<int>(p.n), p.activation);
-  return launched();
+  ffnb200::GemmParams G = h->gemm;
+  int rc = encode_rows(&G.tm_x, x, p.dtype, p.k, p.m, ldx, 128);
+  if (!rc) rc = encode_rows(&G.tm_y, y, p.dtype, p.n, p.m, ldy, 32);
+  if (rc) return rc;
+  G.residual = static_cast<const uint16_t*>(res);
+  G.ldr = ldr;
+  G.y = static_cast<uint16_t*>(y);
+  G.ldy = ldy;
+  const GemmTile tile = gemm_tile(h->plan.tile);
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(h->plan.block_num), 1, 1);
+  cfg.blockDim = dim3(ffnb200::kGemmThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(tile.smem);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const int cluster = h->plan.tile == FFN_B200_LINEAR_PAIR256 ? 2 : h->plan.split;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  if (cudaLaunchKernelEx(&cfg, tile.fn[p.dtype == FFN_B200_BF16], G) == cudaSuccess) return FFN_B200_OK;
+  cudaGetLastError();
+  return FFN_B200_ERR_CUDA;
+}
+
+int ffn_b200_linear_reset(ffn_b200_linear* h, void* stream) {
+  if (!h) return FFN_B200_ERR_INVALID;
+  if (cudaMemsetAsync(h->status, 0, 4 * h->plan.status_words, static_cast<cudaStream_t>(stream)) == cudaSuccess)
+    return FFN_B200_OK;
+  cudaGetLastError();
+  return FFN_B200_ERR_CUDA;
 }
 
 int ffn_b200_linear_destroy(ffn_b200_linear* h) {

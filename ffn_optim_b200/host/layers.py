@@ -160,8 +160,8 @@ def raise_for(rc, what):
 
 
 class PreparedLayer:
-    """What the prepared operators share: the preparation stream, the reused output and graph
-    capture.  Subclasses launch in ``_launch(stream_pointer, ...)``."""
+    """What the prepared operators share: the preparation stream, the kernel's status and graph
+    capture (``_capture(stream_pointer)`` of the subclass launches once on the prepared inputs)."""
 
     def _open(self, device):
         import torch
@@ -176,6 +176,30 @@ class PreparedLayer:
         if self._torch.cuda.current_stream(self.device).cuda_stream != self._stream_ptr:
             raise RuntimeError(f"{type(self).__name__} must run on its preparation stream; "
                                "concurrent reuse is unsupported")
+
+    def status(self):
+        """Synchronises the stream and returns the kernel's status words [code, cta, aux, 0]."""
+        self.stream.synchronize()
+        return [int(v) for v in self._status.tolist()]
+
+    def check(self):
+        """Raises RuntimeError if a launch since the last reset reported a device error."""
+        from .. import _lib
+
+        st = self.status()
+        if st[0] != 0:
+            self.reset()
+            raise RuntimeError(f"{type(self).__name__} kernel failed: {_lib.KERNEL_ERRORS.get(st[0], st[0])} "
+                               f"(cta {st[1]}, aux {st[2]})")
+        return True
+
+    def reset(self):
+        """Clears the kernel's counters and status."""
+        from .. import _lib
+
+        rc = self._reset(self._stream_ptr)
+        if rc != _lib.OK:
+            raise RuntimeError(f"{type(self).__name__}.reset: {_lib.strerror(rc)}")
 
     def capture_graph(self, runs=1):
         """Captures ``runs`` launches on the prepared inputs into a ``torch.cuda.CUDAGraph``.

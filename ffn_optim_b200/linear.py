@@ -60,16 +60,15 @@ class PreparedLinear(L.PreparedLayer):
             self._weight = L.packed_weight(weight)
             self._bias = _prepared_bias(bias, n, x, "bias")
             self._out, self._range = L.output_buffer(m, n, x)
-            self._ws = torch.empty(max(plan.workspace_floats, 4), dtype=torch.float32, device=x.device)
-            self._counters = torch.zeros(max(plan.counter_words, 4), dtype=torch.int32, device=x.device)
+            self._status = torch.zeros(plan.status_words, dtype=torch.int32, device=x.device)
             self._view = self._out[:, :n].view(self.output_shape)
         self._x, self._r = L.RowStorage(m, k, x, x.shape), L.RowStorage(m, n, x, self.output_shape)
         self.x, self.residual = x, residual
         handle = ctypes.c_void_p()
         rc = lib.ffn_b200_linear_prepare(
             ctypes.byref(prob), self._weight.data_ptr(), L.row_pitch(self._weight, n, k),
-            self._bias.data_ptr() if self._bias is not None else None, self._ws.data_ptr(), self._counters.data_ptr(),
-            x.device.index or 0, ctypes.byref(handle))
+            self._bias.data_ptr() if self._bias is not None else None, self._status.data_ptr(), x.device.index or 0,
+            ctypes.byref(handle))
         L.raise_for(rc, "prepare_linear")
         self.handle = handle
         self._run = lib.ffn_b200_linear_run
@@ -97,6 +96,9 @@ class PreparedLinear(L.PreparedLayer):
         self._check_stream()
         self._launch(self._stream_ptr, self.x if x is None else x, self.residual if residual is None else residual)
         return self._view
+
+    def _reset(self, stream):
+        return _lib.load().ffn_b200_linear_reset(self.handle, stream)
 
     def close(self):
         if self.handle is not None:

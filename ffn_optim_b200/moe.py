@@ -238,24 +238,8 @@ class PreparedMoE(L.PreparedLayer):
         self._alive += (ids, weights)
         return y
 
-    def status(self):
-        """Synchronises the stream and returns the kernel's status words [code, cta, aux, 0]."""
-        self.stream.synchronize()
-        return [int(v) for v in self._status.tolist()]
-
-    def check(self):
-        """Raises RuntimeError if a launch since the last reset reported a device error."""
-        st = self.status()
-        if st[0] != 0:
-            self.reset()
-            raise RuntimeError(f"MoE kernel failed: {_lib.KERNEL_ERRORS.get(st[0], st[0])} (cta {st[1]}, aux {st[2]})")
-        return True
-
-    def reset(self):
-        """Clears the kernel's counters and status."""
-        rc = _lib.load().ffn_b200_moe_reset(self.handle, ctypes.c_void_p(self._stream_ptr))
-        if rc != _lib.OK:
-            raise RuntimeError(f"ffn_b200_moe_reset: {_lib.strerror(rc)}")
+    def _reset(self, stream):
+        return _lib.load().ffn_b200_moe_reset(self.handle, stream)
 
     def set_wait_limit(self, seconds: float):
         """Upper bound of every in-kernel wait; on expiry the kernel reports an error."""

@@ -343,22 +343,29 @@ typedef struct {
   int32_t block_num;   /* CTAs launched */
   int32_t split;       /* CTAs that share one tile's K range, at most */
   int64_t smem_bytes;
-  int64_t workspace_floats;
-  int64_t counter_words;
+  int64_t status_words;
 } ffn_b200_linear_plan;
+
+/* Tile families: the weight rows dealt out over all CTAs (M <= 128), 256x256 by a CTA pair, 128x128
+ * and 128x64 by one CTA (for few tiles clusters split K). */
+typedef enum {
+  FFN_B200_LINEAR_STREAM = 1, FFN_B200_LINEAR_PAIR256 = 2, FFN_B200_LINEAR_CTA128 = 3, FFN_B200_LINEAR_CTA64 = 4
+} ffn_b200_linear_tile;
 
 typedef struct ffn_b200_linear ffn_b200_linear;
 
 FFN_B200_EXPORT int ffn_b200_linear_make_plan(const ffn_b200_linear_problem* problem, ffn_b200_linear_plan* plan);
-/* Binds the weight (and bias, or NULL) and the scratch of the planned sizes (counters zeroed).
+/* Binds the weight (and bias, or NULL) and the status words (zeroed; as ffn_b200_buffers.status).
  * Row pitches in elements, multiples of 8; bases 16-byte aligned. */
 FFN_B200_EXPORT int ffn_b200_linear_prepare(const ffn_b200_linear_problem* problem, const void* w, int64_t ldw,
-                                            const void* bias, float* workspace, uint32_t* counters, int device,
+                                            const void* bias, int32_t* status, int device,
                                             ffn_b200_linear** handle);
 /* One asynchronous launch on `stream`; `residual` may be NULL.  Y must not overlap X or the
- * residual.  Runs of one handle must be serialised on one stream (they share its scratch). */
+ * residual.  Runs need no scratch: they may overlap, given Y of their own. */
 FFN_B200_EXPORT int ffn_b200_linear_run(ffn_b200_linear* handle, const void* x, int64_t ldx, const void* residual,
                                         int64_t ldr, void* y, int64_t ldy, void* stream);
+/* Clears the status words; call after a run reported a kernel error. */
+FFN_B200_EXPORT int ffn_b200_linear_reset(ffn_b200_linear* handle, void* stream);
 FFN_B200_EXPORT int ffn_b200_linear_destroy(ffn_b200_linear* handle);
 
 /* ---- Expert router ------------------------------------------------------------------------

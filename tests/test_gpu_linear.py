@@ -48,6 +48,22 @@ def test_epilogues(m, act, gelu, use):
     check(linear(x, w, bias=b, residual=r, activation=act, gelu=gelu), x, w, b, r, act, gelu)
 
 
+@pytest.mark.parametrize("tile", ["stream", "pair256", "cta128", "cta64"])
+@pytest.mark.parametrize("m,k,n", [(1, 64, 64), (33, 1000, 130), (128, 2048, 512), (200, 72, 600), (257, 4096, 65),
+                                   (300, 520, 1030), (1000, 512, 2048), (3000, 136, 1160)], ids=lambda v: str(v))
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_every_tile(tile, m, k, n, act):
+    """Each tile family at sizes the automatic choice gives to another, split K and ragged edges included."""
+    x, w, b, r = make(m, k, n, BF)
+    if tile == "stream" and m > 128:
+        with pytest.raises(ValueError):
+            prepare_linear(x, w, tile=tile)
+        return
+    p = prepare_linear(x, w, bias=b, residual=r, activation=act, tile=tile)
+    check(p.run(), x, w, b, r, act)
+    p.check()
+
+
 @pytest.mark.parametrize("m,k,n", [(5000, 1024, 2304), (8191, 520, 1288), (16384, 256, 768)])
 def test_long_inputs(m, k, n):
     x, w, b, r = make(m, k, n, BF)

@@ -111,6 +111,40 @@ def test_c_entries_reject_bad_problems(lib):
     assert lib.ffn_b200_moe_reset(None, None) == _lib.ERR_INVALID
 
 
+def test_linear_plans(lib):
+    """Every plan covers the output with one tile per owner at least, whole clusters and no more CTAs than asked."""
+    plan = _lib.LinearPlan()
+    for m in (1, 16, 17, 64, 128, 129, 300, 512, 1000, 4096, 6993, 16384, 2**31 - 16):
+        for k in (8, 100, 512, 2048, 65535):
+            for n in (1, 64, 130, 512, 1000, 4096, 65535):
+                for blocks in (0, 1, 2, 7, 100):
+                    prob = _lib.LinearProblem(m, k, n, 1, 4, blocks, 148, 0, 0)
+                    rc = lib.ffn_b200_linear_make_plan(ctypes.byref(prob), ctypes.byref(plan))
+                    if rc == _lib.ERR_TOO_LARGE:
+                        assert m > 10**9
+                        continue
+                    assert rc == _lib.OK, (m, k, n, blocks)
+                    assert 1 <= plan.block_num <= (blocks or 148) and plan.smem_bytes <= 232448 and plan.stages >= 2
+                    assert plan.split in (1, 2, 4, 8) and plan.block_num % plan.split == 0
+                    if plan.tile == _lib.LINEAR_TILES["stream"]:
+                        assert m <= 128 <= 128 and plan.tile_n >= m and 1 <= plan.tile_m <= 128
+                    else:
+                        tiles = -(-m // plan.tile_m) * -(-n // plan.tile_n)
+                        assert plan.split == 1 or plan.block_num == tiles * plan.split and -(-k // 64) >= 4 * plan.split
+
+
+def test_moe_plans(lib):
+    plan = _lib.MoePlan()
+    for m in (1, 2, 16, 17, 32, 33, 64, 65, 128, 129, 256):
+        for e, top in ((1, 1), (8, 2), (64, 6), (256, 8), (512, 32)):
+            for act in (0, 3):
+                prob = _lib.MoeProblem(m, 4096, 1000, 2048, e, top, 1, act, 0, 148)
+                assert lib.ffn_b200_moe_make_plan(ctypes.byref(prob), ctypes.byref(plan)) == _lib.OK
+                assert plan.smem_bytes <= 232448 and plan.stages >= 2 and plan.block_num == 148
+                assert min(m, 128) <= plan.chunk <= 128 and plan.hidden_rows == m * top and plan.hidden_pitch == 1000
+                assert plan.sorted_pitch in (0, 4096)
+
+
 def test_operands_read_in_place_or_copied():
     """Which views the kernels read in place: unit column stride, 16-byte base, pitch a multiple of 8."""
     base = torch.zeros(9 * 40, dtype=torch.bfloat16)
