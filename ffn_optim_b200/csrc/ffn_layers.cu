@@ -168,10 +168,30 @@ int launch_stream(StreamFn fn, const ffnb200::StreamParams& params, int grid, in
 
 using RouteFn = void (*)(const ffnb200::RouteParams);
 
-int launch_route(RouteFn fn, const ffnb200::RouteParams& P, int mt, int nt, void* stream) {
-  const int64_t rows = cdiv(P.M, 16 * mt);
-  if (rows > 65535) return FFN_B200_ERR_TOO_LARGE;
-  const int smem = ffnb200::kRouteWarps * std::max(128 * mt * nt * 12, P.E * 16);  // parts of K; then logits and scores
+struct RouteFns {
+  RouteFn few, few32, many32, logits, choose;
+};
+template <bool BF16, int PER>
+constexpr RouteFns route_fns() {
+  return {ffnb200::route_kernel<BF16, false, 1, 1, PER>, ffnb200::route_kernel<BF16, true, 1, 1, PER>,
+          ffnb200::route_kernel<BF16, true, 2, 4, PER>, ffnb200::route_logits_kernel<BF16>,
+          ffnb200::route_choose_kernel<BF16, PER>};
+}
+const RouteFns kRouteFns[3][2] = {{route_fns<false, 2>(), route_fns<true, 2>()},
+                                  {route_fns<false, 8>(), route_fns<true, 8>()},
+                                  {route_fns<false, 16>(), route_fns<true, 16>()}};
+
+// Tokens from which the router runs as two kernels (16-bit weights), and the parts of K of its first.
+constexpr int64_t kRouteMany = 128;
+int route_parts(const ffn_b200_router_problem& p) {
+  if (p.m < kRouteMany || p.weight_f32) return 1;
+  const int64_t tiles = cdiv(p.m, ffnb200::kLogitTile) * cdiv(p.experts, ffnb200::kLogitTile);
+  const int64_t steps = cdiv(p.k, ffnb200::kRouteStep);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 296 / tiles, steps / 8})));  // two CTAs per SM
+}
+
+int launch_route(RouteFn fn, const ffnb200::RouteParams& P, dim3 grid, int smem, void* stream) {
+  if (grid.y > 65535) return FFN_B200_ERR_TOO_LARGE;
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
@@ -179,7 +199,7 @@ int launch_route(RouteFn fn, const ffnb200::RouteParams& P, int mt, int nt, void
   }
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(cdiv(P.E, 8 * nt)), static_cast<unsigned>(rows), 1);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(ffnb200::kRouteThreads, 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = static_cast<cudaStream_t>(stream);
@@ -191,6 +211,11 @@ int launch_route(RouteFn fn, const ffnb200::RouteParams& P, int mt, int nt, void
   if (cudaLaunchKernelEx(&cfg, fn, P) == cudaSuccess) return FFN_B200_OK;
   cudaGetLastError();
   return FFN_B200_ERR_CUDA;
+}
+// One kernel of 16 mt x 8 nt tiles; shared memory: the warps' parts of K, then logits and scores.
+int launch_route(RouteFn fn, const ffnb200::RouteParams& P, int mt, int nt, void* stream) {
+  const dim3 grid(static_cast<unsigned>(cdiv(P.E, 8 * nt)), static_cast<unsigned>(cdiv(P.M, 16 * mt)), 1);
+  return launch_route(fn, P, grid, ffnb200::kRouteWarps * std::max(128 * mt * nt * 12, P.E * 8), stream);
 }
 
 int set_smem(const void* fn, int64_t smem) {
@@ -451,7 +476,7 @@ int ffn_b200_router_scratch(const ffn_b200_router_problem* pr, int64_t* logit_do
   if (!pr || !logit_doubles || !counter_words) return FFN_B200_ERR_INVALID;
   const int rc = check_router(*pr);
   if (rc) return rc;
-  const int64_t cells = pr->m * pr->experts;
+  const int64_t cells = pr->m * pr->experts * route_parts(*pr);
   *logit_doubles = cells + (cells + 1) / 2;  // fp64 logits, then fp32 sums of |x w|
   *counter_words = cdiv(pr->m, 16);
   return FFN_B200_OK;
@@ -468,21 +493,23 @@ int ffn_b200_router_run(const ffn_b200_router_problem* pr, const void* x, int64_
   P.x = x; P.ldx = ldx; P.w = w; P.ldw = ldw;
   P.choice_bias = cbias; P.mask = mask; P.ids = ids; P.weights = weights;
   P.logits = logits;
-  P.sums = reinterpret_cast<float*>(logits + pr->m * pr->experts);
+  P.parts = route_parts(*pr);
+  P.sums = reinterpret_cast<float*>(logits + P.parts * pr->m * pr->experts);
   P.counters = counters;
   P.M = static_cast<int>(pr->m); P.K = static_cast<int>(pr->k); P.E = pr->experts; P.top = pr->top_k;
   P.sigmoid = pr->sigmoid; P.renormalize = pr->renormalize; P.scale = pr->scale;
-  const bool bf = pr->dtype == FFN_B200_BF16, w32 = pr->weight_f32 != 0;
-  // Small tiles spread few tokens over more CTAs; from 128 tokens on the larger tile halves and
-  // quarters the operand reads.
-  if (pr->m < 128) {
-    return launch_route(bf ? (w32 ? ffnb200::route_kernel<true, true, 1, 1> : ffnb200::route_kernel<true, false, 1, 1>)
-                           : (w32 ? ffnb200::route_kernel<false, true, 1, 1> : ffnb200::route_kernel<false, false, 1, 1>),
-                        P, 1, 1, stream);
-  }
-  return launch_route(bf ? (w32 ? ffnb200::route_kernel<true, true, 2, 4> : ffnb200::route_kernel<true, false, 2, 4>)
-                         : (w32 ? ffnb200::route_kernel<false, true, 2, 4> : ffnb200::route_kernel<false, false, 2, 4>),
-                      P, 2, 4, stream);
+  const int many = pr->m >= kRouteMany, w32 = pr->weight_f32;
+  // Experts per lane of a warp: as few registers and as little code as the number of experts needs.
+  const int per = pr->experts <= 64 ? 0 : (pr->experts <= 256 ? 1 : 2);
+  const RouteFns& fns = pr->dtype == FFN_B200_BF16 ? kRouteFns[per][1] : kRouteFns[per][0];
+  if (!many) return launch_route(w32 ? fns.few32 : fns.few, P, 1, 1, stream);  // small tiles: more CTAs
+  if (w32) return launch_route(fns.many32, P, 2, 4, stream);
+  const dim3 tiles(static_cast<unsigned>(cdiv(P.E, ffnb200::kLogitTile)), static_cast<unsigned>(cdiv(P.M, ffnb200::kLogitTile)),
+                   static_cast<unsigned>(P.parts));
+  const int rc2 = launch_route(fns.logits, P, tiles, ffnb200::kLogitSmem, stream);
+  if (rc2) return rc2;
+  return launch_route(fns.choose, P, dim3(static_cast<unsigned>(cdiv(P.M, ffnb200::kRouteWarps)), 1, 1),
+                      ffnb200::kRouteWarps * P.E * 8, stream);
 }
 
 // ---- mixture-of-experts layer --------------------------------------------------------------

@@ -12,11 +12,14 @@
 //     few tokens in a thousand.
 //   * fp32 weights are summed in fp64 outright (S = 0: nothing is summed twice).
 //
-// A CTA takes 16 MT tokens x 8 NT experts; its 8 warps split K in steps of 64 (operands straight
-// from L2 to registers: a lane reads 16 bytes of a row, and since A and B use the same order of
-// K inside a step, no shuffle is needed).  The CTA that arrives last at its tokens finishes
-// them, a warp per token.  What bounds it: for a few tokens the launch and three dependent L2
-// trips; for many the L2 reads of the operand tiles.
+// Fewer than 128 tokens, and fp32 weights (route_kernel): a CTA takes 16 MT tokens x 8 NT experts;
+// its 8 warps split K in steps of 64 (operands straight from L2 to registers: a lane reads 16
+// bytes of a row, and since A and B use the same order of K inside a step, no shuffle is needed).
+// The CTA that arrives last at its tokens finishes them, a warp per token.  Bound by the launch
+// and three dependent L2 trips.
+// More tokens (route_logits_kernel, route_choose_kernel): 64 x 64 tiles with K split over CTAs,
+// operands through shared memory (the first form's L2 reads took 60 us for 1000 tokens and 256
+// experts of 4096), then a warp per token over all SMs.
 #pragma once
 
 #include "ffn_kernel.cuh"
@@ -37,8 +40,9 @@ struct RouteParams {
   const uint8_t* mask;
   int* ids;
   float* weights;
-  double* logits;   // [M][E]
-  float* sums;      // [M][E]: sum |x w|
+  double* logits;   // [parts][M][E]: sums over a part of K
+  float* sums;      // [parts][M][E]: sum |x w|
+  int parts;
   unsigned* counters;
   int M, K, E, top;
   int sigmoid, renormalize;
@@ -97,32 +101,43 @@ __device__ __forceinline__ unsigned long long ordered(double v) {
   const long long b = __double_as_longlong(v + 0.0);  // (+ 0.0: one zero)
   return static_cast<unsigned long long>(b ^ (b < 0 ? -1ll : static_cast<long long>(1ull << 63)));
 }
-// The key of expert e: its score, with the choice bias; NaN ranks last.
-__device__ __forceinline__ double route_key(const RouteParams& p, double score, int e) {
-  const double key = p.choice_bias ? score + static_cast<double>(__ldg(p.choice_bias + e)) : score;
-  return key == key ? key : -INFINITY;
+__device__ __forceinline__ double unordered(unsigned long long k) {
+  const long long b = static_cast<long long>(k);
+  return __longlong_as_double(b < 0 ? b ^ static_cast<long long>(1ull << 63) : ~b);
 }
 
-// One token's choice by a warp; z and q: this warp's logits and scores in shared memory [E].
-// (Loops are kept rolled: the code runs once per token, and fetching it costs more than running it.)
-template <bool BF16, bool W32>
-__device__ __forceinline__ void route_token(const RouteParams& p, int t, int lane, double* z, double* q) {
+// One token's choice by a warp: lane l holds experts l, l + 32, ... (PER of them) in registers; q: this
+// warp's scores in shared memory [E].  (Code that runs once per token is fetched more slowly than it
+// runs: only the short loops over a lane's own experts are unrolled.)
+template <bool BF16, bool W32, int PER>
+__device__ __forceinline__ void route_token(const RouteParams& p, int t, int lane, double* q) {
   int* ids = p.ids + static_cast<size_t>(t) * p.top;
   float* weights = p.weights + static_cast<size_t>(t) * p.top;
   if (p.mask && !p.mask[t]) {
     for (int j = lane; j < p.top; j += 32) ids[j] = -1, weights[j] = 0.f;
     return;
   }
+  double z[PER], bias[PER];
   float s = 0.f;
   bool odd = false;  // a logit left fp32's range
+  const size_t cells = static_cast<size_t>(p.M) * p.E;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    z[i] = -INFINITY, bias[i] = 0.0;
+    if (e < p.E) {
+      const size_t at = static_cast<size_t>(t) * p.E + e;
+      z[i] = __ldcg(p.logits + at);
+      float size = W32 ? 0.f : __ldcg(p.sums + at);
+      if (p.choice_bias) bias[i] = static_cast<double>(__ldg(p.choice_bias + e));
 #pragma unroll 2
-  for (int e = lane; e < p.E; e += 32) {
-    const double v = __ldcg(p.logits + static_cast<size_t>(t) * p.E + e);
-    if (!W32) {
-      s = fmaxf(s, __ldcg(p.sums + static_cast<size_t>(t) * p.E + e));
-      odd |= !isfinite(v);
+      for (int c = 1; c < p.parts; ++c) {
+        z[i] += __ldcg(p.logits + c * cells + at);
+        size += __ldcg(p.sums + c * cells + at);
+      }
+      s = fmaxf(s, size);
+      odd |= !W32 && !isfinite(z[i]);
     }
-    z[e] = v;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
@@ -132,116 +147,125 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
 #pragma unroll 1
   for (int pass = 0;; ++pass) {
     // Scores.  A NaN logit makes every softmax score NaN.
-    double scale = 1.0;
-    if (!p.sigmoid) {
+    double v[PER];
+    if (p.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = 1.0 / (1.0 + exp(-z[i]));
+    } else {
       double top = -INFINITY, sum = 0.0;
       bool nan = false;
-#pragma unroll 1
-      for (int e = lane; e < p.E; e += 32) top = fmax(top, z[e]), nan |= z[e] != z[e];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) top = fmax(top, z[i]), nan |= z[i] != z[i];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (__any_sync(0xffffffffu, nan)) top = NAN;
-#pragma unroll 1
-      for (int e = lane; e < p.E; e += 32) sum += q[e] = exp(z[e] - top);
-      scale = 1.0 / warp_sum(sum);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sum += v[i] = lane + 32 * i < p.E ? exp(z[i] - top) : 0.0;
+      const double scale = 1.0 / warp_sum(sum);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] *= scale;
     }
-    // This lane's best expert not yet chosen.
-    unsigned used = 0;  // bit i: expert lane + 32 i
-    int at = -1;
-    double best = 0.0;
-    unsigned long long order = 0;
-#pragma unroll 1
-    for (int e = lane; e < p.E; e += 32) {
-      const double v = p.sigmoid ? 1.0 / (1.0 + exp(-z[e])) : q[e] * scale;
-      q[e] = v;
-      const double key = route_key(p, v, e);
-      if (at < 0 || key > best) best = key, at = e;
+    // Keys as integers; 0 ranks below all of them: no expert, or one already chosen.
+    unsigned long long key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = lane + 32 * i;
+      const double k = v[i] + bias[i];
+      key[i] = e < p.E ? ordered(k == k ? k : -INFINITY) : 0ull;
+      if (e < p.E) q[e] = v[i];
     }
-    order = at < 0 ? 0 : ordered(best);
+    __syncwarp();
     // The k largest keys and the next one, equal ones by index.
-    double key = 0.0, rest = 0.0;  // lane j: the j-th key; the key after the last choice
+    unsigned long long mine = 0, rest = 0;  // lane j: the j-th key; the key after the last choice
     const int want = W32 || pass || p.top == p.E ? p.top : p.top + 1;
 #pragma unroll 1
     for (int j = 0; j < want; ++j) {
-      const unsigned hi = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(order >> 32));
-      bool mine = static_cast<unsigned>(order >> 32) == hi;
-      const unsigned lo = __reduce_max_sync(0xffffffffu, mine ? static_cast<unsigned>(order) : 0u);
-      mine = mine && static_cast<unsigned>(order) == lo;
-      const unsigned e = __reduce_min_sync(0xffffffffu, mine && at >= 0 ? static_cast<unsigned>(at) : 0xffffffffu);
-      const double kj = __shfl_sync(0xffffffffu, best, static_cast<int>(e & 31u));
+      unsigned long long best = key[0];
+      int at = 0;
+#pragma unroll
+      for (int i = 1; i < PER; ++i)
+        if (key[i] > best) best = key[i], at = i;
+      const unsigned hi = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(best >> 32));
+      const bool high = static_cast<unsigned>(best >> 32) == hi;
+      const unsigned lo = __reduce_max_sync(0xffffffffu, high ? static_cast<unsigned>(best) : 0u);
+      const bool top = high && static_cast<unsigned>(best) == lo;
+      const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, top ? static_cast<unsigned>(lane + 32 * at) : 0xffffffffu));
+      const unsigned long long k = static_cast<unsigned long long>(hi) << 32 | lo;
       if (j == p.top) {
-        rest = kj;
+        rest = k;
         break;
       }
-      if (lane == j) chosen = static_cast<int>(e), key = kj, score = q[e];
-      if (lane == static_cast<int>(e & 31u)) {
-        used |= 1u << (e >> 5);
-        at = -1;
-#pragma unroll 1
-        for (int f = lane; f < p.E; f += 32)
-          if (!(used >> (f >> 5) & 1u)) {
-            const double v = route_key(p, q[f], f);
-            if (at < 0 || v > best) best = v, at = f;
-          }
-        order = at < 0 ? 0 : ordered(best);
-      }
-      __syncwarp();
+      if (lane == j) chosen = e, mine = k;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (e == lane + 32 * i) key[i] = 0;
     }
+    if (lane < p.top) score = q[chosen];
     if (W32 || pass) break;
     // Could the errors of two logits have swapped neighbours?  A score moves by at most its slope
-    // times a logit's error: p (1 - p) for the sigmoid, 2 p with softmax's normaliser.
-    const double after = __shfl_down_sync(0xffffffffu, key, 1);
-    const double next = lane == p.top - 1 ? rest : after;
-    const double slope = p.sigmoid ? 0.25 : 2.0 * score;
+    // times a logit's error: 1/4 for the sigmoid, 2 p with softmax's normaliser.
+    const double reach = 2.0 * loss * (p.sigmoid ? 0.25 : 2.0 * score);
+    const unsigned long long after = __shfl_down_sync(0xffffffffu, mine, 1);
     const bool last = lane == p.top - 1 && p.top == p.E;
-    const bool near = lane < p.top && !last && key - next <= 2.0 * loss * slope && loss > 0.0;
-    if (!__any_sync(0xffffffffu, near || odd)) break;
+    const double here = unordered(mine);
+    const bool near = lane < p.top && !last && loss > 0.0 && here - unordered(lane == p.top - 1 ? rest : after) <= reach;
+    const unsigned nears = __ballot_sync(0xffffffffu, near);
+    const bool odds = __any_sync(0xffffffffu, odd);
+    if (!nears && !odds) break;
     // Sums again in fp64, unless the token itself is not finite.
     const long long xo = static_cast<long long>(t) * p.ldx;
     bool finite = true;
 #pragma unroll 1
-    for (int k = 8 * lane; k < p.K; k += 256) {
-      const uint4 v = row_chunk(p.x, xo, k, p.K);
-      const uint32_t r[4] = {v.x, v.y, v.z, v.w};
+    for (int k = odds ? 8 * lane : p.K; k < p.K; k += 256) {
+      const uint4 c = row_chunk(p.x, xo, k, p.K);
+      const uint32_t r[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) finite = finite && isfinite(unpack_lo<BF16>(r[i])) && isfinite(unpack_hi<BF16>(r[i]));
     }
     if (!__all_sync(0xffffffffu, finite)) break;
-    // Which: logits out of range, and experts whose key is as close to a chosen one's or to the
-    // next one's.  (Of two scores within reach of one another the chosen one's slope is the larger.)
+    // Which: logits out of range, and experts whose key is as close to a chosen one's, or a chosen one
+    // whose neighbour is.  (Of two scores within reach of one another the chosen one's slope is the larger.)
+    unsigned again = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < p.E && !isfinite(z[i])) again |= 1u << i;
 #pragma unroll 1
-    for (int base = 0; base < p.E; base += 32) {
-      const int e = base + lane;
-      const double ke = e < p.E ? route_key(p, q[e], e) : 0.0;
-      bool again = e < p.E && !isfinite(z[e]);
-#pragma unroll 1
-      for (int j = 0; j < p.top; ++j) {
-        const double kj = __shfl_sync(0xffffffffu, key, j), sj = __shfl_sync(0xffffffffu, slope, j);
-        const int cj = __shfl_sync(0xffffffffu, chosen, j);
-        again |= e < p.E && e != cj && fabs(ke - kj) <= 2.0 * loss * sj;
-        // (the chosen one itself, when its neighbour is that close)
-        const bool nj = __shfl_sync(0xffffffffu, near, j) || (j > 0 && __shfl_sync(0xffffffffu, near, j > 0 ? j - 1 : 0));
-        again |= e == cj && nj;
-      }
-      unsigned todo = __ballot_sync(0xffffffffu, again);
-#pragma unroll 1
-      while (todo) {
-        const int src = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const long long wo = static_cast<long long>(base + src) * p.ldw;
-        double a = 0.0, b = 0.0;
-#pragma unroll 1
-        for (int k = 8 * lane; k < p.K; k += 512) {
-          const uint4 xa = row_chunk(p.x, xo, k, p.K), wa = row_chunk(p.w, wo, k, p.K);
-          const uint4 xb = row_chunk(p.x, xo, k + 256, p.K), wb = row_chunk(p.w, wo, k + 256, p.K);
-          a = dot8<BF16>(xa, wa, a);
-          b = dot8<BF16>(xb, wb, b);
-        }
-        a = warp_sum(a + b);
-        if (lane == src) z[base + src] = a;
+    for (int j = 0; j < p.top; ++j) {
+      const double kj = __shfl_sync(0xffffffffu, here, j), rj = __shfl_sync(0xffffffffu, reach, j);
+      const int cj = __shfl_sync(0xffffffffu, chosen, j);
+      const bool nj = (nears >> j | (j ? nears >> (j - 1) : 0u)) & 1u;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int e = lane + 32 * i;
+        if (e < p.E && (e == cj ? nj : fabs(v[i] + bias[i] - kj) <= rj)) again |= 1u << i;
       }
     }
-    __syncwarp();
+#pragma unroll 1
+    for (unsigned todo = __ballot_sync(0xffffffffu, again != 0); todo; todo = __ballot_sync(0xffffffffu, again != 0)) {
+      const int src = __ffs(todo) - 1;
+      const int i = __ffs(__shfl_sync(0xffffffffu, again, src)) - 1;
+      const long long wo = static_cast<long long>(src + 32 * i) * p.ldw;
+      double a = 0.0;
+#pragma unroll 1
+      for (int k = 8 * lane; k < p.K; k += 256 * 8) {
+        uint4 xv[8], wv[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          xv[c] = row_chunk(p.x, xo, k + 256 * c, p.K);
+          wv[c] = row_chunk(p.w, wo, k + 256 * c, p.K);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) a = dot8<BF16>(xv[c], wv[c], a);
+      }
+      a = warp_sum(a);
+      if (lane == src) {
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+          if (c == i) z[c] = a;
+        again &= again - 1;
+      }
+    }
+    __syncwarp();  // (q is written again)
   }
   const double total = warp_sum(lane < p.top ? score : 0.0);
   if (lane < p.top) {
@@ -250,7 +274,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
   }
 }
 
-template <bool BF16, bool W32, int MT, int NT>
+template <bool BF16, bool W32, int MT, int NT, int PER>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   double* part = reinterpret_cast<double*>(smem);  // [warps][16 MT][8 NT], then the |x w| sums
@@ -356,12 +380,121 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   __syncthreads();
   if (!last) return;
   __threadfence();
-  double* z_of = reinterpret_cast<double*>(smem) + 2 * warp * p.E;  // (the parts have been added up)
+  double* q_of = reinterpret_cast<double*>(smem) + warp * p.E;  // (the parts have been added up)
 #pragma unroll 1
   for (int t = t0 + warp; t < min(t0 + 16 * MT, p.M); t += kRouteWarps) {
-    route_token<BF16, W32>(p, t, lane, z_of, z_of + p.E);
+    route_token<BF16, W32, PER>(p, t, lane, q_of);
     __syncwarp();
   }
+}
+
+// ---- many tokens -----------------------------------------------------------------------------
+constexpr int kLogitTile = 64;                            // tokens and experts of a tile
+constexpr int kLogitStages = 4;
+constexpr int kLogitStage = 2 * kLogitTile * kRouteStep * 2;  // bytes: 64 x 64 of x and of w
+constexpr int kLogitSmem = kLogitStages * kLogitStage;
+
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, int bytes) {  // the rest is zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Part blockIdx.z of K of a 64 x 64 tile of logits: warps 2 x 4, each 32 tokens x 16 experts.
+template <bool BF16>
+__global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const RouteParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, q = lane & 3;
+  const int t0 = blockIdx.y * kLogitTile, e0 = blockIdx.x * kLogitTile;
+  const int steps = (p.K + kRouteStep - 1) / kRouteStep;
+  const int s0 = steps * blockIdx.z / gridDim.z, s1 = steps * (blockIdx.z + 1) / gridDim.z;
+  if (threadIdx.x == 0) grid_dep_launch();
+  grid_dep_wait();
+  // Thread i copies 16-byte chunk i % 8 of rows i / 8 and i / 8 + 32 of both operands; rows past the
+  // last repeat it.  Chunk c of row r lies at c ^ (r % 8).
+  const int row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
+  auto load = [&](int step, int slot) {
+    const int k = step * kRouteStep + 8 * chunk;
+    const int bytes = max(0, min(16, 2 * (p.K - k)));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = row + 32 * h;
+      const uint32_t dst = base + slot * kLogitStage + r * 128 + ((chunk ^ (r & 7)) << 4);
+      const long long x = static_cast<long long>(min(t0 + r, p.M - 1)) * p.ldx, w = static_cast<long long>(min(e0 + r, p.E - 1)) * p.ldw;
+      copy_async16(dst, static_cast<const uint16_t*>(p.x) + x + (bytes ? k : 0), bytes);
+      copy_async16(dst + kLogitStage / 2, static_cast<const uint16_t*>(p.w) + w + (bytes ? k : 0), bytes);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kLogitStages - 1; ++i) {
+    if (s0 + i < s1) load(s0 + i, i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  const int m0 = (warp & 1) * 32, n0 = (warp >> 1) * 16;  // of the tile
+  double z[2][2][4] = {};
+  float sa[2][2][4] = {};
+#pragma unroll 1
+  for (int s = s0; s < s1; ++s) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLogitStages - 2) : "memory");
+    __syncthreads();
+    if (s + kLogitStages - 1 < s1) load(s + kLogitStages - 1, (s - s0 + kLogitStages - 1) % kLogitStages);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    const uint32_t sx = base + (s - s0) % kLogitStages * kLogitStage, sw = sx + kLogitStage / 2;
+    float d[2][2][4] = {};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint4 xv[4], wv[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xv[i] = ld_shared_u4(sx + (m0 + 8 * i + g) * 128 + (((4 * h + q) ^ g) << 4));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) wv[j] = ld_shared_u4(sw + (n0 + 8 * j + g) * 128 + (((4 * h + q) ^ g) << 4));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          constexpr uint32_t kAbs = 0x7FFF7FFFu;
+          const uint4 &a = xv[2 * i], &b = xv[2 * i + 1], &w = wv[j];
+          mma_16816<BF16>(d[i][j], a.x, b.x, a.y, b.y, w.x, w.y);
+          mma_16816<BF16>(d[i][j], a.z, b.z, a.w, b.w, w.z, w.w);
+          mma_16816<BF16>(sa[i][j], a.x & kAbs, b.x & kAbs, a.y & kAbs, b.y & kAbs, w.x & kAbs, w.y & kAbs);
+          mma_16816<BF16>(sa[i][j], a.z & kAbs, b.z & kAbs, a.w & kAbs, b.w & kAbs, w.z & kAbs, w.w & kAbs);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) z[i][j][v] += static_cast<double>(d[i][j][v]);
+  }
+  const size_t part = static_cast<size_t>(blockIdx.z) * p.M * p.E;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int t = t0 + m0 + 16 * i + 8 * (v / 2) + g, e = e0 + n0 + 8 * j + 2 * q + v % 2;
+        if (t < p.M && e < p.E) {
+          p.logits[part + static_cast<size_t>(t) * p.E + e] = z[i][j][v];
+          p.sums[part + static_cast<size_t>(t) * p.E + e] = sa[i][j][v];
+        }
+      }
+}
+
+template <bool BF16, int PER>
+__global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) grid_dep_launch();
+  grid_dep_wait();
+  const int t = blockIdx.x * kRouteWarps + warp;
+  if (t < p.M) route_token<BF16, false, PER>(p, t, lane, reinterpret_cast<double*>(smem) + warp * p.E);
 }
 
 }  // namespace ffnb200
