@@ -58,7 +58,8 @@ EXPORTED = ("ffn_b200_abi_version", "ffn_b200_strerror", "ffn_b200_device_info",
             "ffn_b200_linear_make_plan", "ffn_b200_linear_prepare", "ffn_b200_linear_run", "ffn_b200_linear_reset",
             "ffn_b200_linear_destroy",
             "ffn_b200_router_scratch", "ffn_b200_router_run",
-            "ffn_b200_moe_make_plan", "ffn_b200_moe_prepare", "ffn_b200_moe_run", "ffn_b200_moe_reset",
+            "ffn_b200_moe_make_plan", "ffn_b200_moe_prepare", "ffn_b200_moe_set_router", "ffn_b200_moe_run",
+            "ffn_b200_moe_run_routed", "ffn_b200_moe_reset",
             "ffn_b200_moe_set_wait_limit", "ffn_b200_moe_set_fault_injection", "ffn_b200_moe_destroy")
 
 
@@ -130,7 +131,7 @@ class MoeProblem(ctypes.Structure):
 class MoePlan(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in ("block_num", "stages", "chunk", "reserved")] + [
         (name, ctypes.c_int64) for name in ("smem_bytes", "hidden_rows", "hidden_pitch", "sorted_pitch", "workspace_floats",
-                                            "counter_words", "status_words")]
+                                            "counter_words", "status_words", "route_doubles")]
 
 
 class MoeBuffers(ctypes.Structure):
@@ -202,7 +203,9 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
             "ffn_b200_moe_make_plan": ([ctypes.POINTER(MoeProblem), ctypes.POINTER(MoePlan)], i32),
             "ffn_b200_moe_prepare": ([ctypes.POINTER(MoeProblem), ctypes.POINTER(MoeBuffers), i32, ctypes.POINTER(vp)],
                                      i32),
-            "ffn_b200_moe_run": ([vp, vp, i64, vp, vp, vp, i64, vp, i64, vp], i32),
+            "ffn_b200_moe_set_router": ([vp, ctypes.POINTER(RouterProblem), vp, i64, vp, vp], i32),
+            "ffn_b200_moe_run": ([vp, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp], i32),
+            "ffn_b200_moe_run_routed": ([vp, vp, i64, vp, vp, vp, i64, vp, i64, vp], i32),
             "ffn_b200_moe_reset": ([vp, vp], i32),
             "ffn_b200_moe_set_wait_limit": ([vp, u64], i32),
             "ffn_b200_moe_set_fault_injection": ([vp, i32], i32),

@@ -168,6 +168,28 @@ int launch_stream(StreamFn fn, const ffnb200::StreamParams& params, int grid, in
 
 using RouteFn = void (*)(const ffnb200::RouteParams);
 
+ffnb200::RouteParams route_params(const ffn_b200_router_problem& pr, const void* w, int64_t ldw, const float* cbias,
+                                  double* logits, int parts, uint32_t* counters) {
+  ffnb200::RouteParams P;
+  std::memset(&P, 0, sizeof(P));
+  P.w = w;
+  P.ldw = ldw;
+  P.choice_bias = cbias;
+  P.logits = logits;
+  P.sums = reinterpret_cast<float*>(logits + parts * pr.m * pr.experts);
+  P.parts = parts;
+  P.counters = counters;
+  P.M = static_cast<int>(pr.m);
+  P.K = static_cast<int>(pr.k);
+  P.E = pr.experts;
+  P.top = pr.top_k;
+  P.weight_f32 = pr.weight_f32;
+  P.sigmoid = pr.sigmoid;
+  P.renormalize = pr.renormalize;
+  P.scale = pr.scale;
+  return P;
+}
+
 struct RouteFns {
   RouteFn few, few32, many32, logits, choose;
 };
@@ -279,6 +301,7 @@ struct ffn_b200_moe {
   int device;
   ffnb200::StreamParams params;
   StreamFn fn;
+  uint32_t* route_counters;
 };
 
 // ---- dense projection ----------------------------------------------------------------------
@@ -489,15 +512,12 @@ int ffn_b200_router_run(const ffn_b200_router_problem* pr, const void* x, int64_
   const int rc = check_router(*pr);
   if (rc) return rc;
   if (bad_rows(x, ldx, pr->k) || bad_rows(w, ldw, pr->k)) return FFN_B200_ERR_ALIGNMENT;
-  ffnb200::RouteParams P;
-  P.x = x; P.ldx = ldx; P.w = w; P.ldw = ldw;
-  P.choice_bias = cbias; P.mask = mask; P.ids = ids; P.weights = weights;
-  P.logits = logits;
-  P.parts = route_parts(*pr);
-  P.sums = reinterpret_cast<float*>(logits + P.parts * pr->m * pr->experts);
-  P.counters = counters;
-  P.M = static_cast<int>(pr->m); P.K = static_cast<int>(pr->k); P.E = pr->experts; P.top = pr->top_k;
-  P.sigmoid = pr->sigmoid; P.renormalize = pr->renormalize; P.scale = pr->scale;
+  ffnb200::RouteParams P = route_params(*pr, w, ldw, cbias, logits, route_parts(*pr), counters);
+  P.x = x;
+  P.ldx = ldx;
+  P.mask = mask;
+  P.ids = ids;
+  P.weights = weights;
   const int many = pr->m >= kRouteMany, w32 = pr->weight_f32;
   // Experts per lane of a warp: as few registers and as little code as the number of experts needs.
   const int per = pr->experts <= 64 ? 0 : (pr->experts <= 256 ? 1 : 2);
@@ -513,6 +533,12 @@ int ffn_b200_router_run(const ffn_b200_router_problem* pr, const void* x, int64_
 }
 
 // ---- mixture-of-experts layer --------------------------------------------------------------
+// Parts of K of the router's logits, so that its tiles of 16 tokens x 8 experts fill the CTAs.
+static int moe_route_parts(const ffn_b200_moe_problem& p, int grid) {
+  const int64_t tiles = cdiv(p.m, 16) * cdiv(p.experts, 8), steps = cdiv(p.k, ffnb200::kRouteStep);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, grid / tiles, cdiv(steps, 16)})));
+}
+
 int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* pr, ffn_b200_moe_plan* out) {
   if (!pr || !out) return FFN_B200_ERR_INVALID;
   int rc = check_moe(*pr);
@@ -537,7 +563,8 @@ int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* pr, ffn_b200_moe_plan* ou
   const int64_t down = cdiv(pr->n, 128);
   if (items * down * cdiv(pr->h, 64) >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
   out->workspace_floats = slots + out->hidden_rows * down * 128;
-  out->counter_words = ffnb200::kStreamSync + items;
+  out->counter_words = ffnb200::kStreamSync + items + cdiv(pr->m, 16) + 1;
+  out->route_doubles = (pr->m * pr->experts * moe_route_parts(*pr, grid) * 3 + 1) / 2;  // fp64 logits, fp32 sums
   out->status_words = 4;
   return FFN_B200_OK;
 }
@@ -607,6 +634,7 @@ int ffn_b200_moe_prepare(const ffn_b200_moe_problem* pr, const ffn_b200_moe_buff
   P.pieces = b->workspace;
   P.whole = b->workspace + slots;
   P.counters = b->counters;
+  h->route_counters = b->counters + plan.counter_words - cdiv(pr->m, 16) - 1;
   P.status = b->status;
   P.experts = pr->experts;
   P.top = pr->top_k;
@@ -621,25 +649,59 @@ int ffn_b200_moe_prepare(const ffn_b200_moe_problem* pr, const ffn_b200_moe_buff
   return FFN_B200_OK;
 }
 
-int ffn_b200_moe_run(ffn_b200_moe* h, const void* x, int64_t ldx, const int32_t* ids, const float* weights,
-                     const void* res, int64_t ldr, void* y, int64_t ldy, void* stream) {
-  if (!h || !x || !ids || !weights || !y) return FFN_B200_ERR_INVALID;
+// The router's part of a run's arguments: set once per handle, before its first routed run.
+int ffn_b200_moe_set_router(ffn_b200_moe* h, const ffn_b200_router_problem* pr, const void* w, int64_t ldw,
+                            const float* choice_bias, double* logits) {
+  if (!h || !pr || !w || !logits) return FFN_B200_ERR_INVALID;
+  const int rc = check_router(*pr);
+  if (rc) return rc;
+  const ffn_b200_moe_problem& p = h->prob;
+  if (pr->m != p.m || pr->k != p.k || pr->experts != p.experts || pr->top_k != p.top_k || pr->dtype != p.dtype)
+    return FFN_B200_ERR_INVALID;
+  if (bad_rows(w, ldw, pr->k)) return FFN_B200_ERR_ALIGNMENT;
+  h->params.route = route_params(*pr, w, ldw, choice_bias, logits, moe_route_parts(p, h->plan.block_num), h->route_counters);
+  return FFN_B200_OK;
+}
+
+static int moe_launch(ffn_b200_moe* h, ffnb200::StreamParams& P, const void* x, int64_t ldx, const void* res, int64_t ldr,
+                      void* y, int64_t ldy, void* stream) {
   const ffn_b200_moe_problem& p = h->prob;
   if (bad_rows(x, ldx, p.k) || bad_rows(y, ldy, p.n) || (res && bad_rows(res, ldr, p.n))) return FFN_B200_ERR_ALIGNMENT;
   DeviceScope scope(h->device);
   if (!scope.ok) return FFN_B200_ERR_DEVICE;
-  ffnb200::StreamParams P = h->params;
   const int rc = P.sorted ? FFN_B200_OK : encode_rows(&P.tm_x, x, p.dtype, p.k, p.m, ldx, 1);
+  if (rc) return rc;
   P.x = static_cast<const uint16_t*>(x);
   P.ldx = ldx;
-  if (rc) return rc;
-  P.ids = ids;
-  P.weights = weights;
   P.residual = static_cast<const uint16_t*>(res);
   P.ldr = ldr;
   P.y = static_cast<uint16_t*>(y);
   P.ldy = ldy;
   return launch_stream(h->fn, P, h->plan.block_num, h->plan.smem_bytes, true, stream);
+}
+
+int ffn_b200_moe_run(ffn_b200_moe* h, const void* x, int64_t ldx, const uint8_t* mask, int32_t* ids, float* weights,
+                     const void* res, int64_t ldr, void* y, int64_t ldy, void* stream) {
+  if (!h || !x || !ids || !weights || !y || !h->params.route.w) return FFN_B200_ERR_INVALID;
+  ffnb200::StreamParams P = h->params;
+  P.routed = 1;
+  P.route.x = x;
+  P.route.ldx = ldx;
+  P.route.mask = mask;
+  P.route.ids = ids;
+  P.route.weights = weights;
+  P.ids = ids;
+  P.weights = weights;
+  return moe_launch(h, P, x, ldx, res, ldr, y, ldy, stream);
+}
+
+int ffn_b200_moe_run_routed(ffn_b200_moe* h, const void* x, int64_t ldx, const int32_t* ids, const float* weights,
+                            const void* res, int64_t ldr, void* y, int64_t ldy, void* stream) {
+  if (!h || !x || !ids || !weights || !y) return FFN_B200_ERR_INVALID;
+  ffnb200::StreamParams P = h->params;
+  P.ids = ids;
+  P.weights = weights;
+  return moe_launch(h, P, x, ldx, res, ldr, y, ldy, stream);
 }
 
 int ffn_b200_moe_reset(ffn_b200_moe* h, void* stream) {

@@ -45,7 +45,7 @@ struct RouteParams {
   int parts;
   unsigned* counters;
   int M, K, E, top;
-  int sigmoid, renormalize;
+  int weight_f32, sigmoid, renormalize;
   float scale;
 };
 
@@ -109,7 +109,7 @@ __device__ __forceinline__ double unordered(unsigned long long k) {
 // One token's choice by a warp: lane l holds experts l, l + 32, ... (PER of them) in registers; q: this
 // warp's scores in shared memory [E].  (Code that runs once per token is fetched more slowly than it
 // runs: only the short loops over a lane's own experts are unrolled.)
-template <bool BF16, bool W32, int PER>
+template <bool BF16, int PER>
 __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lane, double* q) {
   int* ids = p.ids + static_cast<size_t>(t) * p.top;
   float* weights = p.weights + static_cast<size_t>(t) * p.top;
@@ -128,7 +128,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
     if (e < p.E) {
       const size_t at = static_cast<size_t>(t) * p.E + e;
       z[i] = __ldcg(p.logits + at);
-      float size = W32 ? 0.f : __ldcg(p.sums + at);
+      float size = p.weight_f32 != 0 ? 0.f : __ldcg(p.sums + at);
       if (p.choice_bias) bias[i] = static_cast<double>(__ldg(p.choice_bias + e));
 #pragma unroll 2
       for (int c = 1; c < p.parts; ++c) {
@@ -136,7 +136,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
         size += __ldcg(p.sums + c * cells + at);
       }
       s = fmaxf(s, size);
-      odd |= !W32 && !isfinite(z[i]);
+      odd |= p.weight_f32 == 0 && !isfinite(z[i]);
     }
   }
 #pragma unroll
@@ -177,7 +177,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
     __syncwarp();
     // The k largest keys and the next one, equal ones by index.
     unsigned long long mine = 0, rest = 0;  // lane j: the j-th key; the key after the last choice
-    const int want = W32 || pass || p.top == p.E ? p.top : p.top + 1;
+    const int want = p.weight_f32 != 0 || pass || p.top == p.E ? p.top : p.top + 1;
 #pragma unroll 1
     for (int j = 0; j < want; ++j) {
       unsigned long long best = key[0];
@@ -201,7 +201,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
         if (e == lane + 32 * i) key[i] = 0;
     }
     if (lane < p.top) score = q[chosen];
-    if (W32 || pass) break;
+    if (p.weight_f32 != 0 || pass) break;
     // Could the errors of two logits have swapped neighbours?  A score moves by at most its slope
     // times a logit's error: 1/4 for the sigmoid, 2 p with softmax's normaliser.
     const double reach = 2.0 * loss * (p.sigmoid ? 0.25 : 2.0 * score);
@@ -274,20 +274,12 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
   }
 }
 
-template <bool BF16, bool W32, int MT, int NT, int PER>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams p) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  double* part = reinterpret_cast<double*>(smem);  // [warps][16 MT][8 NT], then the |x w| sums
-  float* part_s = reinterpret_cast<float*>(part + kRouteWarps * 128 * MT * NT);
-  __shared__ int last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// K steps first, first + stride, ... below `end` of 16 MT x 8 NT logits (and of their sums |x w|), in
+// the MMA's lane layout: value v of tile (i, j) is token 16 i + 8 (v / 2) + g, expert 8 j + 2 q + v % 2.
+template <bool BF16, bool W32, int MT, int NT>
+__device__ __forceinline__ void route_sums(const RouteParams& p, int t0, int e0, int first, int stride, int end, int lane,
+                                           double (&z)[MT][NT][4], float (&sa)[MT][NT][4]) {
   const int g = lane >> 2, q = lane & 3;
-  const int t0 = blockIdx.y * 16 * MT, e0 = blockIdx.x * 8 * NT;
-  if (threadIdx.x == 0) grid_dep_launch();
-  grid_dep_wait();
-
-  double z[MT][NT][4] = {};
-  float sa[MT][NT][4] = {};
   if constexpr (!W32) {
     long long xo[2 * MT], wo[NT];  // rows past the last token or expert repeat it; nobody reads their sums
 #pragma unroll
@@ -295,7 +287,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
 #pragma unroll
     for (int j = 0; j < NT; ++j) wo[j] = static_cast<long long>(min(e0 + 8 * j + g, p.E - 1)) * p.ldw;
 #pragma unroll(MT == 1 ? 4 : 1)
-    for (int k0 = warp * kRouteStep; k0 < p.K; k0 += kRouteWarps * kRouteStep) {
+    for (int s = first; s < end; s += stride) {
+      const int k0 = s * kRouteStep;
       uint4 xv[2][2 * MT], wv[2][NT];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -324,8 +317,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
     }
   } else {
     const float* w = static_cast<const float*>(p.w);
-    for (int k0 = warp * kRouteStep; k0 < p.K; k0 += kRouteWarps * kRouteStep)
-      for (int k = k0; k < min(k0 + kRouteStep, p.K); ++k) {
+#pragma unroll 1
+    for (int s = first; s < end; s += stride)
+#pragma unroll 4
+      for (int k = s * kRouteStep; k < min((s + 1) * kRouteStep, p.K); ++k) {
         double xd[2 * MT], wd[2 * NT];
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i)
@@ -342,7 +337,20 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
             for (int v = 0; v < 4; ++v) z[i][j][v] = fma(xd[2 * i + v / 2], wd[2 * j + v % 2], z[i][j][v]);
       }
   }
-  // The warps' parts of K, added in warp order.
+}
+
+// Part `kp` of `parts` of K of a tile by a CTA of WARPS warps: each takes every WARPS-th step, their
+// sums are added in warp order and go to part kp of the scratch.
+template <bool BF16, bool W32, int MT, int NT, int WARPS>
+__device__ __forceinline__ void route_tile(const RouteParams& p, int t0, int e0, int kp, int parts, uint8_t* smem) {
+  double* part = reinterpret_cast<double*>(smem);  // [warps][16 MT][8 NT], then the |x w| sums
+  float* part_s = reinterpret_cast<float*>(part + WARPS * 128 * MT * NT);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, q = lane & 3;
+  const int steps = (p.K + kRouteStep - 1) / kRouteStep;
+  double z[MT][NT][4] = {};
+  float sa[MT][NT][4] = {};
+  route_sums<BF16, W32, MT, NT>(p, t0, e0, steps * kp / parts + warp, WARPS, steps * (kp + 1) / parts, lane, z, sa);
   constexpr int kCols = 8 * NT, kCells = 128 * MT * NT;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -352,38 +360,48 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
       for (int v = 0; v < 4; ++v) {
         const int cell = (16 * i + 8 * (v / 2) + g) * kCols + 8 * j + 2 * q + v % 2;
         part[warp * kCells + cell] = z[i][j][v];
-        if (!W32) part_s[warp * kCells + cell] = sa[i][j][v];
+        part_s[warp * kCells + cell] = sa[i][j][v];
       }
   __syncthreads();
-  for (int cell = threadIdx.x; cell < kCells; cell += kRouteThreads) {
+  for (int cell = threadIdx.x; cell < kCells; cell += 32 * WARPS) {
     const int t = t0 + cell / kCols, e = e0 + cell % kCols;
     double sum = 0.0;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kRouteWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       sum += part[w * kCells + cell];
-      if (!W32) s += part_s[w * kCells + cell];
+      s += part_s[w * kCells + cell];
     }
     if (t < p.M && e < p.E) {
-      __stcg(p.logits + static_cast<size_t>(t) * p.E + e, sum);
-      if (!W32) __stcg(p.sums + static_cast<size_t>(t) * p.E + e, s);
+      const size_t at = (static_cast<size_t>(kp) * p.M + t) * p.E + e;
+      __stcg(p.logits + at, sum);
+      __stcg(p.sums + at, s);
     }
   }
-  __threadfence();
   __syncthreads();
+}
+
+template <bool BF16, bool W32, int MT, int NT, int PER>
+__global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t0 = blockIdx.y * 16 * MT;
+  if (threadIdx.x == 0) grid_dep_launch();
+  grid_dep_wait();
+  route_tile<BF16, W32, MT, NT, kRouteWarps>(p, t0, blockIdx.x * 8 * NT, 0, 1, smem);
   if (threadIdx.x == 0) {
-    unsigned old;
+    unsigned old;  // (releases what the whole CTA wrote: the barrier above)
     asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.counters + blockIdx.y) : "memory");
     last = old == gridDim.x - 1;
     if (last) p.counters[blockIdx.y] = 0;  // for the next launch
   }
   __syncthreads();
   if (!last) return;
-  __threadfence();
   double* q_of = reinterpret_cast<double*>(smem) + warp * p.E;  // (the parts have been added up)
 #pragma unroll 1
   for (int t = t0 + warp; t < min(t0 + 16 * MT, p.M); t += kRouteWarps) {
-    route_token<BF16, W32, PER>(p, t, lane, q_of);
+    route_token<BF16, PER>(p, t, lane, q_of);
     __syncwarp();
   }
 }
@@ -494,7 +512,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
   if (threadIdx.x == 0) grid_dep_launch();
   grid_dep_wait();
   const int t = blockIdx.x * kRouteWarps + warp;
-  if (t < p.M) route_token<BF16, false, PER>(p, t, lane, reinterpret_cast<double*>(smem) + warp * p.E);
+  if (t < p.M) route_token<BF16, PER>(p, t, lane, reinterpret_cast<double*>(smem) + warp * p.E);
 }
 
 }  // namespace ffnb200

@@ -11,6 +11,9 @@
 // `blocks` of them (a wait on a barrier costs its thread about 150 clocks, which small slots would
 // spend per step).
 //
+// Routing (experts, if asked for): all CTAs share the router's logits, cut by tokens, experts and K;
+// the CTA that arrives last at 16 tokens chooses for them, a warp per token, and everyone waits
+// for all choices (a launch of its own took 17 to 32 us with cold weights, most of it waiting).
 // First product (the only one of the projection): the weight rows are dealt out evenly over the
 // CTAs (one per SM) in groups -- the projection's rows / CTAs, or 16 rows of an expert -- and a
 // CTA takes each of its tiles over the whole of K, so no sum is ever split between CTAs.
@@ -29,7 +32,7 @@
 // wait is bounded as in ffn_kernel.cuh.
 #pragma once
 
-#include "ffn_kernel.cuh"
+#include "router_kernel.cuh"
 
 namespace ffnb200 {
 
@@ -71,6 +74,8 @@ struct StreamParams {
   const int* ids;            // experts: [tokens][top]
   const float* weights;
   int experts, top;
+  int routed;                // 1: the kernel chooses the experts itself (into ids and weights)
+  RouteParams route;         // counters: of 16 tokens each, then the choices made
   unsigned long long wait_limit_ns;
   int inject;
 };
@@ -270,12 +275,44 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   grid_dep_wait();
 
   if constexpr (MOE) {
+    if (p.routed) {
+      const RouteParams& r = p.route;
+      const int groups = (p.experts + 7) / 8, tiles = (p.tokens + 15) / 16;
+      const int units = groups * tiles * r.parts;
+#pragma unroll 1
+      for (int u = c; u < units; u += C) {  // (token tile fastest: its CTAs share weights)
+        const int tile = u % tiles, v = u / tiles, group = v % groups, kp = v / groups;
+        if (r.weight_f32) route_tile<BF16, true, 1, 1, kStreamThreads / 32>(r, tile * 16, group * 8, kp, r.parts, gbase);
+        else route_tile<BF16, false, 1, 1, kStreamThreads / 32>(r, tile * 16, group * 8, kp, r.parts, gbase);
+        if (threadIdx.x == 0) {
+          unsigned old;  // (releases what the whole CTA wrote: the barrier above)
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(r.counters + tile) : "memory");
+          *last_flag = old == static_cast<unsigned>(groups * r.parts - 1);
+        }
+        __syncthreads();
+        if (*last_flag) {
+          const int t = tile * 16 + warp;
+          double* q = reinterpret_cast<double*>(gbase) + warp * p.experts;
+          if (t < p.tokens) {
+            if (p.experts <= 64) route_token<BF16, 2>(r, t, lane, q);
+            else if (p.experts <= 256) route_token<BF16, 8>(r, t, lane, q);
+            else route_token<BF16, 16>(r, t, lane, q);
+          }
+          __syncthreads();
+          if (threadIdx.x == 0) red_release_add(r.counters + tiles, 1u);
+        }
+        __syncthreads();
+      }
+      if (threadIdx.x == 0) stream_wait_word(r.counters + tiles, static_cast<unsigned>(tiles), abort_flag, p, 2, -2);
+      fence_async_shared();  // the ring's bytes were used above; TMA writes them next
+      __syncthreads();
+    }
     // Pairs (token, expert) ordered by expert, then token: each expert's tokens as a bit set, so
     // that every CTA finds the same order whatever order its threads run in.  A token that names
     // an expert twice is one pair; an id outside [0, experts) is none.
     const int pairs = p.tokens * p.top;
     for (int i = threadIdx.x; i < pairs; i += kStreamThreads) {
-      const int e = __ldg(p.ids + i);
+      const int e = __ldcg(p.ids + i);
       const int t = i / p.top;
       if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts))
         atomicOr(&sets[e * lists.words + (t >> 5)], 1u << (t & 31));
@@ -660,9 +697,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       }
       pieces = 0;
       if (lane < p.top) {
-        const int e = __ldg(p.ids + t * p.top + lane);
+        const int e = __ldcg(p.ids + t * p.top + lane);
         if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts)) {
-          wt = __ldg(p.weights + t * p.top + lane);
+          wt = __ldcg(p.weights + t * p.top + lane);
           int rank = 0;
           for (int w = 0; w < (t >> 5); ++w) rank += __popc(sets[e * lists.words + w]);
           rank += __popc(sets[e * lists.words + (t >> 5)] & ((1u << (t & 31)) - 1u));
@@ -744,6 +781,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     if (*last_flag) {
       for (int i = threadIdx.x; i < items; i += kStreamThreads) item_done[i] = 0;
       if (threadIdx.x < kStreamSync) sync_words[threadIdx.x] = 0;
+      if (p.routed && threadIdx.x <= (p.tokens + 15) / 16) p.route.counters[threadIdx.x] = 0;
     }
   }
 }

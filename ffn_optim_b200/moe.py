@@ -113,9 +113,9 @@ def route_experts(x, weight, **configuration):
 
 
 class PreparedMoE(L.PreparedLayer):
-    """A prepared mixture-of-experts layer.  :meth:`run` routes and computes, :meth:`run_routed`
-    computes with given choices; both return the output viewed as ``(*x.shape[:-1], N)``.
-    ``ids`` and ``weights`` hold the choices of the last :meth:`run`."""
+    """A prepared mixture-of-experts layer.  :meth:`run` routes and computes in one launch,
+    :meth:`run_routed` computes with given choices; both return the output viewed as
+    ``(*x.shape[:-1], N)``.  ``ids`` and ``weights`` hold the choices of the last :meth:`run`."""
 
     def __init__(self, x, router_weight, weight1, weight2, activation, gelu, residual, block_num, routing):
         import torch
@@ -172,7 +172,13 @@ class PreparedMoE(L.PreparedLayer):
         L.raise_for(lib.ffn_b200_moe_prepare(ctypes.byref(prob), ctypes.byref(bufs), x.device.index or 0,
                                              ctypes.byref(handle)), "prepare_moe_ffn")
         self.handle = handle
-        self._run = lib.ffn_b200_moe_run
+        with torch.cuda.device(x.device):
+            self._logits = torch.empty(plan.route_doubles, dtype=torch.float64, device=x.device)
+        r = self.router
+        L.raise_for(lib.ffn_b200_moe_set_router(handle, ctypes.byref(r.problem), *r._fixed, self._logits.data_ptr()),
+                    "prepare_moe_ffn")
+        self._choices = r._outs[:2]
+        self._run, self._run_routed = lib.ffn_b200_moe_run, lib.ffn_b200_moe_run_routed
         self._ldy = self._out.stride(0)
 
     @staticmethod
@@ -191,20 +197,22 @@ class PreparedMoE(L.PreparedLayer):
     def weights(self):
         return self.router._weights
 
-    def _launch(self, stream, x, residual, ids, weights):
+    def _launch(self, stream, fn, x, residual, *choice):
         if self.handle is None:
             raise RuntimeError("PreparedMoE has been closed")
         xp, ldx, xk = self._x.bind(x, "x", self._range)
         rp, ldr, rk = self._r.bind(residual, "residual", self._range) if residual is not None else (None, 0, None)
-        rc = self._run(self.handle, xp, ldx, ids, weights, rp, ldr, self._range[0], self._ldy, stream)
+        rc = fn(self.handle, xp, ldx, *choice, rp, ldr, self._range[0], self._ldy, stream)
         if rc != _lib.OK:
-            raise RuntimeError(f"ffn_b200_moe_run: {_lib.strerror(rc)}")
+            raise RuntimeError(f"moe_ffn: {_lib.strerror(rc)}")
         self._alive = xk, rk
         return self._view
 
     def _layer(self, stream, x, residual, mask):
-        self.router._launch(stream, x, mask)
-        return self._launch(stream, x, residual, self.router._outs[0], self.router._outs[1])
+        mask = self.router._mask_of(mask) if mask is not None else None
+        y = self._launch(stream, self._run, x, residual, mask.data_ptr() if mask is not None else None, *self._choices)
+        self._alive += (mask,)
+        return y
 
     def _capture(self, stream):
         self._layer(stream, self.x, self.residual, self.router.mask)
@@ -217,7 +225,7 @@ class PreparedMoE(L.PreparedLayer):
         return residual
 
     def run(self, x=None, residual=None, mask=None):
-        """The whole layer: router launch, experts launch.  Arguments default to the tensors given
+        """The whole layer, one launch.  Arguments default to the tensors given
         at preparation.  A token whose mask is False asks for no expert: its output is its
         residual, or zero."""
         self._check_stream()
@@ -225,7 +233,7 @@ class PreparedMoE(L.PreparedLayer):
                            self.router.mask if mask is None else mask)
 
     def run_routed(self, ids, weights, x=None, residual=None):
-        """The experts' launch with given choices: ``ids`` int32 and ``weights`` fp32
+        """The layer with given choices: ``ids`` int32 and ``weights`` fp32
         ``(*x.shape[:-1], top_k)``.  An id outside [0, E) contributes nothing (an expert held
         elsewhere, a padded token); an id given twice counts with the sum of its weights."""
         self._check_stream()
@@ -233,8 +241,8 @@ class PreparedMoE(L.PreparedLayer):
             if t.shape != self._choice_shape or t.dtype != dtype or t.device != self.device:
                 raise ValueError(f"{name} must be a {list(self._choice_shape)} tensor of {dtype} on {self.device}")
         ids, weights = ids.contiguous(), weights.contiguous()
-        y = self._launch(self._stream_ptr, self.x if x is None else x, self._residual_of(residual), ids.data_ptr(),
-                         weights.data_ptr())
+        y = self._launch(self._stream_ptr, self._run_routed, self.x if x is None else x, self._residual_of(residual),
+                         ids.data_ptr(), weights.data_ptr())
         self._alive += (ids, weights)
         return y
 

@@ -426,6 +426,7 @@ typedef struct {
   int64_t workspace_floats;
   int64_t counter_words;
   int64_t status_words;
+  int64_t route_doubles;              /* the router's scratch */
 } ffn_b200_moe_plan;
 
 typedef struct {
@@ -443,11 +444,20 @@ typedef struct ffn_b200_moe ffn_b200_moe;
 FFN_B200_EXPORT int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* problem, ffn_b200_moe_plan* plan);
 FFN_B200_EXPORT int ffn_b200_moe_prepare(const ffn_b200_moe_problem* problem, const ffn_b200_moe_buffers* buffers,
                                          int device, ffn_b200_moe** handle);
-/* One asynchronous launch on `stream`; residual may be NULL.  Y must not overlap X or the
+/* The router of ffn_b200_moe_run (a problem of the same m, k, experts, top_k and dtype): weights,
+ * choice_bias (or NULL) and scratch of plan.route_doubles, which must stay valid. */
+FFN_B200_EXPORT int ffn_b200_moe_set_router(ffn_b200_moe* handle, const ffn_b200_router_problem* problem, const void* w,
+                                            int64_t ldw, const float* choice_bias, double* logits);
+/* The whole layer, one asynchronous launch on `stream`: chooses the experts as ffn_b200_router_run does
+ * (into ids and weights) and computes.  mask and residual may be NULL.  Y must not overlap X or the
  * residual.  Runs of one handle must be serialised on one stream (they share its scratch). */
-FFN_B200_EXPORT int ffn_b200_moe_run(ffn_b200_moe* handle, const void* x, int64_t ldx, const int32_t* ids,
-                                     const float* weights, const void* residual, int64_t ldr, void* y, int64_t ldy,
-                                     void* stream);
+FFN_B200_EXPORT int ffn_b200_moe_run(ffn_b200_moe* handle, const void* x, int64_t ldx, const uint8_t* mask,
+                                     int32_t* ids, float* weights, const void* residual, int64_t ldr, void* y,
+                                     int64_t ldy, void* stream);
+/* The same with given choices. */
+FFN_B200_EXPORT int ffn_b200_moe_run_routed(ffn_b200_moe* handle, const void* x, int64_t ldx, const int32_t* ids,
+                                            const float* weights, const void* residual, int64_t ldr, void* y,
+                                            int64_t ldy, void* stream);
 /* Clears counters and status; call after a run reported a kernel error. */
 FFN_B200_EXPORT int ffn_b200_moe_reset(ffn_b200_moe* handle, void* stream);
 /* Bounded waits and the test hook that makes one run out, as for ffn_b200_handle. */

@@ -105,9 +105,10 @@ def test_c_entries_reject_bad_problems(lib):
         assert lib.ffn_b200_moe_make_plan(ctypes.byref(_lib.MoeProblem(*args)), ctypes.byref(mp)) == _lib.ERR_INVALID
     many = _lib.MoeProblem(257, 8, 8, 8, 4, 2, 1, 3, 0, 148)
     assert lib.ffn_b200_moe_make_plan(ctypes.byref(many), ctypes.byref(mp)) == _lib.ERR_TOO_LARGE
-    for fn in (lib.ffn_b200_linear_run, lib.ffn_b200_moe_run):
-        assert fn(None, None, 8, None, *([None] if fn is lib.ffn_b200_moe_run else []),
-                  *([None] if fn is lib.ffn_b200_moe_run else []), 8, None, 8, None) == _lib.ERR_INVALID
+    assert lib.ffn_b200_linear_run(None, None, 8, None, 8, None, 8, None) == _lib.ERR_INVALID
+    assert lib.ffn_b200_moe_run(None, None, 8, None, None, None, None, 8, None, 8, None) == _lib.ERR_INVALID
+    assert lib.ffn_b200_moe_run_routed(None, None, 8, None, None, None, 8, None, 8, None) == _lib.ERR_INVALID
+    assert lib.ffn_b200_moe_set_router(None, None, None, 8, None, None) == _lib.ERR_INVALID
     assert lib.ffn_b200_moe_reset(None, None) == _lib.ERR_INVALID
 
 
