@@ -367,11 +367,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       expert = 0, start = 0, count = p.tokens;
     }
   };
-  // Experts, first product: C / items CTAs per item where that takes no more than a quarter longer than
-  // an even deal (one token, 6 of 64 experts: ends 6 us earlier, as no CTA is left with two tiles).
+  // Experts, first product: C / items CTAs per item where no CTA gets more groups by that than by an
+  // even deal (one token, 6 of 64 experts: ends 6 us earlier, as no CTA is left with two short tiles).
   const int per_item = max(1, MOE && items ? C / items : 1);
-  const bool whole_items =
-      items <= C && 4ll * items * p.groups1 >= 3ll * C * ((p.groups1 + per_item - 1) / per_item);
+  const bool whole_items = items > 0 && items <= C &&
+                           (p.groups1 + per_item - 1) / per_item <= (static_cast<long long>(items) * p.groups1 + C - 1) / C;
   // This CTA's tiles, in the same order for every role: tile(ph, item, g0, groups, k0, k1) returns
   // false to stop.  First product: groups [g0, g0 + groups) of the item over all of K.  Second:
   // tile g0, K steps [k0, k1).

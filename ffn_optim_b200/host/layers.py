@@ -168,12 +168,13 @@ class PreparedLayer:
 
         self._torch = torch
         self.device = device
+        self._index = device.index or 0
         with torch.cuda.device(device):
             self.stream = torch.cuda.current_stream()
         self._stream_ptr = self.stream.cuda_stream
 
     def _check_stream(self):
-        if self._torch.cuda.current_stream(self.device).cuda_stream != self._stream_ptr:
+        if self._torch.cuda.current_stream(self._index).cuda_stream != self._stream_ptr:
             raise RuntimeError(f"{type(self).__name__} must run on its preparation stream; "
                                "concurrent reuse is unsupported")
 
