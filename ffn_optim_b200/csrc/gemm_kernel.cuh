@@ -286,15 +286,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     const bool works = kChunks >= 2 || half == 0;
     const uint32_t stg = sStage + static_cast<uint32_t>((warp - 4) * kStageBufBytes);
     int n_acc = 0;
-#pragma unroll 1
-    for (int t = owner; t < tiles; t += owners, ++n_acc) {
+    uint32_t r[32];  // the next chunk's residual
+    auto place = [&](int t, int& row0, int& first) {
       int tm, tn;
       coords(t, tm, tn);
+      row0 = tm * kTileM + (PAIR ? static_cast<int>(rank) * kBM : 0) + sub * 32;
+      first = tn * BN + half * kMine * 64;
+    };
+    int row0 = 0, first = 0;
+    if (owner < tiles) place(owner, row0, first);
+    if (works && p.residual && owner < tiles) load_row<64>(r, p.residual, p.ldr, row0 + lane, p.M, first, p.N);
+#pragma unroll 1
+    for (int t = owner; t < tiles; t += owners, ++n_acc) {
       const int a = n_acc & 1;
-      const int row0 = tm * kTileM + (PAIR ? static_cast<int>(rank) * kBM : 0) + sub * 32;
-      uint32_t r[32];
-      const int first = tn * BN + half * kMine * 64;
-      if (works && p.residual) load_row<64>(r, p.residual, p.ldr, row0 + lane, p.M, first, p.N);
+      int next_row0 = 0, next_first = 0;
+      const bool more = t + owners < tiles;
+      if (more) place(t + owners, next_row0, next_first);
       int ok = 1;
       if (lane == 0) ok = gemm_wait(tfull_bar(a), (n_acc >> 1) & 1, abort_flag, p, 400 + a) ? 1 : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -314,7 +321,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             else mbar_arrive(tempty_bar(a));
           }
         }
-        if (!works || col0 >= p.N || row0 >= p.M) continue;
+        // The residual of the chunk after this one (of the next tile, if it is the last).
+        auto read_ahead = [&]() {
+          if (!p.residual || !works) return;
+          if (c + 1 < kMine) load_row<64>(r, p.residual, p.ldr, row0 + lane, p.M, col0 + 64, p.N);
+          else if (more) load_row<64>(r, p.residual, p.ldr, next_row0 + lane, p.M, next_first, p.N);
+        };
+        if (!works || col0 >= p.N || row0 >= p.M) {
+          read_ahead();
+          continue;
+        }
         if (p.bias) add_bias<BF16, 64>(v, p.bias, col0, p.N);
         apply_act<64>(v, p.act);
         if (p.residual) {
@@ -323,7 +339,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             v[2 * j] += unpack_lo<BF16>(r[j]);
             v[2 * j + 1] += unpack_hi<BF16>(r[j]);
           }
-          if (c + 1 < kMine) load_row<64>(r, p.residual, p.ldr, row0 + lane, p.M, col0 + 64, p.N);
+          read_ahead();
         }
         if (col0 + 64 > p.N && (p.N & 7) != 0) {
           // (A TMA store clips rows, but columns only to 16 bytes: the last columns go out one by one.)
@@ -344,6 +360,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           bulk_commit();
         }
       }
+      row0 = next_row0, first = next_first;
     }
     if (lane == 0) bulk_wait_all();
     __syncwarp();

@@ -203,8 +203,9 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
     if (lane < p.top) score = q[chosen];
     if (p.weight_f32 != 0 || pass) break;
     // Could the errors of two logits have swapped neighbours?  A score moves by at most its slope
-    // times a logit's error: 1/4 for the sigmoid, 2 p with softmax's normaliser.
-    const double reach = 2.0 * loss * (p.sigmoid ? 0.25 : 2.0 * score);
+    // times a logit's error: p (1 - p) for the sigmoid (a little more, for where p changes on the
+    // way), 2 p with softmax's normaliser.
+    const double reach = 2.0 * loss * (p.sigmoid ? score * (1.0 - score) + loss : 2.0 * score);
     const unsigned long long after = __shfl_down_sync(0xffffffffu, mine, 1);
     const bool last = lane == p.top - 1 && p.top == p.E;
     const double here = unordered(mine);
@@ -245,19 +246,15 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
       const int src = __ffs(todo) - 1;
       const int i = __ffs(__shfl_sync(0xffffffffu, again, src)) - 1;
       const long long wo = static_cast<long long>(src + 32 * i) * p.ldw;
-      double a = 0.0;
-#pragma unroll 1
-      for (int k = 8 * lane; k < p.K; k += 256 * 8) {
-        uint4 xv[8], wv[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          xv[c] = row_chunk(p.x, xo, k + 256 * c, p.K);
-          wv[c] = row_chunk(p.w, wo, k + 256 * c, p.K);
-        }
-#pragma unroll
-        for (int c = 0; c < 8; ++c) a = dot8<BF16>(xv[c], wv[c], a);
+      double a = 0.0, b = 0.0;
+#pragma unroll 2
+      for (int k = 8 * lane; k < p.K; k += 512) {  // (rolled: this code is fetched for a token in hundreds)
+        const uint4 xa = row_chunk(p.x, xo, k, p.K), wa = row_chunk(p.w, wo, k, p.K);
+        const uint4 xb = row_chunk(p.x, xo, k + 256, p.K), wb = row_chunk(p.w, wo, k + 256, p.K);
+        a = dot8<BF16>(xa, wa, a);
+        b = dot8<BF16>(xb, wb, b);
       }
-      a = warp_sum(a);
+      a = warp_sum(a + b);
       if (lane == src) {
 #pragma unroll
         for (int c = 0; c < PER; ++c)

@@ -105,10 +105,10 @@ class RowStorage:
         if addressable(flat, rows, cols) and not out[0] <= ptr < out[1]:
             return ptr, row_pitch(flat, rows, cols), flat
         if self._buf is None:
-            self._buf = _packed(flat, rows, cols)
+            self._buf = _packed(flat, rows, cols)[:, :cols]
         else:
-            self._buf[:, :cols].copy_(flat)
-        return self._buf.data_ptr(), self._buf.stride(0), self._buf
+            self._buf.copy_(flat)
+        return self._buf.data_ptr(), row_pitch(self._buf, rows, cols), self._buf
 
 
 def output_buffer(rows, cols, like):
