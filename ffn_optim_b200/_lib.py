@@ -60,7 +60,8 @@ EXPORTED = ("ffn_b200_abi_version", "ffn_b200_strerror", "ffn_b200_device_info",
             "ffn_b200_router_scratch", "ffn_b200_router_run",
             "ffn_b200_moe_make_plan", "ffn_b200_moe_prepare", "ffn_b200_moe_set_router", "ffn_b200_moe_run",
             "ffn_b200_moe_run_routed", "ffn_b200_moe_reset",
-            "ffn_b200_moe_set_wait_limit", "ffn_b200_moe_set_fault_injection", "ffn_b200_moe_destroy")
+            "ffn_b200_moe_set_wait_limit", "ffn_b200_moe_set_fault_injection", "ffn_b200_moe_destroy",
+            "ffn_b200_pack_rows")
 
 
 class Problem(ctypes.Structure):
@@ -210,6 +211,7 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
             "ffn_b200_moe_set_wait_limit": ([vp, u64], i32),
             "ffn_b200_moe_set_fault_injection": ([vp, i32], i32),
             "ffn_b200_moe_destroy": ([vp], i32),
+            "ffn_b200_pack_rows": ([vp, i64, i64, i64, i64, vp, i64, i32, vp], i32),
         }
         for name, (args, res) in sigs.items():
             fn = getattr(lib, name)

@@ -23,6 +23,7 @@ LIB = LIBDIR / "libffn_b200.so"
 SOURCES = [CSRC / "ffn_capi.cu", CSRC / "ffn_noalloc.cu", CSRC / "ffn_placement.cu", CSRC / "ffn_quant.cu",
            CSRC / "ffn_layers.cu"]
 HEADERS = [CSRC / "ffn_kernel.cuh", CSRC / "ffn_rowblock.cuh", CSRC / "ffn_hslice.cuh", CSRC / "gemm_kernel.cuh",
+           CSRC / "pack_kernel.cuh",
            CSRC / "stream_kernel.cuh", CSRC / "router_kernel.cuh", ROOT / "include" / "ffn_b200.h"]
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
 

@@ -12,6 +12,7 @@
 
 #include "../../include/ffn_b200.h"
 #include "gemm_kernel.cuh"
+#include "pack_kernel.cuh"
 #include "router_kernel.cuh"
 #include "stream_kernel.cuh"
 
@@ -730,6 +731,33 @@ int ffn_b200_moe_set_fault_injection(ffn_b200_moe* h, int mode) {
 int ffn_b200_moe_destroy(ffn_b200_moe* h) {
   delete h;
   return FFN_B200_OK;
+}
+
+// ---- operand packing -----------------------------------------------------------------------
+int ffn_b200_pack_rows(const void* src, int64_t row_stride, int64_t col_stride, int64_t rows, int64_t cols, void* dst,
+                       int64_t ld, int device, void* stream) {
+  if (!src || !dst || rows <= 0 || cols <= 0 || cols > kMaxDim || row_stride < 0 || col_stride < 0 || ld < cols)
+    return FFN_B200_ERR_INVALID;
+  const int64_t tiles = cdiv(rows, ffnb200::kPackTile);
+  if (tiles >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
+  DeviceScope scope(device);
+  if (!scope.ok) return FFN_B200_ERR_DEVICE;
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(cdiv(cols, ffnb200::kPackTile)), 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, ffnb200::pack_rows_kernel, static_cast<const uint16_t*>(src), static_cast<long long>(row_stride),
+                         static_cast<long long>(col_stride), static_cast<long long>(rows), static_cast<int>(cols),
+                         static_cast<uint16_t*>(dst), static_cast<long long>(ld)) == cudaSuccess)
+    return FFN_B200_OK;
+  cudaGetLastError();
+  return FFN_B200_ERR_CUDA;
 }
 
 }  // extern "C"

@@ -5,7 +5,7 @@ from __future__ import annotations
 
 from math import prod
 
-from .inputs import _packed, pitch_of
+from .inputs import pitch_of
 
 MAX_DIM = 65535
 MAX_ROWS = 2**31 - 16
@@ -53,15 +53,6 @@ def require_cuda(x, what):
         raise ValueError(f"{what} requires CUDA tensors; no CPU fallback is used")
 
 
-def addressable(t, rows, cols):
-    """True when ``t`` is a [rows, cols] view whose rows the kernels can read in place: unit
-    column stride, 16-byte base and row pitch (the pitch of a single row is never used)."""
-    if t.dim() != 2 or t.stride(1) != 1 and cols > 1 or t.data_ptr() & 15:
-        return False
-    ld = t.stride(0)
-    return rows == 1 or ld % 8 == 0 and ld >= cols
-
-
 def row_pitch(t, rows, cols):
     return t.stride(0) if rows > 1 else pitch_of(cols)
 
@@ -85,30 +76,40 @@ class RowStorage:
     rows are addressable, else a copy in storage owned by the operator."""
 
     def __init__(self, rows, cols, like, shape):
-        import torch
-
         self.rows, self.cols, self.shape = rows, cols, tuple(shape)
         self.dtype, self.device = like.dtype, like.device
-        self._torch = torch
-        self._buf = None
+        self._pitch, self._buf, self._pack = pitch_of(cols), None, None
 
-    def bind(self, t, name, out):
-        """(address, row pitch, the tensor that must stay alive); ``out`` is the output buffer a
-        kernel run writes, which an operand may not overlap: such a view is copied first."""
+    def bind(self, t, name, out, stream):
+        """(address, row pitch, the tensor that must stay alive) for a launch on ``stream``; ``out`` is
+        the output's address range, which an operand may not overlap: such a view is copied first."""
         if t.shape != self.shape or t.dtype != self.dtype or t.device != self.device:
             raise ValueError(f"{name} must have the prepared shape, dtype and device")
         if t.requires_grad:
             raise ValueError(f"{name}: inference-only operator; detach inputs explicitly")
         rows, cols = self.rows, self.cols
-        flat = t if t.dim() == 2 else t.reshape(rows, cols)
-        ptr = flat.data_ptr()
-        if addressable(flat, rows, cols) and not out[0] <= ptr < out[1]:
-            return ptr, row_pitch(flat, rows, cols), flat
+        if t.dim() != 2:
+            t = t.reshape(rows, cols)
+        ptr, (row, col) = t.data_ptr(), t.stride()
+        if (col == 1 or cols == 1) and not ptr & 15 and not out[0] <= ptr < out[1]:
+            if rows == 1:
+                return ptr, self._pitch, t
+            if not row & 7 and row >= cols:
+                return ptr, row, t
+        return self._packed(t, ptr, row, col, stream)
+
+    def _packed(self, t, ptr, row, col, stream):
+        from .. import _lib
+
         if self._buf is None:
-            self._buf = _packed(flat, rows, cols)[:, :cols]
-        else:
-            self._buf.copy_(flat)
-        return self._buf.data_ptr(), row_pitch(self._buf, rows, cols), self._buf
+            import torch
+
+            self._buf = torch.empty((self.rows, self._pitch), dtype=self.dtype, device=self.device)
+            self._pack = _lib.load().ffn_b200_pack_rows
+        buf = self._buf.data_ptr()
+        rc = self._pack(ptr, row, col, self.rows, self.cols, buf, self._pitch, self.device.index or 0, stream)
+        raise_for(rc, "ffn_b200_pack_rows")
+        return buf, self._pitch, t
 
 
 def output_buffer(rows, cols, like):

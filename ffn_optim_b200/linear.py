@@ -77,12 +77,12 @@ class PreparedLinear(L.PreparedLayer):
     def _launch(self, stream, x, residual):
         if self.handle is None:
             raise RuntimeError("PreparedLinear has been closed")
-        xp, ldx, xk = self._x.bind(x, "x", self._range)
-        rp, ldr, rk = self._r.bind(residual, "residual", self._range) if residual is not None else (None, 0, None)
+        xp, ldx, xk = self._x.bind(x, "x", self._range, stream)
+        rp, ldr, rk = self._r.bind(residual, "residual", self._range, stream) if residual is not None else (None, 0, None)
         rc = self._run(self.handle, xp, ldx, rp, ldr, self._range[0], self._ldy, stream)
         if rc != _lib.OK:
             raise RuntimeError(f"ffn_b200_linear_run: {_lib.strerror(rc)}")
-        self._alive = xk, rk  # a copy made for this launch lives until the next one
+        self._alive = xk, rk  # (a reshaped copy lives until the next launch)
 
     def _capture(self, stream):
         self._launch(stream, self.x, self.residual)

@@ -75,7 +75,7 @@ class PreparedRouter(L.PreparedLayer):
         return mask if mask.is_contiguous() else mask.contiguous()
 
     def _launch(self, stream, x, mask):
-        xp, ldx, xk = self._x.bind(x, "x", (0, 0))
+        xp, ldx, xk = self._x.bind(x, "x", (0, 0), stream)
         mask = self._mask_of(mask) if mask is not None else None
         with self._torch.cuda.device(self.device):
             rc = self._fn(self._prob_ptr, xp, ldx, *self._fixed, mask.data_ptr() if mask is not None else None,
@@ -200,8 +200,8 @@ class PreparedMoE(L.PreparedLayer):
     def _launch(self, stream, fn, x, residual, *choice):
         if self.handle is None:
             raise RuntimeError("PreparedMoE has been closed")
-        xp, ldx, xk = self._x.bind(x, "x", self._range)
-        rp, ldr, rk = self._r.bind(residual, "residual", self._range) if residual is not None else (None, 0, None)
+        xp, ldx, xk = self._x.bind(x, "x", self._range, stream)
+        rp, ldr, rk = self._r.bind(residual, "residual", self._range, stream) if residual is not None else (None, 0, None)
         rc = fn(self.handle, xp, ldx, *choice, rp, ldr, self._range[0], self._ldy, stream)
         if rc != _lib.OK:
             raise RuntimeError(f"moe_ffn: {_lib.strerror(rc)}")

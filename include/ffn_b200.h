@@ -465,6 +465,11 @@ FFN_B200_EXPORT int ffn_b200_moe_set_wait_limit(ffn_b200_moe* handle, uint64_t n
 FFN_B200_EXPORT int ffn_b200_moe_set_fault_injection(ffn_b200_moe* handle, int mode);
 FFN_B200_EXPORT int ffn_b200_moe_destroy(ffn_b200_moe* handle);
 
+/* Copies a strided [rows, cols] view of 16-bit values (strides in elements, not negative) into rows of
+ * pitch ld: an operand whose own rows the kernels above cannot address.  Asynchronous on `stream`. */
+FFN_B200_EXPORT int ffn_b200_pack_rows(const void* src, int64_t row_stride, int64_t col_stride, int64_t rows,
+                                       int64_t cols, void* dst, int64_t ld, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

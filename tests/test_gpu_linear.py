@@ -92,6 +92,21 @@ def test_strided_operands(m):
         assert y.shape == (*lead, n) and torch.equal(y.reshape(m, n), want)
 
 
+@pytest.mark.parametrize("shape", [(1, 1), (7, 500), (33, 100), (6993, 100), (100, 4097)])
+def test_packed_views(shape):
+    """Every kind of view the kernels cannot address, through the packing kernel: equal values."""
+    from ffn_optim_b200.host import layers as L
+
+    m, k = shape
+    flat = torch.randn(2 * m * (2 * k + 3) + 8, device="cuda").to(HF)
+    views = [flat[1:1 + m * k].view(m, k), flat[:m * k].view(k, m).t(), flat[:m * (2 * k + 1)].view(m, 2 * k + 1)[:, 1::2],
+             flat[3:3 + k].view(1, k).expand(m, k), flat[:m].view(m, 1).expand(m, k)]
+    for v in views:
+        store = L.RowStorage(m, k, v, v.shape)
+        ptr, pitch, _ = store._packed(v, v.data_ptr(), *v.stride(), torch.cuda.current_stream().cuda_stream)
+        assert ptr == store._buf.data_ptr() and torch.equal(store._buf[:, :k], v)
+
+
 @pytest.mark.parametrize("m", [1, 24, 640, 4096])
 def test_new_inputs_repeat_and_leave_nothing_behind(m):
     """One handle over changing inputs equals a fresh handle on each, bit for bit, and NaN or

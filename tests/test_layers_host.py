@@ -146,24 +146,53 @@ def test_moe_plans(lib):
                 assert plan.sorted_pitch in (0, 4096)
 
 
+class FakePack:
+    """Records the packing calls that RowStorage makes instead of launching them."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __call__(self, *args):
+        self.calls.append(args)
+        return _lib.OK
+
+
 def test_operands_read_in_place_or_copied():
     """Which views the kernels read in place: unit column stride, 16-byte base, pitch a multiple of 8."""
     base = torch.zeros(9 * 40, dtype=torch.bfloat16)
     assert base.data_ptr() % 16 == 0
     m = base.view(9, 40)
-    assert L.addressable(m, 9, 40) and L.addressable(m[:, 8:30], 9, 22) and L.addressable(m[:1, :7], 1, 7)
-    assert not L.addressable(m[:, 4:30], 9, 26)       # base off the 16-byte grid
-    assert not L.addressable(m.t(), 40, 9)            # columns not contiguous
-    assert not L.addressable(base[:39 * 9].view(9, 39), 9, 39)  # odd pitch
-    assert not L.addressable(m[:1].expand(9, 40), 9, 40)        # rows on top of one another
+
+    def bind(t, out=(0, 0)):
+        store = L.RowStorage(t.shape[0], t.shape[1], t, t.shape)
+        store._buf, store._pack = torch.zeros(t.shape[0], L.pitch_of(t.shape[1]), dtype=t.dtype), FakePack()
+        ptr, pitch, _ = store.bind(t, "x", out, None)
+        assert (ptr == store._buf.data_ptr()) == bool(store._pack.calls)
+        return not store._pack.calls, pitch
+
+    assert bind(m) == (True, 40) and bind(m[:, 8:30]) == (True, 40) and bind(m[:1, :7]) == (True, 8)
+    assert bind(m[:, 4:30]) == (False, 32)                     # base off the 16-byte grid
+    assert bind(m.t()) == (False, 16)                          # columns not contiguous
+    assert bind(base[:39 * 9].view(9, 39)) == (False, 40)      # odd pitch
+    assert bind(m[:1].expand(9, 40)) == (False, 40)            # rows on top of one another
+    own = (m.data_ptr(), m.data_ptr() + m.numel() * 2)
+    assert bind(m[1:], own) == (False, 40)                     # inside the output
     w = torch.zeros(4, 6, 24, dtype=torch.bfloat16)
     assert L.packed_weight(w) is w and L.packed_weight(w[:, ::2]).data_ptr() == w.data_ptr()
     odd = torch.randn(4, 6, 21).to(torch.bfloat16)
     packed = L.packed_weight(odd)
     assert torch.equal(packed, odd) and packed.stride() == (6 * 24, 24, 1)
     store = L.RowStorage(9, 40, m, m.shape)
-    assert store.bind(m, "x", (0, 0))[0] == m.data_ptr()
-    own = (m.data_ptr(), m.data_ptr() + m.numel() * 2)
-    assert store.bind(m[:, :], "x", own)[0] != m.data_ptr()     # inside the output: copied
-    with pytest.raises(ValueError, match="prepared shape"):
-        store.bind(m[:8], "x", (0, 0))
+    for bad in (m[:8], m.half(), m.view(9, 40, 1)):
+        with pytest.raises(ValueError, match="prepared shape"):
+            store.bind(bad, "x", (0, 0), None)
+    with pytest.raises(ValueError, match="detach"):
+        store.bind(m.clone().requires_grad_(), "x", (0, 0), None)
+
+
+def test_pack_rows_rejects_bad_arguments(lib):
+    ok = [1 << 20, 40, 1, 9, 33, 1 << 21, 40, 0, None]
+    for i, v in ((0, None), (5, None), (1, -1), (2, -1), (3, 0), (4, 0), (4, 70000), (6, 32)):
+        args = list(ok)
+        args[i] = v
+        assert lib.ffn_b200_pack_rows(*args) == _lib.ERR_INVALID
