@@ -58,19 +58,6 @@ __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-template <int W>
-__device__ __forceinline__ void apply_act(float* v, int act) {
-  if (act == 0) {
-#pragma unroll
-    for (int j = 0; j < W; j += 2) gelu_rational2(v[j], v[j + 1]);
-  } else if (act == 1) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = gelu_erf(v[j]);
-  } else if (act == 2) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = silu(v[j]);
-  }
-}
 // W residual values of one row (two per word) from column c0; zero outside the matrix.
 template <int W>
 __device__ __forceinline__ void load_row(uint32_t* r, const uint16_t* base, long long ld, int row, int rows, int c0, int cols) {

@@ -102,19 +102,23 @@ struct StreamLists {
   }
 };
 
-// `total` things in a line dealt out over at most `grid` CTAs in even stretches of at least `least`.
+// `total` things in a line dealt out over at most `grid` CTAs in stretches that differ by one at most, of at
+// least `least` each.  (32-bit divisions: every role does this before its first load or wait.)
 struct StreamSplit {
-  long long total;
-  int ctas;
-  __device__ StreamSplit(long long n, int grid, int least) : total(n) {
-    const long long most = n / least;
-    ctas = most < 1 ? 1 : (most < grid ? static_cast<int>(most) : grid);
+  unsigned ctas, each, more;  // the first `more` CTAs take each + 1
+  __device__ StreamSplit(unsigned total, unsigned grid, unsigned least) {
+    const unsigned most = total / least;
+    ctas = most < 1u ? 1u : (most < grid ? most : grid);
+    each = total / ctas;
+    more = total - each * ctas;
   }
-  __device__ int begin(int c) const {
-    return c >= ctas ? static_cast<int>(total) : static_cast<int>(total * c / ctas);
+  __device__ int begin(unsigned c) const {
+    c = min(c, ctas);
+    return static_cast<int>(c * each + min(c, more));
   }
-  __device__ int cta_of(int i) const {
-    return static_cast<int>(((static_cast<long long>(i) + 1) * ctas - 1) / total);
+  __device__ int cta_of(unsigned i) const {
+    const unsigned big = more * (each + 1);
+    return static_cast<int>(i < big ? i / (each + 1) : more + (i - big) / each);
   }
 };
 
@@ -158,11 +162,18 @@ __device__ __forceinline__ unsigned atom_add_acq_rel(unsigned* p, unsigned v) {
   asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
   return old;
 }
-__device__ __forceinline__ float act_value(float z, int act) {
-  if (act == 0) return gelu_rational(z);
-  if (act == 1) return gelu_erf(z);
-  if (act == 2) return silu(z);
-  return z;
+template <int W>
+__device__ __forceinline__ void apply_act(float* v, int act) {
+  if (act == 0) {
+#pragma unroll
+    for (int j = 0; j < W; j += 2) gelu_rational2(v[j], v[j + 1]);
+  } else if (act == 1) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = gelu_erf(v[j]);
+  } else if (act == 2) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = silu(v[j]);
+  }
 }
 __device__ __forceinline__ bool stream_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                             const StreamParams& p, int aux) {
@@ -371,13 +382,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   // even deal (one token, 6 of 64 experts: ends 6 us earlier, as no CTA is left with two short tiles).
   const int per_item = max(1, MOE && items ? C / items : 1);
   const bool whole_items = items > 0 && items <= C &&
-                           (p.groups1 + per_item - 1) / per_item <= (static_cast<long long>(items) * p.groups1 + C - 1) / C;
+                           (p.groups1 + per_item - 1) / per_item <= (items * p.groups1 + C - 1) / C;
   // This CTA's tiles, in the same order for every role: tile(ph, item, g0, groups, k0, k1) returns
   // false to stop.  First product: groups [g0, g0 + groups) of the item over all of K.  Second:
   // tile g0, K steps [k0, k1).
   auto for_tiles = [&](auto&& tile) {
     if (items == 0) return;
-    const StreamSplit rows(static_cast<long long>(items) * p.groups1, C, 1);
+    const StreamSplit rows(items * p.groups1, C, 1);
     int g = rows.begin(c), end = rows.begin(c + 1);
     if (MOE && whole_items) {
       // Few items: each gets CTAs of its own, so that none has two short tiles instead of one.
@@ -396,7 +407,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       g += n;
     }
     if constexpr (MOE) {
-      const StreamSplit line(static_cast<long long>(items) * p.tiles2 * p.steps2, C, kStreamMinSteps);
+      const StreamSplit line(items * p.tiles2 * p.steps2, C, kStreamMinSteps);
       for (int s = line.begin(c), end = line.begin(c + 1); s < end;) {
         const int u = s / p.steps2, k0 = s - u * p.steps2, k1 = min(p.steps2, k0 + end - s);
         const int it = u / p.tiles2;
@@ -593,17 +604,27 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         const int feature = glu ? (g0 + (row >> 4)) * p.group_feats + (row & 7) : g0 * p.group_feats + row;
         const bool live = row < n * p.group_rows && feature < p.feat1;
         const float bias = !MOE && p.bias && live ? unpack_lo<BF16>(static_cast<uint32_t>(__ldg(p.bias + feature))) : 0.f;
+        // 8 columns at a time: for few tokens fetching the code costs more than running it.
+        uint32_t r[8];
+        auto read_ahead = [&](int c0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            r[j] = p.residual && live && c0 + j < count
+                       ? static_cast<uint32_t>(__ldg(p.residual + static_cast<long long>(c0 + j) * p.ldr + feature))
+                       : 0u;
+        };
+        if constexpr (!MOE) read_ahead(0);
 #pragma unroll 1
-        for (int c0 = 0; c0 < count; c0 += 16) {
-          float v[16];
+        for (int c0 = 0; c0 < count; c0 += 8) {
+          float v[8];
+          tmem_ld8(acc + c0, v);
           if constexpr (MOE) {
-            tmem_ld16(acc + c0, v);
             if (glu) {
               // Lane l holds a gate row, lane l + 8 the matching up row: of each column pair the
               // lower lane finishes the first, the upper lane the second.
               const bool low = (lane & 8) == 0;
 #pragma unroll
-              for (int j = 0; j < 16; j += 2) {
+              for (int j = 0; j < 8; j += 2) {
                 const float got = __shfl_xor_sync(0xffffffffu, low ? v[j + 1] : v[j], 8);
                 const float gate = low ? v[j] : got, up = low ? got : v[j + 1];
                 const int col = c0 + j + (low ? 0 : 1);
@@ -611,24 +632,25 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
                   p.hidden[static_cast<long long>(start + col) * p.ldh + feature] = cvt1<BF16>(silu(gate) * up);
               }
             } else {
+              apply_act<8>(v, p.act);
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
+              for (int j = 0; j < 8; ++j)
                 if (live && c0 + j < count)
-                  p.hidden[static_cast<long long>(start + c0 + j) * p.ldh + feature] = cvt1<BF16>(act_value(v[j], p.act));
+                  p.hidden[static_cast<long long>(start + c0 + j) * p.ldh + feature] = cvt1<BF16>(v[j]);
             }
           } else {
-            float r[16];
+            uint32_t now[8];
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              r[j] = p.residual && live && c0 + j < count
-                         ? unpack_lo<BF16>(static_cast<uint32_t>(
-                               __ldg(p.residual + static_cast<long long>(c0 + j) * p.ldr + feature)))
-                         : 0.f;
-            tmem_ld16(acc + c0, v);
+            for (int j = 0; j < 8; ++j) {
+              now[j] = r[j];
+              v[j] += bias;
+            }
+            if (c0 + 8 < count) read_ahead(c0 + 8);
+            apply_act<8>(v, p.act);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
+            for (int j = 0; j < 8; ++j)
               if (live && c0 + j < count)
-                p.y[static_cast<long long>(c0 + j) * p.ldy + feature] = cvt1<BF16>(act_value(v[j] + bias, p.act) + r[j]);
+                p.y[static_cast<long long>(c0 + j) * p.ldy + feature] = cvt1<BF16>(v[j] + unpack_lo<BF16>(now[j]));
           }
         }
         if constexpr (MOE) {
@@ -672,7 +694,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     // (token, 128 output features) and adds the token's experts in order, each expert's pieces in
     // ascending CTA order, with the fp32 weights, then the residual; rounded once.
     // What the sums do not depend on is looked up before the wait.
-    const StreamSplit line(static_cast<long long>(items) * p.tiles2 * p.steps2, C, kStreamMinSteps);
+    const StreamSplit line(items * p.tiles2 * p.steps2, C, kStreamMinSteps);
     const size_t pitch = static_cast<size_t>(p.tiles2) * kBM;
     const size_t slot = static_cast<size_t>(p.chunk) * kBM;
     const int n_units = p.tokens * p.tiles2;
