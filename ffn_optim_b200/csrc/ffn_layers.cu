@@ -525,6 +525,7 @@ int ffn_b200_router_run(const ffn_b200_router_problem* pr, const void* x, int64_
   const RouteFns& fns = pr->dtype == FFN_B200_BF16 ? kRouteFns[per][1] : kRouteFns[per][0];
   if (!many) return launch_route(w32 ? fns.few32 : fns.few, P, 1, 1, stream);  // small tiles: more CTAs
   if (w32) return launch_route(fns.many32, P, 2, 4, stream);
+  P.many = 1;
   const dim3 tiles(static_cast<unsigned>(cdiv(P.E, ffnb200::kLogitTile)), static_cast<unsigned>(cdiv(P.M, ffnb200::kLogitTile)),
                    static_cast<unsigned>(P.parts));
   const int rc2 = launch_route(fns.logits, P, tiles, ffnb200::kLogitSmem, stream);

@@ -4,8 +4,10 @@
 // cores rather than of fp64 arithmetic (64 multiply-adds per clock and SM):
 //   * 16-bit weights: products on mma.sync (m16n8k16, fp32 accumulation) in chains of 64 of K; each
 //     chain's fp32 result is added in fp64.  A chain of four MMAs loses at most 4 * 2^-22 of the
-//     sum of its |x w|, so a logit is off by at most 2^-20 S, S = sum |x w|, which a second set
-//     of MMAs over the operands with their signs cleared gives.
+//     sum of its |x w|, so a logit is off by at most 2^-20 S, S = sum |x w|.  For few tokens a
+//     second set of MMAs over the operands with their signs cleared gives S; for many, where
+//     mma.sync is the bound (1000 tokens of 256 experts of 4096: 29 us with it), the norms of the
+//     two rows bound it.
 //   * The finishing warp picks the top k + 1 keys; experts whose key lies closer to one of them
 //     than those errors allow (and logits that left fp32's range) are summed again in fp64, by the
 //     whole warp, and the choice is made again.  For normally distributed logits that is a
@@ -41,8 +43,8 @@ struct RouteParams {
   int* ids;
   float* weights;
   double* logits;   // [parts][M][E]: sums over a part of K
-  float* sums;      // [parts][M][E]: sum |x w|
-  int parts;
+  float* sums;      // [parts][M][E]: sum |x w|; of many tokens [parts][M + E]: sum x^2, then sum w^2
+  int parts, many;
   unsigned* counters;
   int M, K, E, top;
   int weight_f32, sigmoid, renormalize;
@@ -120,28 +122,40 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
   double z[PER], bias[PER];
   float s = 0.f;
   bool odd = false;  // a logit left fp32's range
-  const size_t cells = static_cast<size_t>(p.M) * p.E;
+  // All of a part's loads are in flight together.
+  const size_t cells = static_cast<size_t>(p.M) * p.E, pitch = p.many ? p.M + p.E : cells;
+  const size_t at = static_cast<size_t>(t) * p.E + lane;
+  const float* sum = p.sums + (p.many ? p.M + lane : at);
+  float size[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) z[i] = 0.0, size[i] = 0.f, bias[i] = 0.0;
+#pragma unroll 1
+  for (int c = 0; c < p.parts; ++c) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < p.E) {
+        z[i] += __ldcg(p.logits + c * cells + at + 32 * i);
+        size[i] += __ldcg(sum + c * pitch + 32 * i);
+      }
+  }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = lane + 32 * i;
-    z[i] = -INFINITY, bias[i] = 0.0;
-    if (e < p.E) {
-      const size_t at = static_cast<size_t>(t) * p.E + e;
-      z[i] = __ldcg(p.logits + at);
-      float size = p.weight_f32 != 0 ? 0.f : __ldcg(p.sums + at);
-      if (p.choice_bias) bias[i] = static_cast<double>(__ldg(p.choice_bias + e));
-#pragma unroll 2
-      for (int c = 1; c < p.parts; ++c) {
-        z[i] += __ldcg(p.logits + c * cells + at);
-        size += __ldcg(p.sums + c * cells + at);
-      }
-      s = fmaxf(s, size);
-      odd |= p.weight_f32 == 0 && !isfinite(z[i]);
+    if (lane + 32 * i < p.E) {
+      if (p.choice_bias) bias[i] = static_cast<double>(__ldg(p.choice_bias + lane + 32 * i));
+      s = fmaxf(s, size[i]);
+      odd |= !p.weight_f32 && !isfinite(z[i]);
+    } else {
+      z[i] = -INFINITY;
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
-  const double loss = kRouteLoss * static_cast<double>(s);
+  if (p.many) {  // |x| |w| of the longest w
+    float x2 = 0.f;
+    for (int c = 0; c < p.parts; ++c) x2 += __ldcg(p.sums + static_cast<size_t>(c) * (p.M + p.E) + t);
+    s = sqrtf(x2) * sqrtf(s) * 1.001f;  // (the sums of squares are fp32)
+  }
+  const double loss = p.weight_f32 ? 0.0 : kRouteLoss * static_cast<double>(s);
   int chosen = -1;     // lane j < top: the j-th choice,
   double score = 0.0;  // its score
 #pragma unroll 1
@@ -418,7 +432,8 @@ __device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr) {
   return v;
 }
 
-// Part blockIdx.z of K of a 64 x 64 tile of logits: warps 2 x 4, each 32 tokens x 16 experts.
+// Part blockIdx.z of K of a 64 x 64 tile of logits: warps 2 x 4, each 32 tokens x 16 experts (warp 0
+// and 1 the first 16 experts, even warps the first 32 tokens).
 template <bool BF16>
 __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const RouteParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -451,8 +466,19 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   const int m0 = (warp & 1) * 32, n0 = (warp >> 1) * 16;  // of the tile
+  // Squares of the rows this warp has in hand anyway: tokens in the first column of tiles, experts in the first row.
+  const bool x_norm = blockIdx.x == 0 && warp < 2, w_norm = blockIdx.y == 0 && (warp & 1) == 0;
+  float x2[4] = {}, w2[2] = {};
+  auto squares = [](const uint4& v, float s) {
+    const uint32_t r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s = fmaf(unpack_lo<BF16>(r[i]), unpack_lo<BF16>(r[i]), s);
+      s = fmaf(unpack_hi<BF16>(r[i]), unpack_hi<BF16>(r[i]), s);
+    }
+    return s;
+  };
   double z[2][2][4] = {};
-  float sa[2][2][4] = {};
 #pragma unroll 1
   for (int s = s0; s < s1; ++s) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kLogitStages - 2) : "memory");
@@ -472,13 +498,18 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          constexpr uint32_t kAbs = 0x7FFF7FFFu;
           const uint4 &a = xv[2 * i], &b = xv[2 * i + 1], &w = wv[j];
           mma_16816<BF16>(d[i][j], a.x, b.x, a.y, b.y, w.x, w.y);
           mma_16816<BF16>(d[i][j], a.z, b.z, a.w, b.w, w.z, w.w);
-          mma_16816<BF16>(sa[i][j], a.x & kAbs, b.x & kAbs, a.y & kAbs, b.y & kAbs, w.x & kAbs, w.y & kAbs);
-          mma_16816<BF16>(sa[i][j], a.z & kAbs, b.z & kAbs, a.w & kAbs, b.w & kAbs, w.z & kAbs, w.w & kAbs);
         }
+      if (x_norm) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x2[i] = squares(xv[i], x2[i]);
+      }
+      if (w_norm) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) w2[j] = squares(wv[j], w2[j]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -495,11 +526,23 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int t = t0 + m0 + 16 * i + 8 * (v / 2) + g, e = e0 + n0 + 8 * j + 2 * q + v % 2;
-        if (t < p.M && e < p.E) {
-          p.logits[part + static_cast<size_t>(t) * p.E + e] = z[i][j][v];
-          p.sums[part + static_cast<size_t>(t) * p.E + e] = sa[i][j][v];
-        }
+        if (t < p.M && e < p.E) p.logits[part + static_cast<size_t>(t) * p.E + e] = z[i][j][v];
       }
+  // A row's squares lie with the four lanes of its group.
+  float* norms = p.sums + static_cast<size_t>(blockIdx.z) * (p.M + p.E);
+  auto put = [&](float s, int at, int end, float* to) {
+    s += __shfl_xor_sync(0xffffffffu, s, 1);
+    s += __shfl_xor_sync(0xffffffffu, s, 2);
+    if (q == 0 && at < end) to[at] = s;
+  };
+  if (x_norm) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) put(x2[i], t0 + m0 + 8 * i + g, p.M, norms);
+  }
+  if (w_norm) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) put(w2[j], e0 + n0 + 8 * j + g, p.E, norms + p.M);
+  }
 }
 
 template <bool BF16, int PER>
