@@ -238,7 +238,8 @@ int launch_route(RouteFn fn, const ffnb200::RouteParams& P, dim3 grid, int smem,
 // One kernel of 16 mt x 8 nt tiles; shared memory: the warps' parts of K, then logits and scores.
 int launch_route(RouteFn fn, const ffnb200::RouteParams& P, int mt, int nt, void* stream) {
   const dim3 grid(static_cast<unsigned>(cdiv(P.E, 8 * nt)), static_cast<unsigned>(cdiv(P.M, 16 * mt)), 1);
-  return launch_route(fn, P, grid, ffnb200::kRouteWarps * std::max(128 * mt * nt * 12, P.E * 8), stream);
+  return launch_route(fn, P, grid, std::max(ffnb200::kRouteWarps * 128 * mt * nt * 12, ffnb200::route_space<ffnb200::kRouteWarps>(P.E)),
+                      stream);
 }
 
 int set_smem(const void* fn, int64_t smem) {
@@ -531,7 +532,7 @@ int ffn_b200_router_run(const ffn_b200_router_problem* pr, const void* x, int64_
   const int rc2 = launch_route(fns.logits, P, tiles, ffnb200::kLogitSmem, stream);
   if (rc2) return rc2;
   return launch_route(fns.choose, P, dim3(static_cast<unsigned>(cdiv(P.M, ffnb200::kRouteWarps)), 1, 1),
-                      ffnb200::kRouteWarps * P.E * 8, stream);
+                      ffnb200::route_space<ffnb200::kRouteWarps>(P.E), stream);
 }
 
 // ---- mixture-of-experts layer --------------------------------------------------------------

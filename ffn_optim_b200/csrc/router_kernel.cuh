@@ -108,60 +108,35 @@ __device__ __forceinline__ double unordered(unsigned long long k) {
   return __longlong_as_double(b < 0 ? b ^ static_cast<long long>(1ull << 63) : ~b);
 }
 
-// One token's choice by a warp: lane l holds experts l, l + 32, ... (PER of them) in registers; q: this
-// warp's scores in shared memory [E].  (Code that runs once per token is fetched more slowly than it
-// runs: only the short loops over a lane's own experts are unrolled.)
-template <bool BF16, int PER>
-__device__ __forceinline__ void route_token(const RouteParams& p, int t, int lane, double* q) {
+// The choice for one token per warp by a CTA's WARPS warps together (token t of this warp; t >= M: none):
+// lane l holds experts l, l + 32, ... (PER of them) in registers.  smem: RouteSpace bytes.  Only
+// sums taken again need the whole CTA: each is split over its warps, since one warp's trips through
+// K would keep all the others waiting.  (Code that runs once per token is fetched more slowly than
+// it runs: only the short loops over a lane's own experts are unrolled.)
+constexpr int kAgainSlots = 4;  // sums again that a warp asks for at a time
+template <int WARPS>
+__host__ __device__ constexpr int route_space(int experts) {
+  return WARPS * experts * 8 + WARPS * kAgainSlots * (WARPS * 8 + 4);
+}
+template <bool BF16, int PER, int WARPS>
+__device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_t* smem) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double* q = reinterpret_cast<double*>(smem) + warp * p.E;  // this warp's scores
+  double* part = reinterpret_cast<double*>(smem) + WARPS * p.E;  // [warp][slot][part of K]
+  int* slots = reinterpret_cast<int*>(part + WARPS * kAgainSlots * WARPS);  // [warp][slot]: expert, or -1
   int* ids = p.ids + static_cast<size_t>(t) * p.top;
   float* weights = p.weights + static_cast<size_t>(t) * p.top;
-  if (p.mask && !p.mask[t]) {
+  const bool live = t < p.M && (!p.mask || p.mask[t]);
+  if (!live && t < p.M)
     for (int j = lane; j < p.top; j += 32) ids[j] = -1, weights[j] = 0.f;
-    return;
-  }
-  double z[PER], bias[PER];
+  double z[PER], bias[PER], v[PER];
   float s = 0.f;
   bool odd = false;  // a logit left fp32's range
-  // All of a part's loads are in flight together.
-  const size_t cells = static_cast<size_t>(p.M) * p.E, pitch = p.many ? p.M + p.E : cells;
-  const size_t at = static_cast<size_t>(t) * p.E + lane;
-  const float* sum = p.sums + (p.many ? p.M + lane : at);
-  float size[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) z[i] = 0.0, size[i] = 0.f, bias[i] = 0.0;
-#pragma unroll 1
-  for (int c = 0; c < p.parts; ++c) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 32 * i < p.E) {
-        z[i] += __ldcg(p.logits + c * cells + at + 32 * i);
-        size[i] += __ldcg(sum + c * pitch + 32 * i);
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (lane + 32 * i < p.E) {
-      if (p.choice_bias) bias[i] = static_cast<double>(__ldg(p.choice_bias + lane + 32 * i));
-      s = fmaxf(s, size[i]);
-      odd |= !p.weight_f32 && !isfinite(z[i]);
-    } else {
-      z[i] = -INFINITY;
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
-  if (p.many) {  // |x| |w| of the longest w
-    float x2 = 0.f;
-    for (int c = 0; c < p.parts; ++c) x2 += __ldcg(p.sums + static_cast<size_t>(c) * (p.M + p.E) + t);
-    s = sqrtf(x2) * sqrtf(s) * 1.001f;  // (the sums of squares are fp32)
-  }
-  const double loss = p.weight_f32 ? 0.0 : kRouteLoss * static_cast<double>(s);
-  int chosen = -1;     // lane j < top: the j-th choice,
-  double score = 0.0;  // its score
-#pragma unroll 1
-  for (int pass = 0;; ++pass) {
+  int chosen = 0;               // lane j < top: the j-th choice,
+  double score = 0.0;           // its score
+  unsigned long long mine = 0, rest = 0;  // and its key; the key after the last choice
+  auto choose = [&](bool first) {
     // Scores.  A NaN logit makes every softmax score NaN.
-    double v[PER];
     if (p.sigmoid) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) v[i] = 1.0 / (1.0 + exp(-z[i]));
@@ -190,8 +165,7 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
     }
     __syncwarp();
     // The k largest keys and the next one, equal ones by index.
-    unsigned long long mine = 0, rest = 0;  // lane j: the j-th key; the key after the last choice
-    const int want = p.weight_f32 != 0 || pass || p.top == p.E ? p.top : p.top + 1;
+    const int want = first && p.top < p.E ? p.top + 1 : p.top;
 #pragma unroll 1
     for (int j = 0; j < want; ++j) {
       unsigned long long best = key[0];
@@ -215,7 +189,44 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
         if (e == lane + 32 * i) key[i] = 0;
     }
     if (lane < p.top) score = q[chosen];
-    if (p.weight_f32 != 0 || pass) break;
+  };
+  unsigned again = 0;  // bit i: expert lane + 32 i has to be summed again
+  if (live) {
+    // All of a part's loads are in flight together.
+    const size_t cells = static_cast<size_t>(p.M) * p.E, pitch = p.many ? p.M + p.E : cells;
+    const size_t at = static_cast<size_t>(t) * p.E + lane;
+    const float* sum = p.sums + (p.many ? p.M + lane : at);
+    float size[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) z[i] = 0.0, size[i] = 0.f, bias[i] = 0.0;
+#pragma unroll 1
+    for (int c = 0; c < p.parts; ++c) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (lane + 32 * i < p.E) {
+          z[i] += __ldcg(p.logits + c * cells + at + 32 * i);
+          size[i] += __ldcg(sum + c * pitch + 32 * i);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (lane + 32 * i < p.E) {
+        if (p.choice_bias) bias[i] = static_cast<double>(__ldg(p.choice_bias + lane + 32 * i));
+        s = fmaxf(s, size[i]);
+        odd |= !p.weight_f32 && !isfinite(z[i]);
+      } else {
+        z[i] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+    if (p.many) {  // |x| |w| of the longest w
+      float x2 = 0.f;
+      for (int c = 0; c < p.parts; ++c) x2 += __ldcg(p.sums + static_cast<size_t>(c) * (p.M + p.E) + t);
+      s = sqrtf(x2) * sqrtf(s) * 1.001f;  // (the sums of squares are fp32)
+    }
+    const double loss = p.weight_f32 ? 0.0 : kRouteLoss * static_cast<double>(s);
+    choose(true);
     // Could the errors of two logits have swapped neighbours?  A score moves by at most its slope
     // times a logit's error: p (1 - p) for the sigmoid (a little more, for where p changes on the
     // way), 2 p with softmax's normaliser.
@@ -223,61 +234,82 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int t, int lan
     const unsigned long long after = __shfl_down_sync(0xffffffffu, mine, 1);
     const bool last = lane == p.top - 1 && p.top == p.E;
     const double here = unordered(mine);
-    const bool near = lane < p.top && !last && loss > 0.0 && here - unordered(lane == p.top - 1 ? rest : after) <= reach;
-    const unsigned nears = __ballot_sync(0xffffffffu, near);
+    const unsigned nears = __ballot_sync(
+        0xffffffffu, lane < p.top && !last && loss > 0.0 && here - unordered(lane == p.top - 1 ? rest : after) <= reach);
     const bool odds = __any_sync(0xffffffffu, odd);
-    if (!nears && !odds) break;
-    // Sums again in fp64, unless the token itself is not finite.
-    const long long xo = static_cast<long long>(t) * p.ldx;
-    bool finite = true;
+    if (nears || odds) {
+      // A token that is not finite itself keeps what the first sums gave.
+      bool finite = true;
 #pragma unroll 1
-    for (int k = odds ? 8 * lane : p.K; k < p.K; k += 256) {
-      const uint4 c = row_chunk(p.x, xo, k, p.K);
-      const uint32_t r[4] = {c.x, c.y, c.z, c.w};
+      for (int k = odds ? 8 * lane : p.K; k < p.K; k += 256) {
+        const uint4 c = row_chunk(p.x, static_cast<long long>(t) * p.ldx, k, p.K);
+        const uint32_t r[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) finite = finite && isfinite(unpack_lo<BF16>(r[i])) && isfinite(unpack_hi<BF16>(r[i]));
-    }
-    if (!__all_sync(0xffffffffu, finite)) break;
-    // Which: logits out of range, and experts whose key is as close to a chosen one's, or a chosen one
-    // whose neighbour is.  (Of two scores within reach of one another the chosen one's slope is the larger.)
-    unsigned again = 0;
+        for (int i = 0; i < 4; ++i) finite = finite && isfinite(unpack_lo<BF16>(r[i])) && isfinite(unpack_hi<BF16>(r[i]));
+      }
+      if (__all_sync(0xffffffffu, finite)) {
+        // Logits out of range, and experts whose key is as close to a chosen one's, or a chosen one whose
+        // neighbour is.  (Of two scores within reach of one another the chosen one's slope is the larger.)
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 32 * i < p.E && !isfinite(z[i])) again |= 1u << i;
+        for (int i = 0; i < PER; ++i)
+          if (lane + 32 * i < p.E && !isfinite(z[i])) again |= 1u << i;
 #pragma unroll 1
-    for (int j = 0; j < p.top; ++j) {
-      const double kj = __shfl_sync(0xffffffffu, here, j), rj = __shfl_sync(0xffffffffu, reach, j);
-      const int cj = __shfl_sync(0xffffffffu, chosen, j);
-      const bool nj = (nears >> j | (j ? nears >> (j - 1) : 0u)) & 1u;
+        for (int j = 0; j < p.top; ++j) {
+          const double kj = __shfl_sync(0xffffffffu, here, j), rj = __shfl_sync(0xffffffffu, reach, j);
+          const int cj = __shfl_sync(0xffffffffu, chosen, j);
+          const bool nj = (nears >> j | (j ? nears >> (j - 1) : 0u)) & 1u;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int e = lane + 32 * i;
-        if (e < p.E && (e == cj ? nj : fabs(v[i] + bias[i] - kj) <= rj)) again |= 1u << i;
+          for (int i = 0; i < PER; ++i) {
+            const int e = lane + 32 * i;
+            if (e < p.E && (e == cj ? nj : loss > 0.0 && fabs(v[i] + bias[i] - kj) <= rj)) again |= 1u << i;
+          }
+        }
       }
     }
-#pragma unroll 1
-    for (unsigned todo = __ballot_sync(0xffffffffu, again != 0); todo; todo = __ballot_sync(0xffffffffu, again != 0)) {
-      const int src = __ffs(todo) - 1;
-      const int i = __ffs(__shfl_sync(0xffffffffu, again, src)) - 1;
-      const long long wo = static_cast<long long>(src + 32 * i) * p.ldw;
-      double a = 0.0, b = 0.0;
-#pragma unroll 2
-      for (int k = 8 * lane; k < p.K; k += 512) {  // (rolled: this code is fetched for a token in hundreds)
-        const uint4 xa = row_chunk(p.x, xo, k, p.K), wa = row_chunk(p.w, wo, k, p.K);
-        const uint4 xb = row_chunk(p.x, xo, k + 256, p.K), wb = row_chunk(p.w, wo, k + 256, p.K);
-        a = dot8<BF16>(xa, wa, a);
-        b = dot8<BF16>(xb, wb, b);
-      }
-      a = warp_sum(a + b);
-      if (lane == src) {
-#pragma unroll
-        for (int c = 0; c < PER; ++c)
-          if (c == i) z[c] = a;
-        again &= again - 1;
-      }
-    }
-    __syncwarp();  // (q is written again)
   }
+  // Sums again in fp64, a few of every warp's at a time, by all warps.
+  bool changed = false;
+#pragma unroll 1
+  while (__syncthreads_or(again != 0)) {
+    int asked[kAgainSlots];
+#pragma unroll
+    for (int c = 0; c < kAgainSlots; ++c) {
+      const unsigned who = __ballot_sync(0xffffffffu, again != 0);
+      const int src = __ffs(who) - 1;
+      asked[c] = who ? src + 32 * (__ffs(__shfl_sync(0xffffffffu, again, max(src, 0))) - 1) : -1;
+      if (lane == src) again &= again - 1;
+      if (lane == 0) slots[warp * kAgainSlots + c] = asked[c];
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int first = 0; first < WARPS * kAgainSlots; first += 32)
+#pragma unroll 1
+      for (unsigned todo = __ballot_sync(0xffffffffu, slots[first + lane] >= 0); todo; todo &= todo - 1) {
+        const int i = first + __ffs(todo) - 1;
+        const long long xo = static_cast<long long>(t - warp + i / kAgainSlots) * p.ldx;
+        const long long wo = static_cast<long long>(slots[i]) * p.ldw;
+        double a = 0.0;
+#pragma unroll 2
+        for (int k = 8 * threadIdx.x; k < p.K; k += 256 * WARPS)
+          a = dot8<BF16>(row_chunk(p.x, xo, k, p.K), row_chunk(p.w, wo, k, p.K), a);
+        a = warp_sum(a);
+        if (lane == 0) part[i * WARPS + warp] = a;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kAgainSlots; ++c)
+      if (asked[c] >= 0) {
+        changed = true;
+        double a = 0.0;
+#pragma unroll 1
+        for (int w = 0; w < WARPS; ++w) a += part[(warp * kAgainSlots + c) * WARPS + w];
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (asked[c] == lane + 32 * i) z[i] = a;
+      }
+  }
+  if (!live) return;
+  if (changed) choose(false);
   const double total = warp_sum(lane < p.top ? score : 0.0);
   if (lane < p.top) {
     ids[lane] = chosen;
@@ -396,7 +428,7 @@ template <bool BF16, bool W32, int MT, int NT, int PER>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   const int t0 = blockIdx.y * 16 * MT;
   if (threadIdx.x == 0) grid_dep_launch();
   grid_dep_wait();
@@ -409,11 +441,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   }
   __syncthreads();
   if (!last) return;
-  double* q_of = reinterpret_cast<double*>(smem) + warp * p.E;  // (the parts have been added up)
 #pragma unroll 1
-  for (int t = t0 + warp; t < min(t0 + 16 * MT, p.M); t += kRouteWarps) {
-    route_token<BF16, PER>(p, t, lane, q_of);
-    __syncwarp();
+  for (int t = t0; t < min(t0 + 16 * MT, p.M); t += kRouteWarps) {  // (the parts have been added up)
+    route_tokens<BF16, PER, kRouteWarps>(p, t + warp, smem);
+    __syncthreads();
   }
 }
 
@@ -548,11 +579,9 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
 template <bool BF16, int PER>
 __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) grid_dep_launch();
   grid_dep_wait();
-  const int t = blockIdx.x * kRouteWarps + warp;
-  if (t < p.M) route_token<BF16, PER>(p, t, lane, reinterpret_cast<double*>(smem) + warp * p.E);
+  route_tokens<BF16, PER, kRouteWarps>(p, blockIdx.x * kRouteWarps + (threadIdx.x >> 5), smem);
 }
 
 }  // namespace ffnb200

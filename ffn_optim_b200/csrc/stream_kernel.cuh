@@ -302,13 +302,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         }
         __syncthreads();
         if (*last_flag) {
+          constexpr int kWarps = kStreamThreads / 32;
+          static_assert(kWarps == 16, "a warp per token of a tile");
           const int t = tile * 16 + warp;
-          double* q = reinterpret_cast<double*>(gbase) + warp * p.experts;
-          if (t < p.tokens) {
-            if (p.experts <= 64) route_token<BF16, 2>(r, t, lane, q);
-            else if (p.experts <= 256) route_token<BF16, 8>(r, t, lane, q);
-            else route_token<BF16, 16>(r, t, lane, q);
-          }
+          if (p.experts <= 64) route_tokens<BF16, 2, kWarps>(r, t, gbase);
+          else if (p.experts <= 256) route_tokens<BF16, 8, kWarps>(r, t, gbase);
+          else route_tokens<BF16, 16, kWarps>(r, t, gbase);
           __syncthreads();
           if (threadIdx.x == 0) red_release_add(r.counters + tiles, 1u);
         }
