@@ -552,9 +552,12 @@ int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* pr, ffn_b200_moe_plan* ou
   std::memset(out, 0, sizeof(*out));
   const int grid = pr->block_num ? pr->block_num : sms;
   const int tokens = static_cast<int>(pr->m);
-  const ffnb200::StreamLists lists(tokens, pr->experts, pr->top_k);
   out->block_num = grid;
-  out->chunk = stream_chunk(pr->m);
+  // Tokens of one item: twice an expert's even share, so that few experts need a second item (and their
+  // weights a second trip) while the ring keeps its room for weights (64 tokens, 6 of 64 experts:
+  // ring slots of 64 token rows held 128 KB of weights, of 16 hold 160 KB).
+  out->chunk = stream_chunk(std::min<int64_t>(pr->m, 2 * cdiv(pr->m * pr->top_k, pr->experts)));
+  const ffnb200::StreamLists lists(tokens, pr->experts, pr->top_k, out->chunk);
   const StreamRing ring(ffnb200::kABytes, out->chunk, lists.bytes);
   out->stages = ring.stages;
   out->smem_bytes = ring.smem;
@@ -562,7 +565,7 @@ int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* pr, ffn_b200_moe_plan* ou
   out->hidden_pitch = pitch_of(pr->h);
   out->sorted_pitch = pr->m > kMoeGather ? pitch_of(pr->k) : 0;
   const int64_t slots = 2ll * grid * out->chunk * 128;
-  const int64_t items = ffnb200::StreamLists::stream_items(tokens, pr->experts, pr->top_k);
+  const int64_t items = ffnb200::StreamLists::most_items(tokens, pr->experts, pr->top_k, out->chunk);
   const int64_t down = cdiv(pr->n, 128);
   if (items * down * cdiv(pr->h, 64) >= (int64_t(1) << 31)) return FFN_B200_ERR_TOO_LARGE;
   out->workspace_floats = slots + out->hidden_rows * down * 128;
@@ -627,7 +630,7 @@ int ffn_b200_moe_prepare(const ffn_b200_moe_problem* pr, const ffn_b200_moe_buff
   P.steps2 = static_cast<int>(cdiv(pr->h, 64));
   P.feat2 = static_cast<int>(pr->n);
   P.chunk = plan.chunk;
-  const StreamRing ring(P.slab, P.chunk, ffnb200::StreamLists(P.tokens, pr->experts, pr->top_k).bytes);
+  const StreamRing ring(P.slab, P.chunk, ffnb200::StreamLists(P.tokens, pr->experts, pr->top_k, P.chunk).bytes);
   P.blocks = ring.blocks;
   P.stages = ring.stages;
   P.act = pr->activation;

@@ -85,20 +85,20 @@ constexpr int kStreamSync = 3;  // CTAs done with the second product; CTAs leavi
 struct StreamLists {
   int words;          // u32 words of an expert's token set
   int sets, first, offset, item, token, bytes;  // byte offsets
-  __host__ __device__ StreamLists(int tokens, int experts, int top) {
+  __host__ __device__ StreamLists(int tokens, int experts, int top, int chunk) {
     words = (tokens + 31) / 32;
     const int pairs = tokens * top;
     sets = 0;
     offset = sets + experts * words * 4;      // u16 [E + 1]: pairs before expert e
     first = offset + (experts + 1) * 2;       // u16 [E + 1]: items before expert e
     item = (first + (experts + 1) * 2 + 7) & ~7;  // uint2 per item: expert | count << 16, first pair
-    token = item + 8 * stream_items(tokens, experts, top);  // u16 per pair: its token
+    token = item + 8 * most_items(tokens, experts, top, chunk);  // u16 per pair: its token
     bytes = (token + pairs * 2 + 15) & ~15;
   }
-  // Items at most: one per chosen expert, and one more for each full 128 pairs.
-  __host__ __device__ static int stream_items(int tokens, int experts, int top) {
+  // Items at most: one per chosen expert, and one more for each full chunk of pairs.
+  __host__ __device__ static int most_items(int tokens, int experts, int top, int chunk) {
     const int pairs = tokens * top;
-    return (experts < pairs ? experts : pairs) + pairs / 128;
+    return (experts < pairs ? experts : pairs) + pairs / chunk;
   }
 };
 
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   int* n_items = reinterpret_cast<int*>(tmem_slot + 3);
   int* n_pairs = n_items + 1;
   int* warp_sums = n_items + 2;  // [16] x 2
-  const StreamLists lists(p.tokens, MOE ? p.experts : 0, MOE ? p.top : 0);
+  const StreamLists lists(p.tokens, MOE ? p.experts : 0, MOE ? p.top : 0, p.chunk);
   uint8_t* lbase = ctrl + kStreamBarBytes;
   unsigned* sets = reinterpret_cast<unsigned*>(lbase + lists.sets);
   uint16_t* offset = reinterpret_cast<uint16_t*>(lbase + lists.offset);

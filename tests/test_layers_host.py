@@ -142,7 +142,7 @@ def test_moe_plans(lib):
                 prob = _lib.MoeProblem(m, 4096, 1000, 2048, e, top, 1, act, 0, 148)
                 assert lib.ffn_b200_moe_make_plan(ctypes.byref(prob), ctypes.byref(plan)) == _lib.OK
                 assert plan.smem_bytes <= 232448 and plan.stages >= 2 and plan.block_num == 148
-                assert min(m, 128) <= plan.chunk <= 128 and plan.hidden_rows == m * top and plan.hidden_pitch == 1000
+                assert min(m, 16) <= plan.chunk <= 128 and plan.hidden_rows == m * top and plan.hidden_pitch == 1000
                 assert plan.sorted_pitch in (0, 4096)
 
 
