@@ -5,6 +5,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <mutex>
@@ -108,7 +109,8 @@ constexpr int kMaxSmem = 232448;
 // the pairs' order first.
 constexpr int64_t kMoeGather = 16;
 
-int stream_chunk(int64_t tokens) { return tokens <= 16 ? 16 : (tokens <= 32 ? 32 : (tokens <= 64 ? 64 : 128)); }
+// Token columns of a tile: a multiple of the MMA's 16, at most 128.
+int stream_chunk(int64_t tokens) { return static_cast<int>(std::min<int64_t>(128, cdiv(tokens, 16) * 16)); }
 // The ring beside `list_bytes` of lists: K steps per slot (of `slab` weight bytes and `chunk` token
 // rows each; about 32 KB, at most 4 steps), slots, and the dynamic shared memory they add up to.
 // (The MMA reads 128 rows from a slab's start.)
@@ -553,10 +555,11 @@ int ffn_b200_moe_make_plan(const ffn_b200_moe_problem* pr, ffn_b200_moe_plan* ou
   const int grid = pr->block_num ? pr->block_num : sms;
   const int tokens = static_cast<int>(pr->m);
   out->block_num = grid;
-  // Tokens of one item: twice an expert's even share, so that few experts need a second item (and their
-  // weights a second trip) while the ring keeps its room for weights (64 tokens, 6 of 64 experts:
-  // ring slots of 64 token rows held 128 KB of weights, of 16 hold 160 KB).
-  out->chunk = stream_chunk(std::min<int64_t>(pr->m, 2 * cdiv(pr->m * pr->top_k, pr->experts)));
+  // Tokens of one item: an expert's even share and three times its spread, so that few experts need a
+  // second item (and their weights a second trip) while the ring keeps its room for weights (64
+  // tokens, 6 of 64 experts: 168 us with slots of 64 token rows, 150 us with 16).
+  const double share = static_cast<double>(pr->m) * pr->top_k / pr->experts;
+  out->chunk = stream_chunk(std::min<int64_t>(pr->m, static_cast<int64_t>(std::ceil(share + 3.0 * std::sqrt(share)))));
   const ffnb200::StreamLists lists(tokens, pr->experts, pr->top_k, out->chunk);
   const StreamRing ring(ffnb200::kABytes, out->chunk, lists.bytes);
   out->stages = ring.stages;

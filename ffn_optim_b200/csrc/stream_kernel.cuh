@@ -53,7 +53,7 @@ struct StreamParams {
   int steps1, feat1;         // K steps; output features
   int tiles2, steps2, feat2; // second product (experts)
   int slab;                  // bytes of a step's weights in a ring slot (a multiple of 1024)
-  int chunk;                 // tokens per item at most (16, 32, 64 or 128)
+  int chunk;                 // tokens per item at most (a multiple of 16 up to 128)
   int blocks, stages;        // K steps per ring slot; ring slots
   int act;                   // ffn_b200_gelu
   const uint16_t* bias;      // projection, optional [N]
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   const int lane = threadIdx.x & 31;
   const int c = blockIdx.x;
   const int C = gridDim.x;
-  const uint32_t tmem_cols = p.chunk <= 16 ? 32u : 2u * static_cast<uint32_t>(p.chunk);
+  const uint32_t tmem_cols = p.chunk <= 16 ? 32u : (p.chunk <= 32 ? 64u : (p.chunk <= 64 ? 128u : 256u));  // two accumulators
 
   if (threadIdx.x == 0) {
 #pragma unroll 1
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         const bool gathered = MOE && ph == 0 && !p.sorted;
         // Boxes of 64 rows, of 8 for a remainder of up to 24.  (Rows behind the item's last belong to
         // columns nobody reads.)
-        const int wide = p.chunk < 64 ? 0 : (count % 64 > 24 ? (count + 63) / 64 : count / 64);
+        const int wide = count / 64 + (count % 64 > 24 && (count / 64 + 1) * 64 <= p.chunk ? 1 : 0);
         const int narrow = max(0, count - wide * 64 + 7) / 8;
         const uint32_t bytes =
             !MOE ? token_bytes : (gathered ? (count + 3) / 4 * 512u : static_cast<uint32_t>(wide) * 8192u + narrow * 1024u);
@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     // Dealt out over the CTAs, a warp taking 512 bytes of a row at a time.  The weights, already on
     // their way, hide the grid-wide wait for them.
     const int vecs = static_cast<int>(p.lds / 8), strips = (vecs + 31) / 32;
-#pragma unroll 2
+#pragma unroll 4
     for (int i = (warp - 8) * C + c; i < *n_pairs * strips; i += C * (kStreamThreads / 32 - 8)) {
       const int pair = i / strips, v = (i - pair * strips) * 32 + lane;
       if (v < vecs)
