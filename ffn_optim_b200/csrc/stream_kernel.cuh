@@ -377,11 +377,16 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       expert = 0, start = 0, count = p.tokens;
     }
   };
-  // Experts, first product: C / items CTAs per item where no CTA gets more groups by that than by an
-  // even deal (one token, 6 of 64 experts: ends 6 us earlier, as no CTA is left with two short tiles).
+  // Experts, first product: C / items CTAs per item, or an even deal of all groups, whichever leaves the
+  // busiest CTA less to load: its groups (2 KB a step) and, for every tile, the tokens (`chunk` rows
+  // of 128 bytes a step); by an even deal a CTA that crosses from one item to the next has a tile
+  // more.  (One token, 6 of 64 experts: CTAs per item end 6 us earlier; 64 tokens: 12 us later.)
   const int per_item = max(1, MOE && items ? C / items : 1);
+  const int most_whole = (p.groups1 + per_item - 1) / per_item, most_even = (items * p.groups1 + C - 1) / C;
+  const int row_cost = (p.chunk + 15) / 16;
   const bool whole_items = items > 0 && items <= C &&
-                           (p.groups1 + per_item - 1) / per_item <= (items * p.groups1 + C - 1) / C;
+                           most_whole + row_cost * ((most_whole + p.unit_groups - 1) / p.unit_groups) <=
+                               most_even + row_cost * ((most_even + p.unit_groups - 1) / p.unit_groups + 1);
   // This CTA's tiles, in the same order for every role: tile(ph, item, g0, groups, k0, k1) returns
   // false to stop.  First product: groups [g0, g0 + groups) of the item over all of K.  Second:
   // tile g0, K steps [k0, k1).
@@ -699,43 +704,46 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     const int n_units = p.tokens * p.tiles2;
     // Lane j < top knows choice j: its weight, its pieces and where the first one lies; every lane
     // its four features of the residual.
-    const float* src = nullptr;
-    int pieces = 0, t = 0, f0 = 0;
-    float wt = 0.f;
-    uint2 res = make_uint2(0u, 0u);
+    struct Share {
+      const float* src;
+      int pieces, t, f0;
+      float wt;
+      uint2 res;
+    };
     auto look_up = [&](int unit) {
-      t = unit / p.tiles2;
-      const int tile = unit - t * p.tiles2;
-      f0 = tile * kBM + 4 * lane;
+      Share u{nullptr, 0, unit / p.tiles2, 0, 0.f, make_uint2(0u, 0u)};
+      if (unit >= n_units) return u;
+      const int t = u.t, tile = unit - t * p.tiles2;
+      u.f0 = tile * kBM + 4 * lane;
       if (p.residual) {  // (rows are 16-byte aligned and padded to 8 elements: four at a time stay inside)
-        const uint16_t* r = p.residual + static_cast<long long>(t) * p.ldr + f0;
-        if (f0 + 4 <= p.feat2) {
-          res = __ldg(reinterpret_cast<const uint2*>(r));
+        const uint16_t* r = p.residual + static_cast<long long>(t) * p.ldr + u.f0;
+        if (u.f0 + 4 <= p.feat2) {
+          u.res = __ldg(reinterpret_cast<const uint2*>(r));
         } else {
-          res = make_uint2(0u, 0u);
-          for (int q = 0; f0 + q < p.feat2; ++q) (q < 2 ? res.x : res.y) |= static_cast<uint32_t>(__ldg(r + q)) << (16 * (q & 1));
+          for (int q = 0; u.f0 + q < p.feat2; ++q)
+            (q < 2 ? u.res.x : u.res.y) |= static_cast<uint32_t>(__ldg(r + q)) << (16 * (q & 1));
         }
       }
-      pieces = 0;
       if (lane < p.top) {
         const int e = __ldcg(p.ids + t * p.top + lane);
         if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts)) {
-          wt = __ldcg(p.weights + t * p.top + lane);
+          u.wt = __ldcg(p.weights + t * p.top + lane);
           int rank = 0;
           for (int w = 0; w < (t >> 5); ++w) rank += __popc(sets[e * lists.words + w]);
           rank += __popc(sets[e * lists.words + (t >> 5)] & ((1u << (t & 31)) - 1u));
           const int chunk_of = rank / p.chunk;
           const int s = ((first[e] + chunk_of) * p.tiles2 + tile) * p.steps2;
           const int c_first = line.cta_of(s);
-          pieces = line.cta_of(s + p.steps2 - 1) - c_first + 1;
-          src = pieces == 1 ? p.whole + static_cast<size_t>(offset[e] + rank) * pitch + static_cast<size_t>(tile) * kBM
-                            : p.pieces + (2 * static_cast<size_t>(c_first) + 1) * slot +
-                                  static_cast<size_t>(rank - chunk_of * p.chunk) * kBM;
+          u.pieces = line.cta_of(s + p.steps2 - 1) - c_first + 1;
+          u.src = u.pieces == 1
+                      ? p.whole + static_cast<size_t>(offset[e] + rank) * pitch + static_cast<size_t>(tile) * kBM
+                      : p.pieces + (2 * static_cast<size_t>(c_first) + 1) * slot + static_cast<size_t>(rank - chunk_of * p.chunk) * kBM;
         }
       }
+      return u;
     };
     int unit = warp * C + c;
-    if (unit < n_units) look_up(unit);
+    Share now = look_up(unit);
     if (threadIdx.x == 0) {
       red_release_add(sync_words, 1u);  // (covers the whole CTA's sums: the barrier above)
       if (!*abort_flag) stream_wait_word(sync_words, static_cast<unsigned>(C), abort_flag, p, 3, -1);
@@ -743,10 +751,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     __syncthreads();
     if (!*abort_flag) {
 #pragma unroll 1
-      while (unit < n_units) {
-        // Four experts' first two pieces in flight at a time.  (Piece q > 0 of a cut tile lies in
-        // the first slot of CTA c_first + q: 2 q - 1 slots behind piece 0.)
+      for (; unit < n_units; unit += C * (kStreamThreads / 32)) {
+        // Four experts' first two pieces in flight at a time, and the next unit's look-up under the
+        // first four.  (Piece q > 0 of a cut tile lies in the first slot of CTA c_first + q: 2 q - 1
+        // slots behind piece 0.)
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        Share next{};
 #pragma unroll 1
         for (int j0 = 0; j0 < p.top; j0 += 4) {
           float4 z[4], z1[4];
@@ -755,15 +765,16 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = (j0 + i) & 31;  // (lanes from `top` on bring no pieces)
-            n[i] = __shfl_sync(0xffffffffu, pieces, j);
+            n[i] = __shfl_sync(0xffffffffu, now.pieces, j);
             at[i] = reinterpret_cast<const float4*>(
-                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j)) + lane;
+                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(now.src), j)) + lane;
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             z[i] = n[i] > 0 ? __ldcg(at[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
             z1[i] = n[i] > 1 ? __ldcg(at[i] + slot / 4) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
+          if (j0 == 0) next = look_up(unit + C * (kStreamThreads / 32));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             z[i].x += z1[i].x, z[i].y += z1[i].y, z[i].z += z1[i].z, z[i].w += z1[i].w;
@@ -772,7 +783,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
               const float4 v = __ldcg(at[i] + static_cast<size_t>(2 * q - 1) * (slot / 4));
               z[i].x += v.x, z[i].y += v.y, z[i].z += v.z, z[i].w += v.w;
             }
-            const float wj = __shfl_sync(0xffffffffu, wt, (j0 + i) & 31);
+            const float wj = __shfl_sync(0xffffffffu, now.wt, (j0 + i) & 31);
             if (n[i] > 0) {
               sum.x = fmaf(wj, z[i].x, sum.x), sum.y = fmaf(wj, z[i].y, sum.y);
               sum.z = fmaf(wj, z[i].z, sum.z), sum.w = fmaf(wj, z[i].w, sum.w);
@@ -780,19 +791,18 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
           }
         }
         if (p.residual) {
-          sum.x += unpack_lo<BF16>(res.x), sum.y += unpack_hi<BF16>(res.x);
-          sum.z += unpack_lo<BF16>(res.y), sum.w += unpack_hi<BF16>(res.y);
+          sum.x += unpack_lo<BF16>(now.res.x), sum.y += unpack_hi<BF16>(now.res.x);
+          sum.z += unpack_lo<BF16>(now.res.y), sum.w += unpack_hi<BF16>(now.res.y);
         }
-        uint16_t* y = p.y + static_cast<long long>(t) * p.ldy + f0;
+        uint16_t* y = p.y + static_cast<long long>(now.t) * p.ldy + now.f0;
         const uint2 out = make_uint2(pack2<BF16>(sum.x, sum.y), pack2<BF16>(sum.z, sum.w));
-        if (f0 + 4 <= p.feat2) {
+        if (now.f0 + 4 <= p.feat2) {
           *reinterpret_cast<uint2*>(y) = out;
         } else {
-          for (int q = 0; f0 + q < p.feat2; ++q)
+          for (int q = 0; now.f0 + q < p.feat2; ++q)
             y[q] = static_cast<uint16_t>((q < 2 ? out.x : out.y) >> (16 * (q & 1)));
         }
-        unit += C * (kStreamThreads / 32);
-        if (unit < n_units) look_up(unit);
+        now = next;
       }
     }
     // The last CTA to leave clears the counters for the next launch.

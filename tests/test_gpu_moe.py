@@ -180,6 +180,50 @@ def test_layer_options(m, act, gelu, residual):
         assert (y[~mask] == 0).all()
 
 
+@pytest.mark.parametrize("m,k,e,top", [(1, 2048, 64, 6), (1, 136, 512, 32), (16, 4096, 32, 4), (40, 1000, 300, 7),
+                                       (100, 264, 512, 32), (256, 512, 200, 8), (256, 64, 1, 1), (33, 31, 65, 65 // 3)])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_layer_routes_as_the_router(m, k, e, top, f32, scoring):
+    """The layer chooses within its own launch, the router in one of its own: both as defined."""
+    g = gen(m + k + e)
+    x, wr = normal(g, m, k), normal(g, e, k, scale=k ** -0.5, dtype=torch.float32 if f32 else BF)
+    w1, w2 = normal(g, e, 32, k, scale=k ** -0.5), normal(g, e, 40, 32, scale=32 ** -0.5)
+    mask = torch.rand(m, generator=g, device="cuda") > 0.2
+    bias = normal(g, e, scale=0.02, dtype=torch.float32)
+    for kw in (dict(top_k=top, scoring=scoring), dict(top_k=top, scoring=scoring, choice_bias=bias, mask=mask, scale=3.0)):
+        layer = prepare_moe_ffn(x, wr, w1, w2, activation="silu", **kw)
+        for _ in range(2):
+            y = layer.run()
+            layer.check()
+            check_route((layer.ids, layer.weights), x, wr, **kw)
+            check_moe(y, x, layer.ids, layer.weights, w1, w2, "silu", "erf", None)
+        ids, _ = route_experts(x, wr, **kw)
+        assert torch.equal(ids, layer.ids)
+
+
+def test_layer_routing_ties_nan_and_close_logits():
+    """As the router's tests of these, through the layer's launch; a token of NaN stays by itself."""
+    g = gen(21)
+    m, k, e = 30, 512, 64
+    x, wr = normal(g, m, k), normal(g, 8, k, scale=0.05).repeat(8, 1)  # every logit eight times
+    w1, w2 = normal(g, e, 24, k, scale=k ** -0.5), normal(g, e, 32, 24, scale=0.2)
+    close = normal(g, 8, k, scale=0.05, dtype=torch.float32).repeat_interleave(8, 0)
+    close += normal(g, e, k, scale=1e-9, dtype=torch.float32)
+    for w in (wr, close):
+        layer = prepare_moe_ffn(x, w, w1, w2, activation="silu", top_k=9)
+        y = layer.run().clone()
+        layer.check()
+        check_route((layer.ids, layer.weights), x, w, top_k=9)
+        bad = x.clone()
+        bad[3] = float("nan")
+        got = layer.run(bad)
+        layer.check()
+        assert torch.equal(layer.ids[3], torch.arange(9, dtype=torch.int32, device="cuda")) and layer.weights[3].isnan().all()
+        keep = torch.arange(m, device="cuda") != 3
+        assert torch.equal(got[keep], y[keep]) and got[3].isnan().all()
+
+
 @pytest.mark.parametrize("m", [5, 256])
 def test_masked_tokens_do_not_matter(m):
     """NaN in masked rows reaches nothing; with every token masked the layer is its residual."""
@@ -325,9 +369,10 @@ def test_block_of_operators(m):
     z = ffn(y, f1, f2)
     assert z.shape == (m, d) and torch.isfinite(z).all()
     ids, wt = route_experts(hidden, wr, top_k=2)
-    assert torch.equal(ids, layer.ids) and torch.equal(wt, layer.weights)
+    assert torch.equal(ids, layer.ids)
+    check_route((ids, wt), hidden, wr, top_k=2)  # (the weights may differ in the last bit: another split of K)
     first = y.clone()
-    assert torch.equal(layer.run_routed(ids, wt), first)
+    assert torch.equal(layer.run_routed(layer.ids.clone(), layer.weights.clone()), first)
     g1, g2 = out.capture_graph(), layer.capture_graph()
     for _ in range(3):
         g1.replay()
