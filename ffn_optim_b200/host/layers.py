@@ -173,9 +173,12 @@ class PreparedLayer:
         with torch.cuda.device(device):
             self.stream = torch.cuda.current_stream()
         self._stream_ptr = self.stream.cuda_stream
+        # (the raw handle, as launchers read it: a Stream object costs a microsecond per run)
+        self._current = getattr(torch._C, "_cuda_getCurrentRawStream",
+                                lambda index: torch.cuda.current_stream(index).cuda_stream)
 
     def _check_stream(self):
-        if self._torch.cuda.current_stream(self._index).cuda_stream != self._stream_ptr:
+        if self._current(self._index) != self._stream_ptr:
             raise RuntimeError(f"{type(self).__name__} must run on its preparation stream; "
                                "concurrent reuse is unsupported")
 
