@@ -112,14 +112,17 @@ constexpr int64_t kMoeGather = 16;
 // Token columns of a tile: a multiple of the MMA's 16, at most 128.
 int stream_chunk(int64_t tokens) { return static_cast<int>(std::min<int64_t>(128, cdiv(tokens, 16) * 16)); }
 // The ring beside `list_bytes` of lists: K steps per slot (of `slab` weight bytes and `chunk` token
-// rows each; about 32 KB, at most 4 steps), slots, and the dynamic shared memory they add up to.
+// rows each), slots, and the dynamic shared memory they add up to.  Up to 60 KB and 8 steps: longer
+// stretches of each weight row at a time and fewer waits, against fewer slots (1x4096x4096: 15.9 us
+// with 2 steps, 11.3 with 4, 9.9 with 8, 10.2 with 12; 16 tokens, 4 of 32 experts: 229 us with 2,
+// 226 with 3, 225 with 4).
 // (The MMA reads 128 rows from a slab's start.)
 struct StreamRing {
   int blocks, stages;
   int64_t smem;
   StreamRing(int slab, int chunk, int list_bytes) {
     const int step = slab + chunk * 128;
-    blocks = std::max(1, std::min(4, 36864 / step));
+    blocks = std::max(1, std::min(8, 61440 / step));
     const int fixed = 1024 + ffnb200::kStreamBarBytes + list_bytes +
                       std::max(0, ffnb200::kABytes - slab - blocks * chunk * 128);
     stages = std::min(ffnb200::kStreamMaxStages, (kMaxSmem - fixed) / (blocks * step));

@@ -138,6 +138,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d_hint(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, int c3,
+                                                 uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "l"(policy)
+      : "memory");
+}
 // One lane of a converged warp, as the compiler knows a single one.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -431,6 +439,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       uint32_t phase = 0;
       long long issued = 0;
       const uint32_t box_bytes = static_cast<uint32_t>(p.group_rows) * 128u;
+      // Experts' weights leave L2 first: another call chooses others (229 -> 225 us for 16 tokens, 4 of 32
+      // experts).  A projection's may stay until its next call (11.5 us with the hint, 11.3 without).
+      const uint64_t policy = policy_evict_first();
       for_tiles([&](int ph, int it, int g0, int n, int k0, int k1) {
         int expert, start, count;
         item_of(it, expert, start, count);
@@ -444,7 +455,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
 #pragma unroll 1
           for (int i = 0; i < nb; ++i) {
             if (MOE && ph) {
-              tma_load_4d(dst + i * slab, &p.tm_w2, (kb + i) * kBK, g0 * kBM, 0, expert, full_bar(stage));
+              tma_load_4d_hint(dst + i * slab, &p.tm_w2, (kb + i) * kBK, g0 * kBM, 0, expert, full_bar(stage), policy);
+            } else if (MOE) {
+#pragma unroll 1
+              for (int j = 0; j < n; ++j)
+                tma_load_4d_hint(dst + i * slab + j * box_bytes, &p.tm_w1, (kb + i) * kBK, (g0 + j) * p.group_feats, 0, expert,
+                                 full_bar(stage), policy);
             } else {
 #pragma unroll 1
               for (int j = 0; j < n; ++j)
