@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   }
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&p.tm_w1);
-    prefetch_tmap(&p.tm_x);
+    prefetch_tmap(MOE && p.sorted ? &p.tm_x8 : &p.tm_x);
     if (MOE) {
       prefetch_tmap(&p.tm_w2);
       prefetch_tmap(&p.tm_h8);

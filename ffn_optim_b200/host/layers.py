@@ -164,6 +164,8 @@ class PreparedLayer:
     """What the prepared operators share: the preparation stream, the kernel's status and graph
     capture (``_capture(stream_pointer)`` of the subclass launches once on the prepared inputs)."""
 
+    _status = None  # the kernel's status words, if it has waits that can fail
+
     def _open(self, device):
         import torch
 
@@ -185,7 +187,7 @@ class PreparedLayer:
     def status(self):
         """Synchronises the stream and returns the kernel's status words [code, cta, aux, 0]."""
         self.stream.synchronize()
-        return [int(v) for v in self._status.tolist()]
+        return [0, 0, 0, 0] if self._status is None else [int(v) for v in self._status.tolist()]
 
     def check(self):
         """Raises RuntimeError if a launch since the last reset reported a device error."""
@@ -202,7 +204,7 @@ class PreparedLayer:
         """Clears the kernel's counters and status."""
         from .. import _lib
 
-        rc = self._reset(self._stream_ptr)
+        rc = _lib.OK if self._status is None else self._reset(self._stream_ptr)
         if rc != _lib.OK:
             raise RuntimeError(f"{type(self).__name__}.reset: {_lib.strerror(rc)}")
 

@@ -122,6 +122,8 @@ def test_router_repeats_graph_and_masks():
         buf.copy_(x)
         graph.replay()
         assert torch.equal(p._ids, ids) and torch.equal(p._weights, wt)
+    assert p.status() == [0, 0, 0, 0] and p.check()
+    p.reset()
     none = torch.zeros(50, dtype=torch.bool, device="cuda")
     ids, wt = p.run(xs[1], mask=none)
     assert (ids == -1).all() and (wt == 0).all()
