@@ -361,7 +361,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     int tm, tn;
     coords(owner, tm, tn);
     int ok = 1;
+    uint32_t r[4];  // the next 8 columns' residual, asked for before anything is waited for
+    auto read_ahead = [&](int c0) {
+      if (p.residual && c0 < share)
+        load_row<8>(r, p.residual, p.ldr, tm * kBM + row, p.M, tn * BN + static_cast<int>(rank) * share + c0, p.N);
+    };
     if (warp >= 4) {
+      read_ahead(8 * half);
       if (lane == 0) ok = gemm_wait(tfull_bar(0), 0, abort_flag, p, 400) ? 1 : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       tc_fence_after();
@@ -405,15 +411,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
           }
         }
-        if (grow >= p.M || col >= p.N || *abort_flag) continue;
-        if (p.bias) add_bias<BF16, 8>(v, p.bias, col, p.N);
+        const bool write = grow < p.M && col < p.N && !*abort_flag;
+        if (write && p.bias) add_bias<BF16, 8>(v, p.bias, col, p.N);
         apply_act<8>(v, p.act);
         if (p.residual) {
-          uint32_t r[4];
-          load_row<8>(r, p.residual, p.ldr, grow, p.M, col, p.N);
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[2 * j] += unpack_lo<BF16>(r[j]), v[2 * j + 1] += unpack_hi<BF16>(r[j]);
+          read_ahead(c0 + 16);
         }
+        if (!write) continue;
         store_row<BF16, 8>(p.y + static_cast<long long>(grow) * p.ldy + col, v, p.N - col);
       }
     }

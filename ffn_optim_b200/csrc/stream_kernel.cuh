@@ -11,9 +11,10 @@
 // `blocks` of them (a wait on a barrier costs its thread about 150 clocks, which small slots would
 // spend per step).
 //
-// Routing (experts, if asked for): all CTAs share the router's logits, cut by tokens, experts and K;
-// the CTA that arrives last at 16 tokens chooses for them, a warp per token, and everyone waits
-// for all choices (a launch of its own took 17 to 32 us with cold weights, most of it waiting).
+// Routing (experts, if asked for): all CTAs share the router's logits, cut by tokens, experts and K.  Of
+// up to 16 tokens every CTA then makes all choices itself, a warp per token (two trips to L2
+// fewer); of more the CTA that arrives last at 16 tokens chooses for them and everyone waits for
+// all choices.  (A launch of its own took 17 to 32 us with cold weights, most of it waiting.)
 // First product (the only one of the projection): the weight rows are dealt out evenly over the
 // CTAs (one per SM) in groups -- the projection's rows / CTAs, or 16 rows of an expert -- and a
 // CTA takes each of its tiles over the whole of K, so no sum is ever split between CTAs.
@@ -79,12 +80,12 @@ struct StreamParams {
   unsigned long long wait_limit_ns;
   int inject;
 };
-constexpr int kStreamSync = 3;  // CTAs done with the second product; CTAs leaving; CTAs done with `sorted`
+constexpr int kStreamSync = 3;  // CTAs done with the second product; CTAs done with the counters; CTAs done with `sorted`
 
 // Shared memory behind the ring and barriers for the experts' lists.
 struct StreamLists {
   int words;          // u32 words of an expert's token set
-  int sets, first, offset, item, token, bytes;  // byte offsets
+  int sets, first, offset, item, token, choice, bytes;  // byte offsets
   __host__ __device__ StreamLists(int tokens, int experts, int top, int chunk) {
     words = (tokens + 31) / 32;
     const int pairs = tokens * top;
@@ -93,7 +94,8 @@ struct StreamLists {
     first = offset + (experts + 1) * 2;       // u16 [E + 1]: items before expert e
     item = (first + (experts + 1) * 2 + 7) & ~7;  // uint2 per item: expert | count << 16, first pair
     token = item + 8 * most_items(tokens, experts, top, chunk);  // u16 per pair: its token
-    bytes = (token + pairs * 2 + 15) & ~15;
+    choice = (token + pairs * 2 + 15) & ~15;  // up to 16 tokens: ids, then weights
+    bytes = choice + (tokens <= 16 ? (pairs * 8 + 15) & ~15 : 0);
   }
   // Items at most: one per chosen expert, and one more for each full chunk of pairs.
   __host__ __device__ static int most_items(int tokens, int experts, int top, int chunk) {
@@ -249,6 +251,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   uint16_t* first = reinterpret_cast<uint16_t*>(lbase + lists.first);
   uint2* item_list = reinterpret_cast<uint2*>(lbase + lists.item);
   uint16_t* token_of = reinterpret_cast<uint16_t*>(lbase + lists.token);
+  int* own_ids = reinterpret_cast<int*>(lbase + lists.choice);
+  float* own_weights = reinterpret_cast<float*>(own_ids + p.tokens * p.top);
+  const bool own_choice = MOE && p.routed && p.tokens <= 16;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -295,33 +300,50 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
 
   if constexpr (MOE) {
     if (p.routed) {
-      const RouteParams& r = p.route;
+      RouteParams r = p.route;
+      constexpr int kWarps = kStreamThreads / 32;
+      static_assert(kWarps == 16, "a warp per token of a tile");
+      auto choose = [&](int tile) {
+        const int t = tile * 16 + warp;
+        if (p.experts <= 64) route_tokens<BF16, 2, kWarps>(r, t, gbase);
+        else if (p.experts <= 256) route_tokens<BF16, 8, kWarps>(r, t, gbase);
+        else route_tokens<BF16, 16, kWarps>(r, t, gbase);
+        __syncthreads();
+      };
       const int groups = (p.experts + 7) / 8, tiles = (p.tokens + 15) / 16;
       const int units = groups * tiles * r.parts;
 #pragma unroll 1
       for (int u = c; u < units; u += C) {  // (token tile fastest: its CTAs share weights)
         const int tile = u % tiles, v = u / tiles, group = v % groups, kp = v / groups;
-        if (r.weight_f32) route_tile<BF16, true, 1, 1, kStreamThreads / 32>(r, tile * 16, group * 8, kp, r.parts, gbase);
-        else route_tile<BF16, false, 1, 1, kStreamThreads / 32>(r, tile * 16, group * 8, kp, r.parts, gbase);
-        if (threadIdx.x == 0) {
-          unsigned old;  // (releases what the whole CTA wrote: the barrier above)
-          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(r.counters + tile) : "memory");
-          *last_flag = old == static_cast<unsigned>(groups * r.parts - 1);
+        if (r.weight_f32) route_tile<BF16, true, 1, 1, kWarps>(r, tile * 16, group * 8, kp, r.parts, gbase);
+        else route_tile<BF16, false, 1, 1, kWarps>(r, tile * 16, group * 8, kp, r.parts, gbase);
+        if (own_choice) {
+          if (threadIdx.x == 0) red_release_add(r.counters, 1u);  // (what the whole CTA wrote: the barrier above)
+          continue;
         }
+        if (threadIdx.x == 0)
+          *last_flag = atom_add_acq_rel(r.counters + tile, 1u) == static_cast<unsigned>(groups * r.parts - 1);
         __syncthreads();
         if (*last_flag) {
-          constexpr int kWarps = kStreamThreads / 32;
-          static_assert(kWarps == 16, "a warp per token of a tile");
-          const int t = tile * 16 + warp;
-          if (p.experts <= 64) route_tokens<BF16, 2, kWarps>(r, t, gbase);
-          else if (p.experts <= 256) route_tokens<BF16, 8, kWarps>(r, t, gbase);
-          else route_tokens<BF16, 16, kWarps>(r, t, gbase);
-          __syncthreads();
+          choose(tile);
           if (threadIdx.x == 0) red_release_add(r.counters + tiles, 1u);
         }
         __syncthreads();
       }
-      if (threadIdx.x == 0) stream_wait_word(r.counters + tiles, static_cast<unsigned>(tiles), abort_flag, p, 2, -2);
+      if (threadIdx.x == 0)
+        stream_wait_word(own_choice ? r.counters : r.counters + tiles, static_cast<unsigned>(own_choice ? units : tiles),
+                         abort_flag, p, 2, -2);
+      __syncthreads();
+      if (own_choice) {
+        r.ids = own_ids;
+        r.weights = own_weights;
+        choose(0);
+        if (c == 0)
+          for (int i = threadIdx.x; i < p.tokens * p.top; i += kStreamThreads) {
+            p.route.ids[i] = own_ids[i];
+            p.route.weights[i] = own_weights[i];
+          }
+      }
       fence_async_shared();  // the ring's bytes were used above; TMA writes them next
       __syncthreads();
     }
@@ -330,7 +352,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     // an expert twice is one pair; an id outside [0, experts) is none.
     const int pairs = p.tokens * p.top;
     for (int i = threadIdx.x; i < pairs; i += kStreamThreads) {
-      const int e = __ldcg(p.ids + i);
+      const int e = own_choice ? own_ids[i] : __ldcg(p.ids + i);
       const int t = i / p.top;
       if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts))
         atomicOr(&sets[e * lists.words + (t >> 5)], 1u << (t & 31));
@@ -745,9 +767,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         }
       }
       if (lane < p.top) {
-        const int e = __ldcg(p.ids + t * p.top + lane);
+        const int at = t * p.top + lane;
+        const int e = own_choice ? own_ids[at] : __ldcg(p.ids + at);
         if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts)) {
-          u.wt = __ldcg(p.weights + t * p.top + lane);
+          u.wt = own_choice ? own_weights[at] : __ldcg(p.weights + at);
           int rank = 0;
           for (int w = 0; w < (t >> 5); ++w) rank += __popc(sets[e * lists.words + w]);
           rank += __popc(sets[e * lists.words + (t >> 5)] & ((1u << (t & 31)) - 1u));
@@ -762,11 +785,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       }
       return u;
     };
+    if (threadIdx.x == 0) red_release_add(sync_words, 1u);  // (covers the whole CTA's sums: the barrier above)
     int unit = warp * C + c;
     Share now = look_up(unit);
     if (threadIdx.x == 0) {
-      red_release_add(sync_words, 1u);  // (covers the whole CTA's sums: the barrier above)
       if (!*abort_flag) stream_wait_word(sync_words, static_cast<unsigned>(C), abort_flag, p, 3, -1);
+      // From here on this CTA reads no counter; the last to say so clears them for the next launch.
+      *last_flag = atom_add_acq_rel(sync_words + 1, 1u) == static_cast<unsigned>(C - 1);
     }
     __syncthreads();
     if (!*abort_flag) {
@@ -825,10 +850,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         now = next;
       }
     }
-    // The last CTA to leave clears the counters for the next launch.
-    __syncthreads();
-    if (threadIdx.x == 0) *last_flag = atom_add_acq_rel(sync_words + 1, 1u) == static_cast<unsigned>(C - 1);
-    __syncthreads();
     if (*last_flag) {
       for (int i = threadIdx.x; i < items; i += kStreamThreads) item_done[i] = 0;
       if (threadIdx.x < kStreamSync) sync_words[threadIdx.x] = 0;
