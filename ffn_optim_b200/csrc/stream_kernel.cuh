@@ -12,9 +12,10 @@
 // spend per step).
 //
 // Routing (experts, if asked for): all CTAs share the router's logits, cut by tokens, experts and K.  Of
-// up to 16 tokens every CTA then makes all choices itself, a warp per token (two trips to L2
-// fewer); of more the CTA that arrives last at 16 tokens chooses for them and everyone waits for
-// all choices.  (A launch of its own took 17 to 32 us with cold weights, most of it waiting.)
+// up to 4 tokens every CTA then makes all choices itself, a warp per token (two trips to L2 fewer: 1
+// token 34.6 -> 33.3 us; but 7 tokens 26.9 -> 29.7, all CTAs reading the same lines); of more the
+// CTA that arrives last at 16 tokens chooses for them and everyone waits for all choices.  (A
+// launch of its own took 17 to 32 us with cold weights, most of it waiting.)
 // First product (the only one of the projection): the weight rows are dealt out evenly over the
 // CTAs (one per SM) in groups -- the projection's rows / CTAs, or 16 rows of an expert -- and a
 // CTA takes each of its tiles over the whole of K, so no sum is ever split between CTAs.
@@ -41,6 +42,7 @@ constexpr int kStreamThreads = 512;  // 8 warps with roles, 8 more for the lists
 constexpr int kStreamMaxStages = 40;
 constexpr int kStreamMinSteps = 4;   // fewest K steps of the second product worth a CTA of their own
 constexpr int kStreamBarBytes = 1024;
+constexpr int kStreamOwnChoice = 4;  // tokens up to which every CTA chooses for itself
 
 struct StreamParams {
   CUtensorMap tm_w1, tm_w2;  // weights [E][halves][rows][K]: a box is one group's rows (SwiGLU: 8 of
@@ -94,8 +96,8 @@ struct StreamLists {
     first = offset + (experts + 1) * 2;       // u16 [E + 1]: items before expert e
     item = (first + (experts + 1) * 2 + 7) & ~7;  // uint2 per item: expert | count << 16, first pair
     token = item + 8 * most_items(tokens, experts, top, chunk);  // u16 per pair: its token
-    choice = (token + pairs * 2 + 15) & ~15;  // up to 16 tokens: ids, then weights
-    bytes = choice + (tokens <= 16 ? (pairs * 8 + 15) & ~15 : 0);
+    choice = (token + pairs * 2 + 15) & ~15;  // kStreamOwnChoice tokens: ids, then weights
+    bytes = choice + (tokens <= kStreamOwnChoice ? (pairs * 8 + 15) & ~15 : 0);
   }
   // Items at most: one per chosen expert, and one more for each full chunk of pairs.
   __host__ __device__ static int most_items(int tokens, int experts, int top, int chunk) {
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   uint16_t* token_of = reinterpret_cast<uint16_t*>(lbase + lists.token);
   int* own_ids = reinterpret_cast<int*>(lbase + lists.choice);
   float* own_weights = reinterpret_cast<float*>(own_ids + p.tokens * p.top);
-  const bool own_choice = MOE && p.routed && p.tokens <= 16;
+  const bool own_choice = MOE && p.routed && p.tokens <= kStreamOwnChoice;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
