@@ -11,11 +11,11 @@
 // `blocks` of them (a wait on a barrier costs its thread about 150 clocks, which small slots would
 // spend per step).
 //
-// Routing (experts, if asked for): all CTAs share the router's logits, cut by tokens, experts and K.  Of
-// up to 4 tokens every CTA then makes all choices itself, a warp per token (two trips to L2 fewer: 1
-// token 34.6 -> 33.3 us; but 7 tokens 26.9 -> 29.7, all CTAs reading the same lines); of more the
-// CTA that arrives last at 16 tokens chooses for them and everyone waits for all choices.  (A
-// launch of its own took 17 to 32 us with cold weights, most of it waiting.)
+// Routing (experts, if asked for): all CTAs share the router's logits, cut by tokens, experts and K;
+// the CTA that arrives last at 16 tokens chooses for them, a warp per token, and everyone waits
+// for all choices.  (A launch of its own took 17 to 32 us with cold weights, most of it waiting.
+// Every CTA choosing for itself saves two trips to L2, but all read the same lines: 1 token 0.2 us
+// less, 7 tokens 2.8 us more.)
 // First product (the only one of the projection): the weight rows are dealt out evenly over the
 // CTAs (one per SM) in groups -- the projection's rows / CTAs, or 16 rows of an expert -- and a
 // CTA takes each of its tiles over the whole of K, so no sum is ever split between CTAs.
@@ -42,7 +42,6 @@ constexpr int kStreamThreads = 512;  // 8 warps with roles, 8 more for the lists
 constexpr int kStreamMaxStages = 40;
 constexpr int kStreamMinSteps = 4;   // fewest K steps of the second product worth a CTA of their own
 constexpr int kStreamBarBytes = 1024;
-constexpr int kStreamOwnChoice = 4;  // tokens up to which every CTA chooses for itself
 
 struct StreamParams {
   CUtensorMap tm_w1, tm_w2;  // weights [E][halves][rows][K]: a box is one group's rows (SwiGLU: 8 of
@@ -87,7 +86,7 @@ constexpr int kStreamSync = 3;  // CTAs done with the second product; CTAs done 
 // Shared memory behind the ring and barriers for the experts' lists.
 struct StreamLists {
   int words;          // u32 words of an expert's token set
-  int sets, first, offset, item, token, choice, bytes;  // byte offsets
+  int sets, first, offset, item, token, bytes;  // byte offsets
   __host__ __device__ StreamLists(int tokens, int experts, int top, int chunk) {
     words = (tokens + 31) / 32;
     const int pairs = tokens * top;
@@ -96,8 +95,7 @@ struct StreamLists {
     first = offset + (experts + 1) * 2;       // u16 [E + 1]: items before expert e
     item = (first + (experts + 1) * 2 + 7) & ~7;  // uint2 per item: expert | count << 16, first pair
     token = item + 8 * most_items(tokens, experts, top, chunk);  // u16 per pair: its token
-    choice = (token + pairs * 2 + 15) & ~15;  // kStreamOwnChoice tokens: ids, then weights
-    bytes = choice + (tokens <= kStreamOwnChoice ? (pairs * 8 + 15) & ~15 : 0);
+    bytes = (token + pairs * 2 + 15) & ~15;
   }
   // Items at most: one per chosen expert, and one more for each full chunk of pairs.
   __host__ __device__ static int most_items(int tokens, int experts, int top, int chunk) {
@@ -253,9 +251,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
   uint16_t* first = reinterpret_cast<uint16_t*>(lbase + lists.first);
   uint2* item_list = reinterpret_cast<uint2*>(lbase + lists.item);
   uint16_t* token_of = reinterpret_cast<uint16_t*>(lbase + lists.token);
-  int* own_ids = reinterpret_cast<int*>(lbase + lists.choice);
-  float* own_weights = reinterpret_cast<float*>(own_ids + p.tokens * p.top);
-  const bool own_choice = MOE && p.routed && p.tokens <= kStreamOwnChoice;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -302,16 +297,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
 
   if constexpr (MOE) {
     if (p.routed) {
-      RouteParams r = p.route;
+      const RouteParams& r = p.route;
       constexpr int kWarps = kStreamThreads / 32;
       static_assert(kWarps == 16, "a warp per token of a tile");
-      auto choose = [&](int tile) {
-        const int t = tile * 16 + warp;
-        if (p.experts <= 64) route_tokens<BF16, 2, kWarps>(r, t, gbase);
-        else if (p.experts <= 256) route_tokens<BF16, 8, kWarps>(r, t, gbase);
-        else route_tokens<BF16, 16, kWarps>(r, t, gbase);
-        __syncthreads();
-      };
       const int groups = (p.experts + 7) / 8, tiles = (p.tokens + 15) / 16;
       const int units = groups * tiles * r.parts;
 #pragma unroll 1
@@ -319,33 +307,20 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         const int tile = u % tiles, v = u / tiles, group = v % groups, kp = v / groups;
         if (r.weight_f32) route_tile<BF16, true, 1, 1, kWarps>(r, tile * 16, group * 8, kp, r.parts, gbase);
         else route_tile<BF16, false, 1, 1, kWarps>(r, tile * 16, group * 8, kp, r.parts, gbase);
-        if (own_choice) {
-          if (threadIdx.x == 0) red_release_add(r.counters, 1u);  // (what the whole CTA wrote: the barrier above)
-          continue;
-        }
-        if (threadIdx.x == 0)
+        if (threadIdx.x == 0)  // (releases what the whole CTA wrote: the barrier above)
           *last_flag = atom_add_acq_rel(r.counters + tile, 1u) == static_cast<unsigned>(groups * r.parts - 1);
         __syncthreads();
         if (*last_flag) {
-          choose(tile);
+          const int t = tile * 16 + warp;
+          if (p.experts <= 64) route_tokens<BF16, 2, kWarps>(r, t, gbase);
+          else if (p.experts <= 256) route_tokens<BF16, 8, kWarps>(r, t, gbase);
+          else route_tokens<BF16, 16, kWarps>(r, t, gbase);
+          __syncthreads();
           if (threadIdx.x == 0) red_release_add(r.counters + tiles, 1u);
         }
         __syncthreads();
       }
-      if (threadIdx.x == 0)
-        stream_wait_word(own_choice ? r.counters : r.counters + tiles, static_cast<unsigned>(own_choice ? units : tiles),
-                         abort_flag, p, 2, -2);
-      __syncthreads();
-      if (own_choice) {
-        r.ids = own_ids;
-        r.weights = own_weights;
-        choose(0);
-        if (c == 0)
-          for (int i = threadIdx.x; i < p.tokens * p.top; i += kStreamThreads) {
-            p.route.ids[i] = own_ids[i];
-            p.route.weights[i] = own_weights[i];
-          }
-      }
+      if (threadIdx.x == 0) stream_wait_word(r.counters + tiles, static_cast<unsigned>(tiles), abort_flag, p, 2, -2);
       fence_async_shared();  // the ring's bytes were used above; TMA writes them next
       __syncthreads();
     }
@@ -354,7 +329,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     // an expert twice is one pair; an id outside [0, experts) is none.
     const int pairs = p.tokens * p.top;
     for (int i = threadIdx.x; i < pairs; i += kStreamThreads) {
-      const int e = own_choice ? own_ids[i] : __ldcg(p.ids + i);
+      const int e = __ldcg(p.ids + i);
       const int t = i / p.top;
       if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts))
         atomicOr(&sets[e * lists.words + (t >> 5)], 1u << (t & 31));
@@ -770,9 +745,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
       }
       if (lane < p.top) {
         const int at = t * p.top + lane;
-        const int e = own_choice ? own_ids[at] : __ldcg(p.ids + at);
+        const int e = __ldcg(p.ids + at);
         if (static_cast<unsigned>(e) < static_cast<unsigned>(p.experts)) {
-          u.wt = own_choice ? own_weights[at] : __ldcg(p.weights + at);
+          u.wt = __ldcg(p.weights + at);
           int rank = 0;
           for (int w = 0; w < (t >> 5); ++w) rank += __popc(sets[e * lists.words + w]);
           rank += __popc(sets[e * lists.words + (t >> 5)] & ((1u << (t & 31)) - 1u));
