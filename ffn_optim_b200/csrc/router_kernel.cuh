@@ -8,10 +8,10 @@
 //     second set of MMAs over the operands with their signs cleared gives S; for many, where
 //     mma.sync is the bound (1000 tokens of 256 experts of 4096: 29 us with it), the norms of the
 //     two rows bound it.
-//   * The finishing warp picks the top k + 1 keys; experts whose key lies closer to one of them
-//     than those errors allow (and logits that left fp32's range) are summed again in fp64, by the
-//     whole warp, and the choice is made again.  For normally distributed logits that is a
-//     few tokens in a thousand.
+//   * The finishing warp picks the top k keys; chosen experts whose key another one's may meet within
+//     those errors, those others, and logits that left fp32's range are summed again in fp64 by the
+//     whole CTA, and the choice is made again.  For normally distributed logits that is a few tokens in
+//     a thousand.
 //   * fp32 weights are summed in fp64 outright (S = 0: nothing is summed twice).
 //
 // Fewer than 128 tokens, and fp32 weights (route_kernel): a CTA takes 16 MT tokens x 8 NT experts;
@@ -134,7 +134,7 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
   bool odd = false;  // a logit left fp32's range
   int chosen = 0;               // lane j < top: the j-th choice,
   double score = 0.0;           // its score
-  unsigned long long mine = 0, rest = 0;  // and its key; the key after the last choice
+  unsigned long long mine = 0;  // and its key
   double loss = 0.0;    // a logit's error at most
   unsigned again = 0;  // bit i: expert lane + 32 i has to be summed again
   if (live) {
@@ -173,6 +173,13 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
     }
     loss = p.weight_f32 ? 0.0 : kRouteLoss * static_cast<double>(s);
   }
+  // A key moves by at most a logit's error times the steepest slope on the way: p (1 - p) for the sigmoid,
+  // whose slope moves by less than the error; p_i (e^(2 loss) - 1), at most 1/2 loss, for the softmax.
+  double other = -INFINITY;
+  const double steep = 2.0 + 3.0 * loss;
+  auto reach = [&](double v) {
+    return loss * (p.sigmoid ? v * (1.0 - v) + loss : loss > 0.5 ? 0.5 : fmin(0.5, steep * v));
+  };
   // Once, and again where sums changed: one loop, so that the code is there once (few tokens wait for
   // instruction fetches more than for arithmetic; 1000 tokens of 256 experts 42.9 -> 41.0 us).
   bool first = true, changed = false;
@@ -207,10 +214,9 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
         if (e < p.E) q[e] = v[i];
       }
       __syncwarp();
-      // The k largest keys and the next one, equal ones by index.
-      const int want = first && p.top < p.E ? p.top + 1 : p.top;
+      // The k largest keys, equal ones by index.
 #pragma unroll 1
-      for (int j = 0; j < want; ++j) {
+      for (int j = 0; j < p.top; ++j) {
         unsigned long long best = key[0];
         int at = 0;
 #pragma unroll
@@ -222,29 +228,36 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
         const bool top = high && static_cast<unsigned>(best) == lo;
         const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, top ? static_cast<unsigned>(lane + 32 * at) : 0xffffffffu));
         const unsigned long long k = static_cast<unsigned long long>(hi) << 32 | lo;
-        if (j == p.top) {
-          rest = k;
-          break;
-        }
         if (lane == j) chosen = e, mine = k;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
           if (e == lane + 32 * i) key[i] = 0;
       }
       if (lane < p.top) score = q[chosen];
+      // The key that another expert may have at most.
+      if (first && loss > 0.0) {
+        other = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (key[i]) other = fmax(other, unordered(key[i]) + reach(v[i]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) other = fmax(other, __shfl_xor_sync(0xffffffffu, other, o));
+      }
     }
     if (!first) break;
     first = false;
     if (live) {
-      // Could the errors of two logits have swapped neighbours?  A score moves by at most its slope
-      // times a logit's error: p (1 - p) for the sigmoid (a little more, for where p changes on the
-      // way), 2 p with softmax's normaliser.
-      const double reach = 2.0 * loss * (p.sigmoid ? score * (1.0 - score) + loss : 2.0 * score);
-      const unsigned long long after = __shfl_down_sync(0xffffffffu, mine, 1);
-      const bool last = lane == p.top - 1 && p.top == p.E;
-      const double here = unordered(mine);
-      const unsigned nears = __ballot_sync(
-          0xffffffffu, lane < p.top && !last && loss > 0.0 && here - unordered(lane == p.top - 1 ? rest : after) <= reach);
+      // Could errors have changed the choice, or its order?  (Keys of infinite size do not move.)
+      const double here = unordered(mine), far = reach(score);
+      bool close = false;
+      if (loss > 0.0) {
+        double later = lane < p.top ? here + far : -INFINITY;  // at most, from this choice on
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) later = fmax(later, __shfl_down_sync(0xffffffffu, later, o));
+        later = __shfl_down_sync(0xffffffffu, later, 1);
+        close = lane < p.top && isfinite(here) && fmax(lane == p.top - 1 ? -INFINITY : later, other) >= here - far;
+      }
+      const bool nears = __any_sync(0xffffffffu, close);
       const bool odds = __any_sync(0xffffffffu, odd);
       if (nears || odds) {
         // A token that is not finite itself keeps what the first sums gave.
@@ -257,21 +270,21 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
           for (int i = 0; i < 4; ++i) finite = finite && isfinite(unpack_lo<BF16>(r[i])) && isfinite(unpack_hi<BF16>(r[i]));
         }
         if (__all_sync(0xffffffffu, finite)) {
-          // Logits out of range, and experts whose key is as close to a chosen one's, or a chosen one whose
-          // neighbour is.  (Of two scores within reach of one another the chosen one's slope is the larger.)
+          // Logits out of range, chosen experts whose key another one's may meet, and those others.
 #pragma unroll
           for (int i = 0; i < PER; ++i)
             if (lane + 32 * i < p.E && !isfinite(z[i])) again |= 1u << i;
 #pragma unroll 1
           for (int j = 0; j < p.top; ++j) {
-            const double kj = __shfl_sync(0xffffffffu, here, j), rj = __shfl_sync(0xffffffffu, reach, j);
+            const double kj = __shfl_sync(0xffffffffu, here, j), rj = __shfl_sync(0xffffffffu, far, j);
             const int cj = __shfl_sync(0xffffffffu, chosen, j);
-            const bool nj = (nears >> j | (j ? nears >> (j - 1) : 0u)) & 1u;
+            bool met = false;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
               const int e = lane + 32 * i;
-              if (e < p.E && (e == cj ? nj : loss > 0.0 && fabs(v[i] + bias[i] - kj) <= rj)) again |= 1u << i;
+              if (loss > 0.0 && e < p.E && e != cj && fabs(v[i] + bias[i] - kj) <= rj + reach(v[i])) met = true, again |= 1u << i;
             }
+            if (__any_sync(0xffffffffu, met) && lane == cj % 32) again |= 1u << (cj / 32);
           }
         }
       }

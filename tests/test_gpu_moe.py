@@ -109,6 +109,28 @@ def test_router_close_logits(m):
     check_route(route_experts(x, w, top_k=16), x, w, top_k=16)
 
 
+@pytest.mark.parametrize("m", [1, 20, 300])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("place", [3, 35])
+def test_router_small_score_chosen_by_its_bias(m, scoring, place):
+    """An expert of score 4e-18 leads by its bias; another one's logit of 1e-6, lost in the fp32 sum beside
+    64 - 64, moves its score of 0.5 past it."""
+    k, e = 512, 40
+    x = torch.zeros(m, k, dtype=BF, device="cuda")
+    x[:, [0, 1, 32]] = 1
+    w = torch.zeros(e, k, dtype=BF, device="cuda")
+    w[:, 0] = -60.0  # nobody's choice
+    w[7, 0] = -40.0
+    w[place, 0], w[place, 1], w[place, 32] = 64.0, 1e-6, -64.0
+    w[11, 0] = 0.0  # (the softmax's other half)
+    bias = torch.zeros(e, device="cuda")
+    bias[11] = -1.0
+    bias[7] = 0.5 + 2.0 ** -23  # between 0.5 and 0.5 + 1e-6 / 4
+    ids, wt = route_experts(x, w, top_k=2, scoring=scoring, choice_bias=bias)
+    assert route64(x, w, 2, scoring, bias)[0][0].tolist() == [place, 7]
+    check_route((ids, wt), x, w, top_k=2, scoring=scoring, choice_bias=bias)
+
+
 def test_router_repeats_graph_and_masks():
     g = gen(9)
     x, w = normal(g, 50, 320), normal(g, 40, 320, scale=0.05)
