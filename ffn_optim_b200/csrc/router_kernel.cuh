@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
   if (threadIdx.x == 0) grid_dep_launch();
   grid_dep_wait();
   // Thread i copies 16-byte chunk i % 8 of rows i / 8 and i / 8 + 32 of both operands; rows past the
-  // last repeat it.  Chunk c of row r lies at c ^ (r % 8).
+  // last repeat it.  Chunk c of row r lies at c ^ 4 (r % 2): eight lanes read the same half of two rows.
   const int row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
   auto load = [&](int step, int slot) {
     const int k = step * kRouteStep + 8 * chunk;
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = row + 32 * h;
-      const uint32_t dst = base + slot * kLogitStage + r * 128 + ((chunk ^ (r & 7)) << 4);
+      const uint32_t dst = base + slot * kLogitStage + r * 128 + ((chunk ^ (4 * (r & 1))) << 4);
       const long long x = static_cast<long long>(min(t0 + r, p.M - 1)) * p.ldx, w = static_cast<long long>(min(e0 + r, p.E - 1)) * p.ldw;
       copy_async16(dst, static_cast<const uint16_t*>(p.x) + x + (bytes ? k : 0), bytes);
       copy_async16(dst + kLogitStage / 2, static_cast<const uint16_t*>(p.w) + w + (bytes ? k : 0), bytes);
@@ -544,9 +544,9 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
     for (int h = 0; h < 2; ++h) {
       uint4 xv[4], wv[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xv[i] = ld_shared_u4(sx + (m0 + 8 * i + g) * 128 + (((4 * h + q) ^ g) << 4));
+      for (int i = 0; i < 4; ++i) xv[i] = ld_shared_u4(sx + (m0 + 8 * i + g) * 128 + (((4 * h + q) ^ (4 * (g & 1))) << 4));
 #pragma unroll
-      for (int j = 0; j < 2; ++j) wv[j] = ld_shared_u4(sw + (n0 + 8 * j + g) * 128 + (((4 * h + q) ^ g) << 4));
+      for (int j = 0; j < 2; ++j) wv[j] = ld_shared_u4(sw + (n0 + 8 * j + g) * 128 + (((4 * h + q) ^ (4 * (g & 1))) << 4));
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
