@@ -472,8 +472,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
 
 // ---- many tokens -----------------------------------------------------------------------------
 constexpr int kLogitTile = 64;                            // tokens and experts of a tile
-constexpr int kLogitStages = 4;
-constexpr int kLogitStage = 2 * kLogitTile * kRouteStep * 2;  // bytes: 64 x 64 of x and of w
+constexpr int kLogitStages = 3;
+constexpr int kLogitChains = 2;                           // K steps of 64 in a stage (one per barrier: 37.8 us, two 36.3)
+constexpr int kLogitPart = kLogitTile * kRouteStep * 2;   // bytes: 64 x 64 of x or of w
+constexpr int kLogitStage = 2 * kLogitChains * kLogitPart;
 constexpr int kLogitSmem = kLogitStages * kLogitStage;
 
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, int bytes) {  // the rest is zeros
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
   const int t0 = blockIdx.y * kLogitTile, e0 = blockIdx.x * kLogitTile;
-  const int steps = (p.K + kRouteStep - 1) / kRouteStep;
+  const int steps = (p.K + kLogitChains * kRouteStep - 1) / (kLogitChains * kRouteStep);
   const int s0 = steps * blockIdx.z / gridDim.z, s1 = steps * (blockIdx.z + 1) / gridDim.z;
   if (threadIdx.x == 0) grid_dep_launch();
   grid_dep_wait();
@@ -502,15 +504,18 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
   // last repeat it.  Chunk c of row r lies at c ^ 4 (r % 2): eight lanes read the same half of two rows.
   const int row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
   auto load = [&](int step, int slot) {
-    const int k = step * kRouteStep + 8 * chunk;
-    const int bytes = max(0, min(16, 2 * (p.K - k)));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = row + 32 * h;
-      const uint32_t dst = base + slot * kLogitStage + r * 128 + ((chunk ^ (4 * (r & 1))) << 4);
       const long long x = static_cast<long long>(min(t0 + r, p.M - 1)) * p.ldx, w = static_cast<long long>(min(e0 + r, p.E - 1)) * p.ldw;
-      copy_async16(dst, static_cast<const uint16_t*>(p.x) + x + (bytes ? k : 0), bytes);
-      copy_async16(dst + kLogitStage / 2, static_cast<const uint16_t*>(p.w) + w + (bytes ? k : 0), bytes);
+#pragma unroll
+      for (int c = 0; c < kLogitChains; ++c) {
+        const int k = (step * kLogitChains + c) * kRouteStep + 8 * chunk;
+        const int bytes = max(0, min(16, 2 * (p.K - k)));
+        const uint32_t dst = base + slot * kLogitStage + 2 * c * kLogitPart + r * 128 + ((chunk ^ (4 * (r & 1))) << 4);
+        copy_async16(dst, static_cast<const uint16_t*>(p.x) + x + (bytes ? k : 0), bytes);
+        copy_async16(dst + kLogitPart, static_cast<const uint16_t*>(p.w) + w + (bytes ? k : 0), bytes);
+      }
     }
   };
 #pragma unroll
@@ -538,38 +543,41 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
     __syncthreads();
     if (s + kLogitStages - 1 < s1) load(s + kLogitStages - 1, (s - s0 + kLogitStages - 1) % kLogitStages);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const uint32_t sx = base + (s - s0) % kLogitStages * kLogitStage, sw = sx + kLogitStage / 2;
-    float d[2][2][4] = {};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint4 xv[4], wv[2];
+    for (int c = 0; c < kLogitChains; ++c) {
+      const uint32_t sx = base + (s - s0) % kLogitStages * kLogitStage + 2 * c * kLogitPart, sw = sx + kLogitPart;
+      float d[2][2][4] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xv[i] = ld_shared_u4(sx + (m0 + 8 * i + g) * 128 + (((4 * h + q) ^ (4 * (g & 1))) << 4));
+      for (int h = 0; h < 2; ++h) {
+        uint4 xv[4], wv[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) wv[j] = ld_shared_u4(sw + (n0 + 8 * j + g) * 128 + (((4 * h + q) ^ (4 * (g & 1))) << 4));
+        for (int i = 0; i < 4; ++i) xv[i] = ld_shared_u4(sx + (m0 + 8 * i + g) * 128 + (((4 * h + q) ^ (4 * (g & 1))) << 4));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) wv[j] = ld_shared_u4(sw + (n0 + 8 * j + g) * 128 + (((4 * h + q) ^ (4 * (g & 1))) << 4));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 &a = xv[2 * i], &b = xv[2 * i + 1], &w = wv[j];
+            mma_16816<BF16>(d[i][j], a.x, b.x, a.y, b.y, w.x, w.y);
+            mma_16816<BF16>(d[i][j], a.z, b.z, a.w, b.w, w.z, w.w);
+          }
+        if (x_norm) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x2[i] = squares(xv[i], x2[i]);
+        }
+        if (w_norm) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) w2[j] = squares(wv[j], w2[j]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 &a = xv[2 * i], &b = xv[2 * i + 1], &w = wv[j];
-          mma_16816<BF16>(d[i][j], a.x, b.x, a.y, b.y, w.x, w.y);
-          mma_16816<BF16>(d[i][j], a.z, b.z, a.w, b.w, w.z, w.w);
-        }
-      if (x_norm) {
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x2[i] = squares(xv[i], x2[i]);
-      }
-      if (w_norm) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) w2[j] = squares(wv[j], w2[j]);
-      }
+          for (int v = 0; v < 4; ++v) z[i][j][v] += static_cast<double>(d[i][j][v]);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) z[i][j][v] += static_cast<double>(d[i][j][v]);
   }
   const size_t part = static_cast<size_t>(blockIdx.z) * p.M * p.E;
 #pragma unroll
