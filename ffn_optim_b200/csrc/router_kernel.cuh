@@ -5,13 +5,13 @@
 //   * 16-bit weights: products on mma.sync (m16n8k16, fp32 accumulation) in chains of 64 of K; each
 //     chain's fp32 result is added in fp64.  A chain of four MMAs loses at most 4 * 2^-22 of the
 //     sum of its |x w|, so a logit is off by at most 2^-20 S, S = sum |x w|.  For few tokens a
-//     second set of MMAs over the operands with their signs cleared gives S; for many, where
-//     mma.sync is the bound (1000 tokens of 256 experts of 4096: 29 us with it), the norms of the
-//     two rows bound it.
+//     second set of MMAs over the operands with their signs cleared gives S; for many, where that
+//     cost most (1000 tokens of 256 experts of 4096: 29 us for the logits), the norms of the two
+//     rows bound it.
 //   * The finishing warp picks the top k keys; chosen experts whose key another one's may meet within
 //     those errors, those others, and logits that left fp32's range are summed again in fp64 by the
-//     whole CTA, and the choice is made again.  For normally distributed logits that is a few tokens in
-//     a thousand.
+//     whole CTA, and the choice is made again.  For normally distributed operands that is one or
+//     two tokens in a hundred.
 //   * fp32 weights are summed in fp64 outright (S = 0: nothing is summed twice).
 //
 // Fewer than 128 tokens, and fp32 weights (route_kernel): a CTA takes 16 MT tokens x 8 NT experts;
