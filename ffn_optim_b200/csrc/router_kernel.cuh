@@ -169,7 +169,14 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
     if (p.many) {  // |x| |w| of the longest w
       float x2 = 0.f;
       for (int c = 0; c < p.parts; ++c) x2 += __ldcg(p.sums + static_cast<size_t>(c) * (p.M + p.E) + t);
-      s = sqrtf(x2) * sqrtf(s) * 1.001f;  // (the sums of squares are fp32)
+      // (The sums of squares are fp32.  Below 2^-100 squares may be missing: such a token's logits, unless
+      // all are zero, are summed again.)
+      const bool small = x2 < 0x1p-100f || s < 0x1p-100f;
+      s = sqrtf(x2) * sqrtf(s) * 1.001f;
+      bool some = false;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) some |= lane + 32 * i < p.E && z[i] != 0.0;
+      if (small && __any_sync(0xffffffffu, some)) s = INFINITY;
     }
     loss = p.weight_f32 ? 0.0 : kRouteLoss * static_cast<double>(s);
   }

@@ -131,6 +131,21 @@ def test_router_small_score_chosen_by_its_bias(m, scoring, place):
     check_route((ids, wt), x, w, top_k=2, scoring=scoring, choice_bias=bias)
 
 
+@pytest.mark.parametrize("m", [20, 300])
+def test_router_operands_whose_squares_leave_fp32(m):
+    """x of 2^-80 and weights up to 2^86: the logits are ordinary, one of them lost beside 64 - 64."""
+    x = torch.zeros(m, 512, dtype=BF, device="cuda")
+    x[:, [0, 1, 32]] = 2.0 ** -80
+    w = torch.zeros(40, 512, dtype=BF, device="cuda")
+    w[:, 0] = -60.0
+    w[5, 0], w[5, 1], w[5, 32] = 64.0, 1e-6, -64.0
+    w[3, 0] = 0.0
+    w *= 2.0 ** 80
+    ids, wt = route_experts(x, w, top_k=2)
+    assert route64(x, w, 2)[0][0].tolist() == [5, 3]
+    check_route((ids, wt), x, w, top_k=2)
+
+
 def test_router_repeats_graph_and_masks():
     g = gen(9)
     x, w = normal(g, 50, 320), normal(g, 40, 320, scale=0.05)
