@@ -211,8 +211,9 @@ const RouteFns kRouteFns[3][2] = {{route_fns<false, 2>(), route_fns<true, 2>()},
 
 // Tokens from which the router runs as two kernels (16-bit weights), and the parts of K of its first.
 constexpr int64_t kRouteMany = 128;
+bool route_many(const ffn_b200_router_problem& p) { return p.m >= kRouteMany && !p.weight_f32; }
 int route_parts(const ffn_b200_router_problem& p) {
-  if (p.m < kRouteMany || p.weight_f32) return 1;
+  if (!route_many(p)) return 1;
   const int64_t tiles = cdiv(p.m, ffnb200::kLogitTile) * cdiv(p.experts, ffnb200::kLogitTile);
   const int64_t steps = cdiv(p.k, ffnb200::kRouteStep);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 296 / tiles, steps / 8})));  // two CTAs per SM
@@ -506,8 +507,11 @@ int ffn_b200_router_scratch(const ffn_b200_router_problem* pr, int64_t* logit_do
   if (!pr || !logit_doubles || !counter_words) return FFN_B200_ERR_INVALID;
   const int rc = check_router(*pr);
   if (rc) return rc;
-  const int64_t cells = pr->m * pr->experts * route_parts(*pr);
-  *logit_doubles = cells + (cells + 1) / 2;  // fp64 logits, then fp32 sums of |x w|
+  // fp64 logits, then fp32: sums of |x w|, or of many tokens the squared norms of their rows and the weights'
+  // (more of them than logits when there is one expert).
+  const int64_t parts = route_parts(*pr), cells = parts * pr->m * pr->experts;
+  const int64_t floats = route_many(*pr) ? std::max(cells, parts * (pr->m + pr->experts)) : cells;
+  *logit_doubles = cells + (floats + 1) / 2;
   *counter_words = cdiv(pr->m, 16);
   return FFN_B200_OK;
 }
@@ -525,12 +529,11 @@ int ffn_b200_router_run(const ffn_b200_router_problem* pr, const void* x, int64_
   P.mask = mask;
   P.ids = ids;
   P.weights = weights;
-  const int many = pr->m >= kRouteMany, w32 = pr->weight_f32;
   // Experts per lane of a warp: as few registers and as little code as the number of experts needs.
   const int per = pr->experts <= 64 ? 0 : (pr->experts <= 256 ? 1 : 2);
   const RouteFns& fns = pr->dtype == FFN_B200_BF16 ? kRouteFns[per][1] : kRouteFns[per][0];
-  if (!many) return launch_route(w32 ? fns.few32 : fns.few, P, 1, 1, stream);  // small tiles: more CTAs
-  if (w32) return launch_route(fns.many32, P, 2, 4, stream);
+  if (pr->m < kRouteMany) return launch_route(pr->weight_f32 ? fns.few32 : fns.few, P, 1, 1, stream);  // small tiles: more CTAs
+  if (!route_many(*pr)) return launch_route(fns.many32, P, 2, 4, stream);
   P.many = 1;
   const dim3 tiles(static_cast<unsigned>(cdiv(P.E, ffnb200::kLogitTile)), static_cast<unsigned>(cdiv(P.M, ffnb200::kLogitTile)),
                    static_cast<unsigned>(P.parts));

@@ -196,3 +196,20 @@ def test_pack_rows_rejects_bad_arguments(lib):
         args = list(ok)
         args[i] = v
         assert lib.ffn_b200_pack_rows(*args) == _lib.ERR_INVALID
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+def test_router_scratch_holds_what_the_kernels_index(lib, f32):
+    """Behind parts x M x E fp64 logits lie as many fp32 sums or, for 128 tokens and more of 16-bit weights,
+    parts x (M + E) fp32 norms: more, when there is one expert."""
+    a, b = ctypes.c_int64(), ctypes.c_int64()
+    for m in (1, 2, 127, 128, 129, 256, 1000, 6993, 100000):
+        for e in (1, 2, 3, 64, 512):
+            for k in (8, 64, 512, 1000, 4096, 65535):
+                prob = _lib.RouterProblem(m, k, e, 1, 1, f32, 0, 1, 1.0, 0)
+                assert lib.ffn_b200_router_scratch(ctypes.byref(prob), ctypes.byref(a), ctypes.byref(b)) == _lib.OK
+                many = m >= 128 and not f32
+                parts = max(1, min(8, 296 // (-(-m // 64) * -(-e // 64)), -(-k // 64) // 8)) if many else 1
+                need = 8 * parts * m * e + 4 * parts * (m + e if many else m * e)
+                assert need <= 8 * a.value <= need + 4 * parts * m * e + 8, (m, e, k)
+                assert b.value >= -(-m // 16)
