@@ -11,7 +11,8 @@
 //   * The finishing warp picks the top k keys; chosen experts whose key another one's may meet within
 //     those errors, those others, and logits that left fp32's range are summed again in fp64 by the
 //     whole CTA, and the choice is made again.  For normally distributed operands that is one or
-//     two tokens in a hundred.
+//     two tokens in a hundred.  (Softmax with a choice bias: all logits of such a token, since its
+//     denominator moves two keys of different scores apart.)
 //   * fp32 weights are summed in fp64 outright (S = 0: nothing is summed twice).
 //
 // Fewer than 128 tokens, and fp32 weights (route_kernel): a CTA takes 16 MT tokens x 8 NT experts;
@@ -277,12 +278,14 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
           for (int i = 0; i < 4; ++i) finite = finite && isfinite(unpack_lo<BF16>(r[i])) && isfinite(unpack_hi<BF16>(r[i]));
         }
         if (__all_sync(0xffffffffu, finite)) {
-          // Logits out of range, chosen experts whose key another one's may meet, and those others.
+          // Logits out of range, chosen experts whose key another one's may meet, and those others.  Beside a
+          // bias the softmax's denominator does not cancel between two keys, and every expert is part of it.
+          const bool all = nears && !p.sigmoid && p.choice_bias;
 #pragma unroll
           for (int i = 0; i < PER; ++i)
-            if (lane + 32 * i < p.E && !isfinite(z[i])) again |= 1u << i;
+            if (lane + 32 * i < p.E && (all || !isfinite(z[i]))) again |= 1u << i;
 #pragma unroll 1
-          for (int j = 0; j < p.top; ++j) {
+          for (int j = 0; j < (all ? 0 : p.top); ++j) {
             const double kj = __shfl_sync(0xffffffffu, here, j), rj = __shfl_sync(0xffffffffu, far, j);
             const int cj = __shfl_sync(0xffffffffu, chosen, j);
             bool met = false;

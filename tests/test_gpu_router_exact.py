@@ -1,0 +1,37 @@
+"""The router's ids are those of 64-bit logits where fp32 sums would decide otherwise: operands made so
+that tensor-core sums lose what the choice depends on, alone and within the layer's launch."""
+import pytest
+import torch
+
+from ffn_optim_b200 import prepare_moe_ffn, prepare_router, route_experts
+from tests.layer_reference import route64
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def ids_of(x, w, **kw):
+    """The router's ids, and for up to 256 tokens the layer's, which have to agree."""
+    ids, _ = route_experts(x, w, **kw)
+    if x.shape[0] <= 256:
+        w1 = torch.zeros(w.shape[0], 8, x.shape[1], dtype=x.dtype, device="cuda")
+        layer = prepare_moe_ffn(x, w, w1, w1[:, :, :8].contiguous(), activation="silu", **kw)
+        layer.run()
+        layer.check()
+        assert torch.equal(layer.ids, ids)
+    return ids
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_softmax_denominator_and_choice_bias(m):
+    """Experts 0 and 1 meet by their biases; which leads depends on the softmax's denominator, to which
+    expert 2, whose logit of 1e-6 is lost in fp32 beside 64 - 64, adds and never competes."""
+    x = torch.zeros(m, 512, dtype=BF, device="cuda")
+    x[:, [0, 1, 32]] = 1
+    w = torch.zeros(3, 512, dtype=BF, device="cuda")
+    w[1, 0] = -1.0
+    w[2, 0], w[2, 1], w[2, 32] = 64.0, 1e-6, -64.0
+    bias = torch.tensor([0.0, 0.2669563293, -1.0], device="cuda")
+    want = route64(x, w, 2, "softmax", bias)[0]
+    assert want[0].tolist() == [1, 0]
+    assert torch.equal(ids_of(x, w, top_k=2, choice_bias=bias), want)
