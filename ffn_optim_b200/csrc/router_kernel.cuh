@@ -3,9 +3,12 @@
 // The ids must be those of 64-bit logits, whatever the order of the sums, at the cost of tensor
 // cores rather than of fp64 arithmetic (64 multiply-adds per clock and SM):
 //   * 16-bit weights: products on mma.sync (m16n8k16, fp32 accumulation) in chains of 64 of K; each
-//     chain's fp32 result is added in fp64.  A chain of four MMAs loses at most 4 * 2^-22 of the
-//     sum of its |x w|, so a logit is off by at most 2^-20 S, S = sum |x w|.  For few tokens a
-//     second set of MMAs over the operands with their signs cleared gives S; for many, where that
+//     chain's fp32 result is added in fp64.  An MMA cuts its addends (16 products, the accumulator) off
+//     at 2^-25 of the largest one's power of two, and its result to 24 bits: it loses at most
+//     16 * 2^-25 + 2^-23 = 2.5 * 2^-22 of the sum of their sizes (measured with operands made for
+//     it: 2.25), and a chain of four 10 * 2^-22 (8.2) of the sum of its |x w|.  So a logit is off by at most
+//     2.5 * 2^-20 S, S = sum |x w|.  For few tokens a second set of MMAs over the operands with their
+//     signs cleared gives S (short by the same rule: K / 16 MMAs lose 0.25 % at most); for many, where that
 //     cost most (1000 tokens of 256 experts of 4096: 29 us for the logits), the norms of the two
 //     rows bound it.
 //   * The finishing warp picks the top k keys; chosen experts whose key another one's may meet within
@@ -32,7 +35,7 @@ namespace ffnb200 {
 constexpr int kRouteWarps = 8;
 constexpr int kRouteThreads = 32 * kRouteWarps;
 constexpr int kRouteStep = 64;                 // K per chain
-constexpr double kRouteLoss = 1.0 / (1 << 20); // error of a logit over the sum of its |x w|
+constexpr double kRouteLoss = 2.51 / (1 << 20);  // error of a logit over the sum of its |x w|
 
 struct RouteParams {
   const void* x;

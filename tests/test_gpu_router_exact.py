@@ -35,3 +35,20 @@ def test_softmax_denominator_and_choice_bias(m):
     want = route64(x, w, 2, "softmax", bias)[0]
     assert want[0].tolist() == [1, 0]
     assert torch.equal(ids_of(x, w, top_k=2, choice_bias=bias), want)
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_every_addend_of_a_chain_truncated(m, dtype, scoring):
+    """One product of 1 and 63 of just under 2^-25, which the sum of a chain loses one by one: together
+    1.96 * 2^-20, upwards for one expert and downwards for the other, whose fp32 sum leads by 3 * 2^-20."""
+    x = torch.zeros(m, 512, dtype=dtype, device="cuda")
+    x[:, 0], x[:, 1:64], x[:, 64] = 1.0, 2.0 ** -13, 2.0 ** -10
+    w = torch.zeros(2, 512, dtype=dtype, device="cuda")
+    w[:, 0] = 1.0
+    w[0, 1:64], w[1, 1:64] = -1.9921875 * 2.0 ** -13, 1.9921875 * 2.0 ** -13
+    w[0, 64] = 3 * 2.0 ** -10
+    want = route64(x, w, 2, scoring)[0]
+    assert want[0].tolist() == [1, 0]
+    assert torch.equal(ids_of(x, w, top_k=2, scoring=scoring), want)
