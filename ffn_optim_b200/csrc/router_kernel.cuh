@@ -173,14 +173,9 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
     if (p.many) {  // |x| |w| of the longest w
       float x2 = 0.f;
       for (int c = 0; c < p.parts; ++c) x2 += __ldcg(p.sums + static_cast<size_t>(c) * (p.M + p.E) + t);
-      // (The sums of squares are fp32.  Below 2^-100 squares may be missing: such a token's logits, unless
-      // all are zero, are summed again.)
-      const bool small = x2 < 0x1p-100f || s < 0x1p-100f;
-      s = sqrtf(x2) * sqrtf(s) * 1.001f;
-      bool some = false;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) some |= lane + 32 * i < p.E && z[i] != 0.0;
-      if (small && __any_sync(0xffffffffu, some)) s = INFINITY;
+      // (The sums of squares are fp32, and zero only of zeros.  Below 2^-100 squares may be missing: such a
+      // token's logits are summed again.)
+      s = x2 == 0.f || s == 0.f ? 0.f : x2 < 0x1p-100f || s < 0x1p-100f ? INFINITY : sqrtf(x2) * sqrtf(s) * 1.001f;
     }
     loss = p.weight_f32 ? 0.0 : kRouteLoss * static_cast<double>(s);
   }
@@ -540,8 +535,10 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
   // Squares of the rows this warp has in hand anyway: tokens in the first column of tiles, experts in the first row.
   const bool x_norm = blockIdx.x == 0 && warp < 2, w_norm = blockIdx.y == 0 && (warp & 1) == 0;
   float x2[4] = {}, w2[2] = {};
-  auto squares = [](const uint4& v, float s) {
+  uint32_t xb[4] = {}, wb[2] = {};  // the bits that their values have set: squares of small ones vanish
+  auto squares = [](const uint4& v, float s, uint32_t& bits) {
     const uint32_t r[4] = {v.x, v.y, v.z, v.w};
+    bits |= (v.x | v.y | v.z | v.w) & 0x7FFF7FFFu;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       s = fmaf(unpack_lo<BF16>(r[i]), unpack_lo<BF16>(r[i]), s);
@@ -577,11 +574,11 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
           }
         if (x_norm) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x2[i] = squares(xv[i], x2[i]);
+          for (int i = 0; i < 4; ++i) x2[i] = squares(xv[i], x2[i], xb[i]);
         }
         if (w_norm) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) w2[j] = squares(wv[j], w2[j]);
+          for (int j = 0; j < 2; ++j) w2[j] = squares(wv[j], w2[j], wb[j]);
         }
       }
 #pragma unroll
@@ -602,20 +599,21 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
         const int t = t0 + m0 + 16 * i + 8 * (v / 2) + g, e = e0 + n0 + 8 * j + 2 * q + v % 2;
         if (t < p.M && e < p.E) p.logits[part + static_cast<size_t>(t) * p.E + e] = z[i][j][v];
       }
-  // A row's squares lie with the four lanes of its group.
+  // A row's squares lie with the four lanes of its group; 2^-120 stands for those of a row whose all vanished.
   float* norms = p.sums + static_cast<size_t>(blockIdx.z) * (p.M + p.E);
-  auto put = [&](float s, int at, int end, float* to) {
+  auto put = [&](float s, uint32_t bits, int at, int end, float* to) {
+    if (bits && s < 0x1p-120f) s = 0x1p-120f;
     s += __shfl_xor_sync(0xffffffffu, s, 1);
     s += __shfl_xor_sync(0xffffffffu, s, 2);
     if (q == 0 && at < end) to[at] = s;
   };
   if (x_norm) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) put(x2[i], t0 + m0 + 8 * i + g, p.M, norms);
+    for (int i = 0; i < 4; ++i) put(x2[i], xb[i], t0 + m0 + 8 * i + g, p.M, norms);
   }
   if (w_norm) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) put(w2[j], e0 + n0 + 8 * j + g, p.E, norms + p.M);
+    for (int j = 0; j < 2; ++j) put(w2[j], wb[j], e0 + n0 + 8 * j + g, p.E, norms + p.M);
   }
 }
 

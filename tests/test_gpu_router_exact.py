@@ -52,3 +52,26 @@ def test_every_addend_of_a_chain_truncated(m, dtype, scoring):
     want = route64(x, w, 2, scoring)[0]
     assert want[0].tolist() == [1, 0]
     assert torch.equal(ids_of(x, w, top_k=2, scoring=scoring), want)
+
+
+@pytest.mark.parametrize("m", [20, 300])
+def test_every_logit_lost_and_squares_below_fp32(m):
+    """x of 2^-80: its squares vanish in fp32, and so does every logit beside 64 - 64."""
+    x = torch.zeros(m, 512, dtype=BF, device="cuda")
+    x[:, [0, 1, 32]] = 2.0 ** -80
+    x[1] = 0  # a token of zeros takes the lowest indices
+    w = torch.zeros(8, 512, dtype=BF, device="cuda")
+    w[:, 0], w[:, 32] = 64.0, -64.0
+    w[:, 1] = 2.0 ** -20 * (1 + torch.arange(8, device="cuda") / 8)
+    w *= 2.0 ** 80
+    want = route64(x, w, 3)[0]
+    assert want[0].tolist() == [7, 6, 5] and want[1].tolist() == [0, 1, 2]
+    assert torch.equal(ids_of(x, w, top_k=3), want)
+
+
+@pytest.mark.parametrize("m", [20, 300])
+@pytest.mark.parametrize("size", [2.0 ** -80, 1.0, 2.0 ** 80])
+def test_weights_of_zeros(m, size):
+    x = torch.full((m, 256), size, dtype=BF, device="cuda")
+    ids = ids_of(x, torch.zeros(70, 256, dtype=BF, device="cuda"), top_k=3)
+    assert torch.equal(ids, torch.arange(3, dtype=torch.int32, device="cuda").expand(m, 3))
