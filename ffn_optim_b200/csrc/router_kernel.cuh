@@ -210,13 +210,13 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
 #pragma unroll
         for (int i = 0; i < PER; ++i) v[i] *= scale;
       }
-      // Keys as integers; 0 ranks below all of them: no expert, or one already chosen.
+      // Keys as integers; 1, NaN, ranks below all numbers, and 0 below that: no expert, or one already chosen.
       unsigned long long key[PER];
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int e = lane + 32 * i;
         const double k = v[i] + bias[i];
-        key[i] = e < p.E ? ordered(k == k ? k : -INFINITY) : 0ull;
+        key[i] = e < p.E ? (k == k ? ordered(k) : 1ull) : 0ull;
         if (e < p.E) q[e] = v[i];
       }
       __syncwarp();

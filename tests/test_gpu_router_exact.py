@@ -75,3 +75,18 @@ def test_weights_of_zeros(m, size):
     x = torch.full((m, 256), size, dtype=BF, device="cuda")
     ids = ids_of(x, torch.zeros(70, 256, dtype=BF, device="cuda"), top_k=3)
     assert torch.equal(ids, torch.arange(3, dtype=torch.int32, device="cuda").expand(m, 3))
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_nan_keys_rank_below_forbidden_experts(m):
+    """A bias of -inf forbids an expert; one whose key is NaN ranks below even that."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = (torch.randn(n, 128, generator=g, device="cuda").to(BF) for n in (m, 6))
+    w[1, 5] = float("nan")
+    bias = torch.zeros(6, device="cuda")
+    bias[4] = -float("inf")
+    ids = ids_of(x, w, top_k=6, scoring="sigmoid", choice_bias=bias)
+    assert (ids[:, 4] == 4).all() and (ids[:, 5] == 1).all()
+    keep = [0, 2, 3, 5]
+    want = torch.tensor(keep, dtype=torch.int32, device="cuda")[route64(x, w[keep], 4, "sigmoid")[0].long()]
+    assert torch.equal(ids[:, :4], want)
