@@ -266,16 +266,16 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int t, uint8_
       const bool nears = __any_sync(0xffffffffu, close);
       const bool odds = __any_sync(0xffffffffu, odd);
       if (nears || odds) {
-        // A token that is not finite itself keeps what the first sums gave.
-        bool finite = true;
+        // Every logit of a token that holds a NaN is NaN, as the first sums are.
+        bool nan = false;
 #pragma unroll 1
         for (int k = odds ? 8 * lane : p.K; k < p.K; k += 256) {
           const uint4 c = row_chunk(p.x, static_cast<long long>(t) * p.ldx, k, p.K);
           const uint32_t r[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) finite = finite && isfinite(unpack_lo<BF16>(r[i])) && isfinite(unpack_hi<BF16>(r[i]));
+          for (int i = 0; i < 4; ++i) nan = nan || isnan(unpack_lo<BF16>(r[i])) || isnan(unpack_hi<BF16>(r[i]));
         }
-        if (__all_sync(0xffffffffu, finite)) {
+        if (!__any_sync(0xffffffffu, nan)) {
           // Logits out of range, chosen experts whose key another one's may meet, and those others.  Beside a
           // bias the softmax's denominator does not cancel between two keys, and every expert is part of it.
           const bool all = nears && !p.sigmoid && p.choice_bias;

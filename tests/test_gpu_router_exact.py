@@ -90,3 +90,20 @@ def test_nan_keys_rank_below_forbidden_experts(m):
     keep = [0, 2, 3, 5]
     want = torch.tensor(keep, dtype=torch.int32, device="cuda")[route64(x, w[keep], 4, "sigmoid")[0].long()]
     assert torch.equal(ids[:, :4], want)
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_infinite_tokens_and_products_that_leave_fp32(m):
+    """An infinite value beside a product of -1e76: the logit is infinite, though an fp32 sum meets
+    both infinities."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.randn(m, 128, generator=g, device="cuda").abs().to(BF)
+    w = torch.randn(6, 128, generator=g, device="cuda").to(BF)
+    x[0, 3], x[0, 70] = float("inf"), 1e38
+    w[:, 3] = torch.tensor([-1.0, -2.0, 1.0, -1.0, 2.0, float("nan")], device="cuda")
+    w[:, 70] = -w[:, 3].nan_to_num() * 1e38
+    w[:, 70][w[:, 3] < 0] = 1e38
+    want = route64(x, w, 6, "sigmoid")[0]
+    assert want[0].tolist() == [2, 4, 0, 1, 3, 5]
+    got = ids_of(x[:, :], w, top_k=6, scoring="sigmoid")
+    assert torch.equal(got, want)
