@@ -220,7 +220,6 @@ int route_parts(const ffn_b200_router_problem& p) {
 }
 
 int launch_route(RouteFn fn, const ffnb200::RouteParams& P, dim3 grid, int smem, void* stream) {
-  if (grid.y > 65535) return FFN_B200_ERR_TOO_LARGE;
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
@@ -243,7 +242,7 @@ int launch_route(RouteFn fn, const ffnb200::RouteParams& P, dim3 grid, int smem,
 }
 // One kernel of 16 mt x 8 nt tiles; shared memory: the warps' parts of K, then logits and scores.
 int launch_route(RouteFn fn, const ffnb200::RouteParams& P, int mt, int nt, void* stream) {
-  const dim3 grid(static_cast<unsigned>(cdiv(P.E, 8 * nt)), static_cast<unsigned>(cdiv(P.M, 16 * mt)), 1);
+  const dim3 grid(static_cast<unsigned>(cdiv(P.E, 8 * nt) * cdiv(P.M, 16 * mt)), 1, 1);
   return launch_route(fn, P, grid, std::max(ffnb200::kRouteWarps * 128 * mt * nt * 12, ffnb200::route_space<ffnb200::kRouteWarps>(P.E)),
                       stream);
 }
@@ -535,8 +534,8 @@ int ffn_b200_router_run(const ffn_b200_router_problem* pr, const void* x, int64_
   if (pr->m < kRouteMany) return launch_route(pr->weight_f32 ? fns.few32 : fns.few, P, 1, 1, stream);  // small tiles: more CTAs
   if (!route_many(*pr)) return launch_route(fns.many32, P, 2, 4, stream);
   P.many = 1;
-  const dim3 tiles(static_cast<unsigned>(cdiv(P.E, ffnb200::kLogitTile)), static_cast<unsigned>(cdiv(P.M, ffnb200::kLogitTile)),
-                   static_cast<unsigned>(P.parts));
+  const dim3 tiles(static_cast<unsigned>(cdiv(P.E, ffnb200::kLogitTile) * cdiv(P.M, ffnb200::kLogitTile)),
+                   static_cast<unsigned>(P.parts), 1);
   const int rc2 = launch_route(fns.logits, P, tiles, ffnb200::kLogitSmem, stream);
   if (rc2) return rc2;
   return launch_route(fns.choose, P, dim3(static_cast<unsigned>(cdiv(P.M, ffnb200::kRouteWarps)), 1, 1),

@@ -459,15 +459,17 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int last;
   const int warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.y * 16 * MT;
+  // Tiles in one grid dimension, which takes any number of tokens, neighbours with the same tokens.
+  const unsigned groups = (p.E + 8 * NT - 1) / (8 * NT), tile = blockIdx.x / groups, group = blockIdx.x - tile * groups;
+  const int t0 = static_cast<int>(tile) * 16 * MT;
   if (threadIdx.x == 0) grid_dep_launch();
   grid_dep_wait();
-  route_tile<BF16, W32, MT, NT, kRouteWarps>(p, t0, blockIdx.x * 8 * NT, 0, 1, smem);
+  route_tile<BF16, W32, MT, NT, kRouteWarps>(p, t0, static_cast<int>(group) * 8 * NT, 0, 1, smem);
   if (threadIdx.x == 0) {
     unsigned old;  // (releases what the whole CTA wrote: the barrier above)
-    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.counters + blockIdx.y) : "memory");
-    last = old == gridDim.x - 1;
-    if (last) p.counters[blockIdx.y] = 0;  // for the next launch
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.counters + tile) : "memory");
+    last = old == groups - 1;
+    if (last) p.counters[tile] = 0;  // for the next launch
   }
   __syncthreads();
   if (!last) return;
@@ -495,7 +497,8 @@ __device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr) {
   return v;
 }
 
-// Part blockIdx.z of K of a 64 x 64 tile of logits: warps 2 x 4, each 32 tokens x 16 experts (warp 0
+// Part blockIdx.y of K of a 64 x 64 tile of logits (blockIdx.x, as in route_kernel): warps 2 x 4, each 32
+// tokens x 16 experts (warp 0
 // and 1 the first 16 experts, even warps the first 32 tokens).
 template <bool BF16>
 __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const RouteParams p) {
@@ -503,9 +506,10 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
   const uint32_t base = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
-  const int t0 = blockIdx.y * kLogitTile, e0 = blockIdx.x * kLogitTile;
+  const unsigned groups = (p.E + kLogitTile - 1) / kLogitTile, tile = blockIdx.x / groups, group = blockIdx.x - tile * groups;
+  const int t0 = static_cast<int>(tile) * kLogitTile, e0 = static_cast<int>(group) * kLogitTile;
   const int steps = (p.K + kLogitChains * kRouteStep - 1) / (kLogitChains * kRouteStep);
-  const int s0 = steps * blockIdx.z / gridDim.z, s1 = steps * (blockIdx.z + 1) / gridDim.z;
+  const int s0 = steps * blockIdx.y / gridDim.y, s1 = steps * (blockIdx.y + 1) / gridDim.y;
   if (threadIdx.x == 0) grid_dep_launch();
   grid_dep_wait();
   // Thread i copies 16-byte chunk i % 8 of rows i / 8 and i / 8 + 32 of both operands; rows past the
@@ -533,7 +537,7 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
   }
   const int m0 = (warp & 1) * 32, n0 = (warp >> 1) * 16;  // of the tile
   // Squares of the rows this warp has in hand anyway: tokens in the first column of tiles, experts in the first row.
-  const bool x_norm = blockIdx.x == 0 && warp < 2, w_norm = blockIdx.y == 0 && (warp & 1) == 0;
+  const bool x_norm = group == 0 && warp < 2, w_norm = tile == 0 && (warp & 1) == 0;
   float x2[4] = {}, w2[2] = {};
   uint32_t xb[4] = {}, wb[2] = {};  // the bits that their values have set: squares of small ones vanish
   auto squares = [](const uint4& v, float s, uint32_t& bits) {
@@ -589,7 +593,7 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
           for (int v = 0; v < 4; ++v) z[i][j][v] += static_cast<double>(d[i][j][v]);
     }
   }
-  const size_t part = static_cast<size_t>(blockIdx.z) * p.M * p.E;
+  const size_t part = static_cast<size_t>(blockIdx.y) * p.M * p.E;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -600,7 +604,7 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
         if (t < p.M && e < p.E) p.logits[part + static_cast<size_t>(t) * p.E + e] = z[i][j][v];
       }
   // A row's squares lie with the four lanes of its group; 2^-120 stands for those of a row whose all vanished.
-  float* norms = p.sums + static_cast<size_t>(blockIdx.z) * (p.M + p.E);
+  float* norms = p.sums + static_cast<size_t>(blockIdx.y) * (p.M + p.E);
   auto put = [&](float s, uint32_t bits, int at, int end, float* to) {
     if (bits && s < 0x1p-120f) s = 0x1p-120f;
     s += __shfl_xor_sync(0xffffffffu, s, 1);

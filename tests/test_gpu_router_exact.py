@@ -107,3 +107,12 @@ def test_infinite_tokens_and_products_that_leave_fp32(m):
     assert want[0].tolist() == [2, 4, 0, 1, 3, 5]
     got = ids_of(x[:, :], w, top_k=6, scoring="sigmoid")
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,f32", [(64 * 65535 + 1, False), (32 * 65535 + 1, True)])
+def test_more_rows_of_tiles_than_a_grid_dimension(m, f32):
+    """More than 65535 tiles of tokens."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(m, 8, generator=g, device="cuda").to(BF)
+    w = torch.randn(3, 8, generator=g, device="cuda").to(torch.float32 if f32 else BF)
+    assert torch.equal(route_experts(x, w, top_k=2)[0], route64(x, w, 2)[0])
