@@ -498,8 +498,7 @@ __device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr) {
 }
 
 // Part blockIdx.y of K of a 64 x 64 tile of logits (blockIdx.x, as in route_kernel): warps 2 x 4, each 32
-// tokens x 16 experts (warp 0
-// and 1 the first 16 experts, even warps the first 32 tokens).
+// tokens x 16 experts (warps 0 and 1 the first 16 experts, even warps the first 32 tokens).
 template <bool BF16>
 __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const RouteParams p) {
   extern __shared__ __align__(16) uint8_t smem[];

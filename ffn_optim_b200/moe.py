@@ -238,6 +238,7 @@ class PreparedMoE(L.PreparedLayer):
         elsewhere, a padded token); an id given twice counts with the sum of its weights."""
         self._check_stream()
         for t, name, dtype in ((ids, "ids", self._torch.int32), (weights, "weights", self._torch.float32)):
+            L.check_tensor(t, name)
             if t.shape != self._choice_shape or t.dtype != dtype or t.device != self.device:
                 raise ValueError(f"{name} must be a {list(self._choice_shape)} tensor of {dtype} on {self.device}")
         ids, weights = ids.contiguous(), weights.contiguous()
