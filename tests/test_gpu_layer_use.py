@@ -3,8 +3,9 @@ choices, waits that run out, captured two-kernel routing, bad values in weights 
 import pytest
 import torch
 
-from ffn_optim_b200 import prepare_moe_ffn
-from tests.test_gpu_moe import BF, make
+from ffn_optim_b200 import linear, prepare_moe_ffn, prepare_router
+from tests.layer_reference import assert_within, linear64
+from tests.test_gpu_moe import BF, check_route, make
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +25,68 @@ def test_given_choices_without_autograd():
         p.run_routed(ids.to_sparse(), wt)
     assert torch.isfinite(p.run_routed(ids, wt)).all()
     p.check()
+
+
+@pytest.mark.parametrize("m", [1, 16, 100])
+def test_a_wait_that_runs_out_is_reported(m):
+    """The hook makes the wait for hidden rows unsatisfiable: the status is that of a wait between CTAs (2, or
+    3 where a CTA with no share of the second product began to wait for the others first)."""
+    x, wr, w1, w2, r = make(m, 512, 256, 512, 8, BF, "swiglu")
+    p = prepare_moe_ffn(x, wr, w1, w2, top_k=2, residual=r)
+    want = p.run().clone()
+    p.check()
+    p.set_wait_limit(0.05)
+    p.set_fault_injection(1)
+    for again in range(2):
+        p.run()
+        assert p.status()[0] in (2, 3)
+        with pytest.raises(RuntimeError, match="MoE kernel failed"):
+            p.check()
+        assert p.status() == [0, 0, 0, 0]
+    p.set_fault_injection(0)
+    p.set_wait_limit(2.0)
+    for _ in range(2):
+        assert torch.equal(p.run(), want)
+        p.check()
+
+
+@pytest.mark.parametrize("m", [127, 128, 129, 300])
+@pytest.mark.parametrize("e,top", [(1, 1), (64, 6), (300, 8)])
+def test_router_captured_on_both_sides_of_its_two_kernels(m, e, top):
+    g = torch.Generator(device="cuda").manual_seed(m + e)
+    xs = [torch.randn(m, 520, generator=g, device="cuda").to(BF) for _ in range(3)]
+    w = (torch.randn(e, 520, generator=g, device="cuda") * 520 ** -0.5).to(BF)
+    buf = xs[0].clone()
+    p = prepare_router(buf, w, top_k=top)
+    graph = p.capture_graph(runs=3)
+    for x in xs:
+        buf.copy_(x)
+        graph.replay()
+        ids, wt = p._ids.clone(), p._weights.clone()
+        check_route((ids, wt), x, w, top_k=top)
+        assert all(torch.equal(a, b) for a, b in zip(p.run(x), (ids, wt)))
+    del graph
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 256])
+def test_bad_values_in_weights_that_nobody_chose(m):
+    """NaN and infinity in the experts beside the chosen ones reach nothing."""
+    e = 8
+    x, wr, w1, w2, r = make(m, 200, 136, 264, e, BF, "swiglu")
+    bias = torch.zeros(e, device="cuda")
+    bias[[0, 3, 7]] = -float("inf")
+    kw = dict(top_k=2, residual=r, choice_bias=bias)
+    want = prepare_moe_ffn(x, wr, w1, w2, **kw).run().clone()
+    for i, v in ((0, "nan"), (3, "inf"), (7, "-inf")):
+        w1[i], w2[i] = float(v), float(v)
+    p = prepare_moe_ffn(x, wr, w1, w2, **kw)
+    assert torch.equal(p.run(), want) and torch.isfinite(want).all()
+    p.check()
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (5, 1, 1), (5, 1, 130), (128, 2, 3), (129, 1, 1), (300, 1, 70), (300, 3, 8)])
+def test_projection_of_one_feature(m, k, n):
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    x, w, b, r = (torch.randn(s, generator=g, device="cuda").to(BF) for s in ((m, k), (n, k), (n,), (m, n)))
+    ref, bound = linear64(x, w, b, r, "none", "erf")
+    assert_within(linear(x, w, bias=b, residual=r), ref, bound, BF)
