@@ -24,6 +24,7 @@ int64_t pitch_of(int64_t cols) { return (cols + 7) / 8 * 8; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool bad_rows(const void* p, int64_t ld, int64_t cols) { return !aligned16(p) || ld % 8 != 0 || ld < cols; }
 constexpr int64_t kMaxDim = 65535;
+constexpr uint64_t kMaxWaitNs = 3600ull * 1000000000ull;  // an hour: a negative number taken for an unsigned one is refused
 
 // Makes `device` current for one call and puts the caller's device back.
 struct DeviceScope {
@@ -730,7 +731,7 @@ int ffn_b200_moe_reset(ffn_b200_moe* h, void* stream) {
 }
 
 int ffn_b200_moe_set_wait_limit(ffn_b200_moe* h, uint64_t ns) {
-  if (!h || ns == 0) return FFN_B200_ERR_INVALID;
+  if (!h || ns == 0 || ns > kMaxWaitNs) return FFN_B200_ERR_INVALID;
   h->params.wait_limit_ns = ns;
   return FFN_B200_OK;
 }

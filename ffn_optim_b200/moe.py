@@ -251,7 +251,7 @@ class PreparedMoE(L.PreparedLayer):
         return _lib.load().ffn_b200_moe_reset(self.handle, stream)
 
     def set_wait_limit(self, seconds: float):
-        """Upper bound of every in-kernel wait; on expiry the kernel reports an error."""
+        """Upper bound of every in-kernel wait, an hour at most; on expiry the kernel reports an error."""
         rc = _lib.load().ffn_b200_moe_set_wait_limit(self.handle, int(seconds * 1e9))
         if rc != _lib.OK:
             raise ValueError(f"set_wait_limit: {_lib.strerror(rc)}")

@@ -460,7 +460,7 @@ FFN_B200_EXPORT int ffn_b200_moe_run_routed(ffn_b200_moe* handle, const void* x,
                                             int64_t ldy, void* stream);
 /* Clears counters and status; call after a run reported a kernel error. */
 FFN_B200_EXPORT int ffn_b200_moe_reset(ffn_b200_moe* handle, void* stream);
-/* Bounded waits and the test hook that makes one run out, as for ffn_b200_handle. */
+/* Bounded waits (1 ns to 1 h) and the test hook that makes one run out, as for ffn_b200_handle. */
 FFN_B200_EXPORT int ffn_b200_moe_set_wait_limit(ffn_b200_moe* handle, uint64_t nanoseconds);
 FFN_B200_EXPORT int ffn_b200_moe_set_fault_injection(ffn_b200_moe* handle, int mode);
 FFN_B200_EXPORT int ffn_b200_moe_destroy(ffn_b200_moe* handle);

@@ -90,3 +90,13 @@ def test_projection_of_one_feature(m, k, n):
     x, w, b, r = (torch.randn(s, generator=g, device="cuda").to(BF) for s in ((m, k), (n, k), (n,), (m, n)))
     ref, bound = linear64(x, w, b, r, "none", "erf")
     assert_within(linear(x, w, bias=b, residual=r), ref, bound, BF)
+
+
+@pytest.mark.parametrize("seconds", [0, -1.0, -1e-9, 3601])
+def test_wait_limits_that_bound_nothing_are_refused(seconds):
+    x, wr, w1, w2, r = make(4, 64, 64, 64, 4, BF, "swiglu")
+    p = prepare_moe_ffn(x, wr, w1, w2, top_k=2, residual=r)
+    with pytest.raises(ValueError, match="set_wait_limit"):
+        p.set_wait_limit(seconds)
+    p.run()
+    p.check()
