@@ -26,6 +26,9 @@ HEADERS = [CSRC / "ffn_kernel.cuh", CSRC / "ffn_rowblock.cuh", CSRC / "ffn_hslic
            CSRC / "pack_kernel.cuh",
            CSRC / "stream_kernel.cuh", CSRC / "router_kernel.cuh", ROOT / "include" / "ffn_b200.h"]
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
+# -fvisibility=hidden keeps the template kernels private; the extern "C" API is exported
+# through the FFN_B200_EXPORT default-visibility attribute in the header.
+FLAGS = [ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 
 
 def nvcc() -> str:
@@ -36,7 +39,7 @@ def nvcc() -> str:
 
 
 def source_digest() -> str:
-    h = hashlib.sha256()
+    h = hashlib.sha256(" ".join(FLAGS).encode())
     for path in SOURCES + HEADERS:
         h.update(path.read_bytes())
     return h.hexdigest()
@@ -60,23 +63,27 @@ def _included(path: Path, seen: set) -> set:
 
 
 def _compile(source: Path, force: bool, verbose: bool) -> Path:
-    """The object file of one source, compiled if it or a file it includes changed."""
+    """The object file of one source, compiled if it, a file it includes, the flags or the compiler changed."""
     obj = LIBDIR / (source.stem + ".o")
     stamp = LIBDIR / (source.stem + ".o.sha256")
-    h = hashlib.sha256()
+    version = subprocess.run([nvcc(), "--version"], capture_output=True, text=True).stdout
+    h = hashlib.sha256(" ".join(FLAGS + [version]).encode())
     for path in sorted(_included(source.resolve(), set())):
         h.update(path.read_bytes())
     digest = h.hexdigest()
     if not force and obj.exists() and stamp.exists() and stamp.read_text().strip() == digest:
         return obj
-    # -fvisibility=hidden keeps the template kernels private; the extern "C" API is exported
-    # through the FFN_B200_EXPORT default-visibility attribute in the header.
-    cmd = [nvcc(), ARCH, "-O3", "-lineinfo", "-std=c++17", "-c", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "-Xptxas", "-v" if verbose else "-O3",
-           "-I", str(ROOT / "include"), "-o", str(obj), str(source)]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+    tmp = obj.with_suffix(f".{os.getpid()}.tmp")  # (an interrupted compilation must not pass for the object)
+    cmd = [nvcc(), *FLAGS, "-c", "-Xptxas", "-v" if verbose else "-O3", "-I", str(ROOT / "include"), "-o", str(tmp),
+           str(source)]
+    try:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+        stamp.unlink(missing_ok=True)  # never beside an object of other sources
+        tmp.replace(obj)
+    finally:
+        tmp.unlink(missing_ok=True)
     if verbose:
         sys.stderr.write(res.stdout + res.stderr)
     stamp.write_text(digest + "\n")
@@ -95,6 +102,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+    stamp_path().unlink(missing_ok=True)
     tmp.replace(LIB)
     stamp_path().write_text(source_digest() + "\n")
     return LIB
