@@ -491,6 +491,8 @@ int ffn_b200_linear_run(ffn_b200_linear* h, const void* x, int64_t ldx, const vo
 
 int ffn_b200_linear_reset(ffn_b200_linear* h, void* stream) {
   if (!h) return FFN_B200_ERR_INVALID;
+  DeviceScope scope(h->device);  // (a null stream is the current device's)
+  if (!scope.ok) return FFN_B200_ERR_DEVICE;
   if (cudaMemsetAsync(h->status, 0, 4 * h->plan.status_words, static_cast<cudaStream_t>(stream)) == cudaSuccess)
     return FFN_B200_OK;
   cudaGetLastError();
@@ -721,6 +723,8 @@ int ffn_b200_moe_run_routed(ffn_b200_moe* h, const void* x, int64_t ldx, const i
 
 int ffn_b200_moe_reset(ffn_b200_moe* h, void* stream) {
   if (!h) return FFN_B200_ERR_INVALID;
+  DeviceScope scope(h->device);
+  if (!scope.ok) return FFN_B200_ERR_DEVICE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cudaMemsetAsync(h->buf.counters, 0, 4 * h->plan.counter_words, st) != cudaSuccess ||
       cudaMemsetAsync(h->buf.status, 0, 4 * h->plan.status_words, st) != cudaSuccess) {

@@ -204,7 +204,10 @@ class PreparedLayer:
         """Clears the kernel's counters and status."""
         from .. import _lib
 
-        rc = _lib.OK if self._status is None else self._reset(self._stream_ptr)
+        if self._status is None:
+            return
+        with self._torch.cuda.device(self.device):
+            rc = self._reset(self._stream_ptr)
         if rc != _lib.OK:
             raise RuntimeError(f"{type(self).__name__}.reset: {_lib.strerror(rc)}")
 

@@ -213,3 +213,31 @@ def test_router_scratch_holds_what_the_kernels_index(lib, f32):
                 need = 8 * parts * m * e + 4 * parts * (m + e if many else m * e)
                 assert need <= 8 * a.value <= need + 4 * parts * m * e + 8, (m, e, k)
                 assert b.value >= -(-m // 16)
+
+
+class FakeTorch:
+    """Stands in for torch on a machine with several devices: `current` is the device that calls go to."""
+
+    class cuda:
+        current = "cuda:0"
+
+        class device:
+            def __init__(self, device):
+                self.device = device
+
+            def __enter__(self):
+                self.before, FakeTorch.cuda.current = FakeTorch.cuda.current, self.device
+
+            def __exit__(self, *exc):
+                FakeTorch.cuda.current = self.before
+
+
+def test_reset_happens_on_the_operators_device():
+    """A null stream is the current device's: counters cleared with another device current would be cleared
+    in that device's order."""
+    layer = L.PreparedLayer()
+    layer._torch, layer.device, layer._stream_ptr, layer._status = FakeTorch, "cuda:1", 0, object()
+    seen = []
+    layer._reset = lambda stream: seen.append((FakeTorch.cuda.current, stream)) or _lib.OK
+    layer.reset()
+    assert seen == [("cuda:1", 0)] and FakeTorch.cuda.current == "cuda:0"
