@@ -216,7 +216,8 @@ class PreparedLayer:
 
         ``graph.replay()`` on the preparation stream then re-runs them: each reads the tensors
         given at preparation (fill them in place) and writes the output view.  Replays and eager
-        runs may alternate; like runs, they must not overlap each other."""
+        runs may alternate; like runs, they must not overlap each other.  The graph keeps the operator
+        and its buffers."""
         torch = self._torch
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.device(self.device):
@@ -226,4 +227,5 @@ class PreparedLayer:
                 for _ in range(runs):
                     self._capture(side.cuda_stream)
             self.stream.wait_stream(side)
+        graph.operator = self
         return graph

@@ -1,9 +1,12 @@
 """Uses of the projection, the router and the layer that the tests of their results do not make: refused
 choices, waits that run out, captured two-kernel routing, bad values in weights that nobody chose."""
+import gc
+import weakref
+
 import pytest
 import torch
 
-from ffn_optim_b200 import linear, prepare_moe_ffn, prepare_router
+from ffn_optim_b200 import linear, prepare_linear, prepare_moe_ffn, prepare_router
 from tests.layer_reference import assert_within, linear64
 from tests.test_gpu_moe import BF, check_route, make
 
@@ -100,3 +103,34 @@ def test_wait_limits_that_bound_nothing_are_refused(seconds):
         p.set_wait_limit(seconds)
     p.run()
     p.check()
+
+
+@pytest.mark.parametrize("kind", ["linear", "packed linear", "router", "moe"])
+def test_a_graph_keeps_what_it_writes(kind):
+    """A graph whose operator nobody else holds replays into the operator's own memory; the operator goes
+    with the graph."""
+    x, wr, w1, w2, r = make(40, 96, 64, 80, 8, BF, "swiglu")
+    w = torch.randn(80, 96, device="cuda").to(BF)
+
+    def prepare():
+        if kind == "router":
+            return prepare_router(x, wr, top_k=2)
+        if kind == "moe":
+            return prepare_moe_ffn(x, wr, w1, w2, top_k=2, residual=r)
+        return prepare_linear(x.t().contiguous().t() if kind == "packed linear" else x, w, residual=r)
+
+    want = [t.clone() for t in (lambda y: y if isinstance(y, tuple) else (y,))(prepare().run())]
+    p = prepare()
+    graph, gone = p.capture_graph(), weakref.ref(p)
+    outs = (p._ids, p._weights) if kind == "router" else (p._view,)
+    del p
+    gc.collect()
+    assert gone() is not None
+    junk = [torch.full((n,), 7.0, device="cuda") for n in (64, 1024, 4096, 16384, 65536) for _ in range(20)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    assert all((j == 7.0).all() for j in junk)
+    del graph
+    gc.collect()
+    assert gone() is None
