@@ -172,9 +172,12 @@ class PreparedMoE(L.PreparedLayer):
         L.raise_for(lib.ffn_b200_moe_prepare(ctypes.byref(prob), ctypes.byref(bufs), x.device.index or 0,
                                              ctypes.byref(handle)), "prepare_moe_ffn")
         self.handle = handle
-        with torch.cuda.device(x.device):
-            self._logits = torch.empty(plan.route_doubles, dtype=torch.float64, device=x.device)
-        r = self.router
+        r = self.router  # (its scratch serves both: they run on one stream)
+        if r._logits.numel() < plan.route_doubles:
+            with torch.cuda.device(x.device):
+                r._logits = torch.empty(plan.route_doubles, dtype=torch.float64, device=x.device)
+            r._outs = (*r._outs[:2], r._logits.data_ptr(), r._outs[3])
+        self._logits = r._logits
         L.raise_for(lib.ffn_b200_moe_set_router(handle, ctypes.byref(r.problem), *r._fixed, self._logits.data_ptr()),
                     "prepare_moe_ffn")
         self._choices = r._outs[:2]

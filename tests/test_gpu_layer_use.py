@@ -134,3 +134,18 @@ def test_a_graph_keeps_what_it_writes(kind):
     del graph
     gc.collect()
     assert gone() is None
+
+
+@pytest.mark.parametrize("m", [1, 100, 256])
+def test_the_layers_router_runs_beside_it(m):
+    """The layer and its router share one scratch; run in turn, each gives what it gives alone."""
+    x, wr, w1, w2, r = make(m, 1032, 64, 80, 60, BF, "swiglu")
+    p = prepare_moe_ffn(x, wr, w1, w2, top_k=4, residual=r)
+    assert p.router._logits is p._logits
+    want = p.run().clone()
+    choice = p.ids.clone(), p.weights.clone()
+    for _ in range(3):
+        check_route(p.router.run(), x, wr, top_k=4)
+        assert torch.equal(p.run(), want)
+        assert torch.equal(p.ids, choice[0]) and torch.equal(p.weights, choice[1])
+    p.check()
