@@ -1,4 +1,4 @@
-// Expert router: logits = X . W^T, scores, top-k and weights in one launch.
+// Expert router: logits = X . W^T, scores, top-k and weights, in one kernel for few tokens and in two for many.
 //
 // The ids must be those of 64-bit logits, whatever the order of the sums, at the cost of tensor
 // cores rather than of fp64 arithmetic (64 multiply-adds per clock and SM):
@@ -13,8 +13,8 @@
 //     rows bound it.
 //   * The finishing warp picks the top k keys; chosen experts whose key another one's may meet within
 //     those errors, those others, and logits that left fp32's range are summed again in fp64 by the
-//     whole CTA, and the choice is made again.  For normally distributed operands that is one or
-//     two tokens in a hundred.  (Softmax with a choice bias: all logits of such a token, since its
+//     whole CTA, and the choice is made again.  For normally distributed operands that is less
+//     than one token in a hundred of 64 experts, two to five of 256 in the many-token form.  (Softmax with a choice bias: all logits of such a token, since its
 //     denominator moves two keys of different scores apart.)
 //   * fp32 weights are summed in fp64 outright (S = 0: nothing is summed twice).
 //

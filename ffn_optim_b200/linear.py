@@ -22,7 +22,7 @@ def activation_code(activation, gelu, allowed):
 
 class PreparedLinear(L.PreparedLayer):
     """A prepared dense projection.  ``plan`` is the C planner's choice; :meth:`run` launches one
-    kernel and returns the output viewed as ``(*x.shape[:-1], N)``."""
+    kernel (before it copies of operands that cannot be read in place) and returns the output viewed as ``(*x.shape[:-1], N)``."""
 
     def __init__(self, x, weight, bias, residual, activation, gelu, block_num, tile):
         import torch
@@ -88,7 +88,7 @@ class PreparedLinear(L.PreparedLayer):
         self._launch(stream, self.x, self.residual)
 
     def run(self, x=None, residual=None):
-        """One launch; ``x`` and ``residual`` default to the tensors given at preparation and keep
+        """Asynchronous; ``x`` and ``residual`` default to the tensors given at preparation and keep
         their shape, dtype and device.  They are read in place when their rows are 16-byte
         addressable, else copied first.  A residual can only be given if one was prepared."""
         if residual is not None and self.residual is None:
@@ -120,7 +120,12 @@ def prepare_linear(x, weight, *, bias=None, residual=None, activation="none", ge
     [..., N], all of x's dtype on one B200.  ``activation`` is 'none', 'gelu' (``gelu='rational'``
     or ``'erf'``, as in ``prepare_ffn``) or 'silu'.  Sums, bias, activation and residual are fp32;
     the output is rounded once.  ``block_num`` limits the CTA count (default: all SMs); ``tile``
-    forces a tile family (None: automatic)."""
+    forces a tile family (None: automatic).
+
+    Every run reads ``weight`` and ``bias`` anew, so that updates in place are seen, unless preparation
+    had to copy them: a weight whose rows are not 16-byte addressable (a K that is no multiple of 8,
+    a transposed view), a bias that is not contiguous and 16-byte aligned.  Prepare again after
+    updating such a one."""
     return PreparedLinear(x, weight, bias, residual, activation, gelu, block_num, tile)
 
 

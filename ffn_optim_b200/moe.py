@@ -18,8 +18,9 @@ SCORINGS = ("softmax", "sigmoid")
 
 
 class PreparedRouter(L.PreparedLayer):
-    """A prepared router.  :meth:`run` launches one kernel and returns ``(ids, weights)``: int32
-    and fp32 ``(*x.shape[:-1], top_k)``, the choices in descending order of their key."""
+    """A prepared router.  :meth:`run` launches one kernel (two from 128 tokens on with 16-bit weights;
+    before them a copy of an ``x`` that cannot be read in place) and returns ``(ids, weights)``: int32 and
+    fp32 ``(*x.shape[:-1], top_k)``, the choices in descending order of their key."""
 
     def __init__(self, x, weight, top_k, scoring, choice_bias, renormalize, scale, mask):
         import torch
@@ -88,7 +89,7 @@ class PreparedRouter(L.PreparedLayer):
         self._launch(stream, self.x, self.mask)
 
     def run(self, x=None, mask=None):
-        """One launch; ``x`` and ``mask`` default to the tensors given at preparation.  A mask can
+        """Asynchronous; ``x`` and ``mask`` default to the tensors given at preparation.  A mask can
         be given whether or not one was prepared."""
         self._check_stream()
         self._launch(self._stream_ptr, self.x if x is None else x, self.mask if mask is None else mask)
@@ -102,8 +103,13 @@ def prepare_router(x, weight, *, top_k, scoring="softmax", choice_bias=None, ren
     ``sigmoid`` of the logits; the ``top_k`` experts of the largest score (+ ``choice_bias``, fp32
     [E], which takes no part in the weights) are chosen, equal keys by the lower index, a NaN key
     after every other.  ``weights`` are their scores, divided by their sum if ``renormalize``,
-    times ``scale``.  The ids are those of 64-bit logits, the weights have fp32 accuracy.  Tokens
-    whose ``mask`` (bool, x's leading shape) is False get ids -1 and weights 0."""
+    times ``scale``.  The ids are those of 64-bit logits.  The weights come from logits of tensor-core sums
+    (off by 2.5 * 2^-20 of ``sum |x w|`` at most; exact sums for fp32 weights and where a choice was
+    close).  Tokens whose ``mask`` (bool, x's leading shape) is False get ids -1 and weights 0.
+
+    Every run reads ``weight`` and ``choice_bias`` anew, so that updates in place are seen, unless
+    preparation had to copy them: a weight whose rows are not 16-byte addressable, a bias that is
+    not contiguous.  Prepare again after updating such a one."""
     return PreparedRouter(x, weight, top_k, scoring, choice_bias, renormalize, scale, mask)
 
 
@@ -114,8 +120,8 @@ def route_experts(x, weight, **configuration):
 
 class PreparedMoE(L.PreparedLayer):
     """A prepared mixture-of-experts layer.  :meth:`run` routes and computes in one launch,
-    :meth:`run_routed` computes with given choices; both return the output viewed as
-    ``(*x.shape[:-1], N)``.  ``ids`` and ``weights`` hold the choices of the last :meth:`run`."""
+    :meth:`run_routed` computes with given choices (copies of operands that cannot be read in
+    place go before them); both return the output viewed as ``(*x.shape[:-1], N)``.  ``ids`` and ``weights`` hold the choices of the last :meth:`run`."""
 
     def __init__(self, x, router_weight, weight1, weight2, activation, gelu, residual, block_num, routing):
         import torch
@@ -290,7 +296,9 @@ def prepare_moe_ffn(x, router_weight, weight1, weight2, *, top_k, activation="sw
 
     with ``ids`` and ``w`` as :func:`prepare_router` defines them (``top_k``, ``scoring``,
     ``choice_bias``, ``renormalize``, ``scale``, ``mask``).  The hidden values are rounded once to
-    the dtype, as in ``ffn``; sums are fp32 in a fixed order, so results repeat bit for bit."""
+    the dtype, as in ``ffn``; sums are fp32 in a fixed order, so results repeat bit for bit.  Weights are
+    read anew by every run or copied at preparation, as :func:`prepare_router` says; K and H that
+    are multiples of 8 avoid the copy."""
     routing = dict(top_k=top_k, scoring=scoring, choice_bias=choice_bias, renormalize=renormalize, scale=scale, mask=mask)
     return PreparedMoE(x, router_weight, weight1, weight2, activation, gelu, residual, block_num, routing)
 

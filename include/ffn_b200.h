@@ -372,8 +372,8 @@ FFN_B200_EXPORT int ffn_b200_linear_destroy(ffn_b200_linear* handle);
  *     p = softmax(X . W^T) or sigmoid(X . W^T);  ids = the top_k experts by p + choice_bias;
  *     weights = p[ids] (divided by their sum when `renormalize`) * scale
  * The ids are those of 64-bit logits (sums whose error could decide a choice are taken again in
- * fp64); the weights have fp32 accuracy.  Equal keys go to the lower index, a NaN key ranks below
- * every other.  A token whose mask byte is 0 gets ids -1 and weights 0. */
+ * fp64).  The weights come from logits that are off by 2.5 * 2^-20 of sum |x w| at most (fp32 W: exact
+ * sums).  Equal keys go to the lower index, a NaN key ranks below every other.  A token whose mask byte is 0 gets ids -1 and weights 0. */
 typedef struct {
   int64_t m, k;
   int32_t experts;     /* at most FFN_B200_MAX_EXPERTS */
@@ -392,7 +392,8 @@ typedef struct {
 /* Scratch of one run: fp64 logits (with their error bounds) and u32 counters (zeroed before the first run). */
 FFN_B200_EXPORT int ffn_b200_router_scratch(const ffn_b200_router_problem* problem, int64_t* logit_doubles,
                                             int64_t* counter_words);
-/* One asynchronous launch on `stream` of the current device.  choice_bias (fp32 [experts]) and
+/* Asynchronous on `stream` of the current device: one kernel, or two from 128 tokens on with 16-bit W.
+ * Runs that share scratch must be serialised on one stream.  choice_bias (fp32 [experts]) and
  * mask (u8 [M]) may be NULL; ids int32 [M, top_k], weights fp32 [M, top_k]. */
 FFN_B200_EXPORT int ffn_b200_router_run(const ffn_b200_router_problem* problem, const void* x, int64_t ldx,
                                         const void* w, int64_t ldw, const float* choice_bias, const uint8_t* mask,

@@ -6,7 +6,7 @@ import weakref
 import pytest
 import torch
 
-from ffn_optim_b200 import linear, prepare_linear, prepare_moe_ffn, prepare_router
+from ffn_optim_b200 import linear, moe_ffn, prepare_linear, prepare_moe_ffn, prepare_router, route_experts
 from tests.layer_reference import assert_within, linear64
 from tests.test_gpu_moe import BF, check_route, make
 
@@ -149,3 +149,20 @@ def test_the_layers_router_runs_beside_it(m):
         assert torch.equal(p.run(), want)
         assert torch.equal(p.ids, choice[0]) and torch.equal(p.weights, choice[1])
     p.check()
+
+
+@pytest.mark.parametrize("k", [64, 60])
+def test_weights_updated_in_place(k):
+    """Read anew by every run where their rows can be addressed, a copy of the preparation's values else."""
+    x, wr, w1, w2, r = make(9, k, 64, 72, 4, BF, "swiglu")
+    w = torch.randn(72, k, device="cuda").to(BF)
+    ops = [prepare_linear(x, w), prepare_router(x, wr, top_k=2), prepare_moe_ffn(x, wr, w1, w2, top_k=2)]
+    before = [[t.clone() for t in (y if isinstance(y, tuple) else (y,))] for y in (op.run() for op in ops)]
+    for t in (w, wr, w1):
+        t.neg_()
+    after = [linear(x, w).clone(), route_experts(x, wr, top_k=2), moe_ffn(x, wr, w1, w2, top_k=2)]
+    for op, old, new in zip(ops, before, after):
+        got = op.run()
+        want = new if k % 8 == 0 else old
+        for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, (tuple, list)) else (want,)):
+            assert torch.equal(a, b)
