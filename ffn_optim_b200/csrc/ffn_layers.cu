@@ -107,7 +107,8 @@ int encode_rows(CUtensorMap* tm, const void* base, int dtype, int64_t cols, int6
 constexpr int kMaxSmem = 232448;
 // Tokens up to which the experts' first product gathers its token rows itself (a gather of four rows
 // takes the TMA about 200 clocks, so a step's weights hide three); above, they are copied into
-// the pairs' order first.
+// the pairs' order first.  Gathered / copied, us: 16 tokens of K 2048, 6 of 64 experts 116 / 121, of K 4096, 4 of
+// 32 214 / 227; 20 tokens 135 / 125 and 249 / 248; 32 tokens 140 / 141 and 261 / 259.
 constexpr int64_t kMoeGather = 16;
 
 // Token columns of a tile: a multiple of the MMA's 16, at most 128.
@@ -210,7 +211,10 @@ const RouteFns kRouteFns[3][2] = {{route_fns<false, 2>(), route_fns<true, 2>()},
                                   {route_fns<false, 8>(), route_fns<true, 8>()},
                                   {route_fns<false, 16>(), route_fns<true, 16>()}};
 
-// Tokens from which the router runs as two kernels (16-bit weights), and the parts of K of its first.
+// Tokens from which the router runs as two kernels (16-bit weights), and the parts of K of its first.  One / two
+// kernels, us: 64 experts of K 2048 at 64 tokens 16.1 / 15.1, 128 18.5 / 17.9, 256 18.9 / 17.9; 256 experts of K 4096
+// 64: 37 / 24, 128: 37 / 31, 512: 78 / 34; 8 experts of K 1000 128: 9.9 / 14.2, 512: 9.9 / 15.9.  (So many
+// experts would gain from two kernels sooner, and a few lose by them.)
 constexpr int64_t kRouteMany = 128;
 bool route_many(const ffn_b200_router_problem& p) { return p.m >= kRouteMany && !p.weight_f32; }
 int route_parts(const ffn_b200_router_problem& p) {
@@ -313,8 +317,19 @@ struct ffn_b200_moe {
 };
 
 // ---- dense projection ----------------------------------------------------------------------
+// Measured on 148 SMs, us.  Streaming kernel (tokens are its MMAs' columns, 128 at most) / 64- and 128-column tiles:
+//   rows   K 4096, N 4096     K 4096, N 16384    K 2048, N 512      K 1024, N 8192
+//     16   10.8 / 12.1 13.4   26.0 / 29.3 27.4    6.8 / 7.0 8.4      7.2 / 10.3 11.0
+//     32   12.3 / 12.2 13.4   27.4 / 29.6 27.5    8.0 / 6.7 8.4      8.5 /  9.7 10.7
+//     64   16.6 / 12.3 13.5   30.2 / 30.0 27.9   10.5 / 6.7 8.4     10.9 /  7.4  9.9
+//    128   25.2 / 12.5 13.7   37.1 / 30.7 28.6   17.1 / 6.7 8.5     16.1 /  7.6 10.1
+// so the streaming kernel up to 32 rows.
+// Pairs of CTAs / 128 columns: K 4096 with 64, 72, 80 tiles of 256 x 256 27.7 / 31.6, 28.5 / 32.8, 44.8 / 40.1 (six
+// tiles of a second wave), K 2048 with 128 28.3 / 32.5; many tiles of 8, 7, 4 K steps 19.1 / 19.4, 18.6 / 18.2, 15.8 / 13.1.
+// 128 / 64 columns, K 2048: 64, 72, 80, 96 tiles of 128 x 128 10.9 / 9.0, 11.1 / 9.0, 11.1 / 13.4, 11.1 / 13.6.
+constexpr int64_t kLinearStream = 32;
 static int linear_tile(const ffn_b200_linear_problem& p, int grid) {
-  if (p.m <= 128) return FFN_B200_LINEAR_STREAM;
+  if (p.m <= kLinearStream) return FFN_B200_LINEAR_STREAM;
   const int64_t pairs = cdiv(p.m, 256) * cdiv(p.n, 256), steps = cdiv(p.k, 64);
   if (grid >= 2 && pairs >= grid / 2 && steps >= 8) return FFN_B200_LINEAR_PAIR256;
   return cdiv(p.m, 128) * cdiv(p.n, 128) >= grid / 2 ? FFN_B200_LINEAR_CTA128 : FFN_B200_LINEAR_CTA64;

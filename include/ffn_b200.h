@@ -347,7 +347,7 @@ typedef struct {
 } ffn_b200_linear_plan;
 
 /* Tile families: the weight rows dealt out over all CTAs (M <= 128), 256x256 by a CTA pair, 128x128
- * and 128x64 by one CTA (for few tiles clusters split K). */
+ * and 128x64 by one CTA (for few tiles clusters split K).  Chosen automatically: the first up to 32 rows. */
 typedef enum {
   FFN_B200_LINEAR_STREAM = 1, FFN_B200_LINEAR_PAIR256 = 2, FFN_B200_LINEAR_CTA128 = 3, FFN_B200_LINEAR_CTA64 = 4
 } ffn_b200_linear_tile;

@@ -241,3 +241,15 @@ def test_reset_happens_on_the_operators_device():
     layer._reset = lambda stream: seen.append((FakeTorch.cuda.current, stream)) or _lib.OK
     layer.reset()
     assert seen == [("cuda:1", 0)] and FakeTorch.cuda.current == "cuda:0"
+
+
+def test_projection_streams_up_to_32_rows(lib):
+    """The streaming kernel up to where it measured faster than the tiles; up to 128 rows where asked for."""
+    plan = _lib.LinearPlan()
+    for m in (1, 16, 31, 32, 33, 64, 128, 129):
+        for k, n in ((512, 512), (4096, 4096), (4096, 16384)):
+            for tile, want in ((0, m <= 32), (_lib.LINEAR_TILES["stream"], m <= 128)):
+                prob = _lib.LinearProblem(m, k, n, 1, 4, 0, 148, tile, 0)
+                rc = lib.ffn_b200_linear_make_plan(ctypes.byref(prob), ctypes.byref(plan))
+                assert rc == (_lib.OK if want or not tile else _lib.ERR_INVALID)
+                assert rc or (plan.tile == _lib.LINEAR_TILES["stream"]) == want, (m, k, n, tile)
