@@ -14,8 +14,9 @@
 //   * The finishing warp picks the top k keys; chosen experts whose key another one's may meet within
 //     those errors, those others, and logits that left fp32's range are summed again in fp64 by the
 //     whole CTA, and the choice is made again.  For normally distributed operands that is less
-//     than one token in a hundred of 64 experts, two to five of 256 in the many-token form.  (Softmax with a choice bias: all logits of such a token, since its
-//     denominator moves two keys of different scores apart.)
+//     than one token in a hundred of 64 experts, two to five of 256 in the many-token form.
+//     (Softmax with a choice bias: all logits of such a token, since its denominator moves two keys
+//     of different scores apart.)
 //   * fp32 weights are summed in fp64 outright (S = 0: nothing is summed twice).
 //
 // Fewer than 128 tokens, and fp32 weights (route_kernel): a CTA takes 16 MT tokens x 8 NT experts;
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(kRouteThreads, 2) route_logits_kernel(const Ro
         const int t = t0 + m0 + 16 * i + 8 * (v / 2) + g, e = e0 + n0 + 8 * j + 2 * q + v % 2;
         if (t < p.M && e < p.E) p.logits[part + static_cast<size_t>(t) * p.E + e] = z[i][j][v];
       }
-  // A row's squares lie with the four lanes of its group; 2^-120 stands for those of a row whose all vanished.
+  // A row's squares lie with the four lanes of its group; 2^-120 stands for those that vanished.
   float* norms = p.sums + static_cast<size_t>(blockIdx.y) * (p.M + p.E);
   auto put = [&](float s, uint32_t bits, int at, int end, float* to) {
     if (bits && s < 0x1p-120f) s = 0x1p-120f;

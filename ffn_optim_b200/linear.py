@@ -22,7 +22,8 @@ def activation_code(activation, gelu, allowed):
 
 class PreparedLinear(L.PreparedLayer):
     """A prepared dense projection.  ``plan`` is the C planner's choice; :meth:`run` launches one
-    kernel (before it copies of operands that cannot be read in place) and returns the output viewed as ``(*x.shape[:-1], N)``."""
+    kernel (before it copies of operands that cannot be read in place) and returns the output viewed
+    as ``(*x.shape[:-1], N)``."""
 
     def __init__(self, x, weight, bias, residual, activation, gelu, block_num, tile):
         import torch

@@ -121,7 +121,8 @@ def route_experts(x, weight, **configuration):
 class PreparedMoE(L.PreparedLayer):
     """A prepared mixture-of-experts layer.  :meth:`run` routes and computes in one launch,
     :meth:`run_routed` computes with given choices (copies of operands that cannot be read in
-    place go before them); both return the output viewed as ``(*x.shape[:-1], N)``.  ``ids`` and ``weights`` hold the choices of the last :meth:`run`."""
+    place go before them); both return the output viewed as ``(*x.shape[:-1], N)``.  ``ids`` and
+    ``weights`` hold the choices of the last :meth:`run`."""
 
     def __init__(self, x, router_weight, weight1, weight2, activation, gelu, residual, block_num, routing):
         import torch

@@ -373,7 +373,8 @@ FFN_B200_EXPORT int ffn_b200_linear_destroy(ffn_b200_linear* handle);
  *     weights = p[ids] (divided by their sum when `renormalize`) * scale
  * The ids are those of 64-bit logits (sums whose error could decide a choice are taken again in
  * fp64).  The weights come from logits that are off by 2.5 * 2^-20 of sum |x w| at most (fp32 W: exact
- * sums).  Equal keys go to the lower index, a NaN key ranks below every other.  A token whose mask byte is 0 gets ids -1 and weights 0. */
+ * sums).  Equal keys go to the lower index, a NaN key ranks below every other.  A token whose mask
+ * byte is 0 gets ids -1 and weights 0. */
 typedef struct {
   int64_t m, k;
   int32_t experts;     /* at most FFN_B200_MAX_EXPERTS */
